@@ -74,10 +74,10 @@ def collection_rotation_signs(schema: str, field: str, dimension: int, index_typ
 
 def build(reference: str | None = None) -> None:
     """Compile the restatement and, when `reference` (else the XVEC_REFERENCE
-    environment variable) names an existing reference checkout, its C kernels."""
+    environment variable) names a reference checkout that holds them, its C kernels."""
     subprocess.run(["make", "-s", "-C", HERE], check=True)
     reference = reference or os.environ.get("XVEC_REFERENCE")
-    if reference and os.path.isdir(reference):
+    if reference and os.path.isdir(os.path.join(reference, "internal", "floats", "src")):
         subprocess.run(["make", "-s", "-C", HERE, "ref", "REFERENCE=" + reference], check=True)
 
 
