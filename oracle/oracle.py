@@ -77,7 +77,7 @@ def build(reference: str | None = None) -> None:
     environment variable) names a reference checkout that holds them, its C kernels."""
     subprocess.run(["make", "-s", "-C", HERE], check=True)
     reference = reference or os.environ.get("XVEC_REFERENCE")
-    if reference and os.path.isdir(os.path.join(reference, "internal", "floats", "src")):
+    if reference and os.path.isdir(os.path.join(str(reference), "internal", "floats", "src")):
         subprocess.run(["make", "-s", "-C", HERE, "ref", "REFERENCE=" + reference], check=True)
 
 
