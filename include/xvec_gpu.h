@@ -102,10 +102,12 @@ typedef enum {
 
 typedef enum {
   XVEC_STORAGE_FP32 = 1, /* rows and queries are float32 */
-  XVEC_STORAGE_FP16 = 2  /* rows and queries are IEEE binary16 bit patterns (uint16);
+  XVEC_STORAGE_FP16 = 2, /* rows and queries are IEEE binary16 bit patterns (uint16);
                             the arithmetic is float32 on the decoded values, as for a
                             VectorFP16 field (collection.go:4607-4613) or QuantizationFP16
                             (quantization.go:187-191) */
+  XVEC_STORAGE_BF16 = 3  /* bfloat16: the learned adapters and gradient clipping only
+                            (indexes refuse it) */
 } xvec_gpu_storage;
 
 typedef struct xvec_gpu_index xvec_gpu_index;
@@ -548,6 +550,174 @@ xvec_gpu_status xvec_gpu_rotate_device(int32_t device, const uint8_t* signs, int
                                        int32_t dimension, const float* d_vectors, int64_t n,
                                        float* d_out, int32_t inverse, int32_t* d_failed,
                                        void* stream);
+
+/* ---- Learned adapters ----------------------------------------------------
+ * A learned adapter maps embeddings into the space an index searches, before
+ * xvec_gpu_index_add* and xvec_gpu_index_search*: the trained counterpart of
+ * the rotation reformer above (no counterpart in the reference).  Its parts
+ * are an affine layer, a gated block, the gradients of both and the clipping
+ * of all gradients to a global norm.
+ *
+ * Matrices are row-major device memory of one element type (`storage`):
+ * float32, binary16 or bfloat16.  A leading dimension is the distance between
+ * rows in elements; 0 means contiguous rows.  Vectors (bias and its gradient)
+ * are contiguous.  Pointers are aligned to their element; 16-byte aligned
+ * matrices whose rows are a multiple of 16 bytes apart are read in place,
+ * others are first copied into scratch.  Nothing outside the described
+ * elements is read or written.
+ *
+ * Arithmetic: sums, activations and gradients in float32 or more, one rounding
+ * to the storage type for each result.  16-bit storage multiplies its
+ * elements exactly; float32 storage multiplies three bfloat16 parts of each
+ * element (all products above 2^-24 of the whole), so float32 results have
+ * float32 accuracy, but an infinity in a float32 operand may come out as a NaN.
+ * Gradients of pre-activations are rounded to 16 bits in between for 16-bit
+ * storage.  Results do not vary from run to run.
+ *
+ * Every call enqueues on `stream` and does not wait; it can be captured into
+ * a CUDA graph.  Scratch is allocated and freed in stream order.  n = 0 does
+ * nothing in the forward calls and gives zero weight and bias gradients.  An
+ * output may not overlap an input or another output (XVEC_GPU_INVALID_ARGUMENT),
+ * except that y may be the residual itself.  `status` (device int32, may be
+ * NULL) is set to XVEC_GPU_TIMEOUT if a bounded device-side wait ran out (the
+ * outputs are then incomplete) and left alone otherwise. */
+typedef enum {
+  XVEC_ACT_NONE = 0,
+  XVEC_ACT_RELU = 1, /* max(z, 0); derivative 0 at z = 0 */
+  XVEC_ACT_GELU = 2, /* z Phi(z), Phi the standard normal distribution */
+  XVEC_ACT_SILU = 3  /* z / (1 + exp(-z)) */
+} xvec_gpu_activation;
+
+/* y = act(x weight' + bias) + residual.  x [n][in_dim], weight
+ * [out_dim][in_dim], bias [out_dim] or NULL, residual [n][out_dim] or NULL,
+ * y [n][out_dim].  preact [n][out_dim] or NULL receives x weight' + bias, which
+ * the backward call needs for every activation but XVEC_ACT_NONE. */
+typedef struct {
+  int32_t device;
+  int32_t storage;    /* xvec_gpu_storage */
+  int32_t activation; /* xvec_gpu_activation */
+  int32_t in_dim;
+  int32_t out_dim;
+  int32_t reserved;
+  int64_t n;
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* residual;
+  void* y;
+  void* preact;
+  int64_t ldx, ldw, ldr, ldy, ldz; /* ldr: residual, ldz: preact */
+  int32_t* status;
+  void* stream;
+} xvec_gpu_linear_args;
+xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* args);
+
+/* Gradients of xvec_gpu_linear_device: with dz = dy act'(preact),
+ *   dx = dz weight [n][in_dim], dweight = dz' x [out_dim][in_dim],
+ *   dbias = the column sums of dz [out_dim];
+ * the residual's gradient is dy itself.  Each of the three may be NULL (not
+ * wanted); weight may be NULL without dx, x without dweight, preact with
+ * XVEC_ACT_NONE. */
+typedef struct {
+  int32_t device;
+  int32_t storage;
+  int32_t activation;
+  int32_t in_dim;
+  int32_t out_dim;
+  int32_t reserved;
+  int64_t n;
+  const void* dy;
+  const void* x;
+  const void* weight;
+  const void* preact;
+  void* dx;
+  void* dweight;
+  void* dbias;
+  int64_t lddy, ldx, ldw, ldz, lddx, lddw;
+  int32_t* status;
+  void* stream;
+} xvec_gpu_linear_backward_args;
+xvec_gpu_status xvec_gpu_linear_backward_device(const xvec_gpu_linear_backward_args* args);
+
+/* The gated block h = act(x gate_weight' + gate_bias) * (x up_weight' + up_bias):
+ * both products, the activation and the elementwise product in one kernel.
+ * x [n][in_dim], the weights [out_dim][in_dim] (both with ldw), the biases
+ * [out_dim] or NULL, h [n][out_dim].  gate and up [n][out_dim] (both with
+ * ldg; both or neither NULL) receive the two affine results, which the backward
+ * call needs.  xvec_gpu_linear_device brings h back to the index's dimension. */
+typedef struct {
+  int32_t device;
+  int32_t storage;
+  int32_t activation;
+  int32_t in_dim;
+  int32_t out_dim;
+  int32_t reserved;
+  int64_t n;
+  const void* x;
+  const void* gate_weight;
+  const void* up_weight;
+  const void* gate_bias;
+  const void* up_bias;
+  void* h;
+  void* gate;
+  void* up;
+  int64_t ldx, ldw, ldh, ldg;
+  int32_t* status;
+  void* stream;
+} xvec_gpu_gated_args;
+xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args);
+
+/* Gradients of xvec_gpu_gated_device from dh [n][out_dim] and the saved gate
+ * and up: with dg = dh up act'(gate) and du = dh act(gate),
+ *   dx = dg gate_weight + du up_weight, dgate_weight = dg' x,
+ *   dup_weight = du' x (both with lddw), dgate_bias and dup_bias the column sums.
+ * Each output may be NULL; the weights may be NULL without dx, x without a
+ * weight gradient. */
+typedef struct {
+  int32_t device;
+  int32_t storage;
+  int32_t activation;
+  int32_t in_dim;
+  int32_t out_dim;
+  int32_t reserved;
+  int64_t n;
+  const void* dh;
+  const void* x;
+  const void* gate_weight;
+  const void* up_weight;
+  const void* gate;
+  const void* up;
+  void* dx;
+  void* dgate_weight;
+  void* dup_weight;
+  void* dgate_bias;
+  void* dup_bias;
+  int64_t lddh, ldx, ldw, ldg, lddx, lddw;
+  int32_t* status;
+  void* stream;
+} xvec_gpu_gated_backward_args;
+xvec_gpu_status xvec_gpu_gated_backward_device(const xvec_gpu_gated_backward_args* args);
+
+/* Clips gradients to a global norm: norm = the square root of the sum of the
+ * squares of every element of every tensor (summed so that neither overflow
+ * nor underflow of a square matters), and each tensor's out = in * min(1,
+ * max_norm / norm).  out may be in itself, else it may not overlap any input
+ * or output.  Tensors may differ in type; empty ones are allowed.  With an
+ * element that is not finite (the norm then is not), or max_norm = infinity,
+ * out = in unchanged: the caller sees the norm and skips the step.  max_norm
+ * >= 0, not NaN.  d_norm: one
+ * float32 in device memory (infinity where the norm exceeds float32).  `tensors`
+ * is host memory, read before the call returns. */
+typedef struct {
+  const void* in;
+  void* out;
+  int64_t count;
+  int32_t storage;
+  int32_t reserved;
+} xvec_gpu_tensor;
+xvec_gpu_status xvec_gpu_clip_gradients_device(int32_t device, const xvec_gpu_tensor* tensors,
+                                               int32_t num_tensors, double max_norm,
+                                               float* d_norm, void* stream);
 
 /* Counters (the reference's RuntimeStats role, collection.go:5185-5315, for
  * the device path).  Device-time fields are filled only while timing is

@@ -36,7 +36,8 @@ METRIC_L2, METRIC_IP, METRIC_COSINE, METRIC_MIPSL2 = 1, 2, 3, 4
 INDEX_FLAT, INDEX_SQ8_FLAT, INDEX_IVF_PQ, INDEX_RABITQ, INDEX_IVF_FLAT, INDEX_IVF_SQ8 = (
     1, 2, 3, 4, 5, 6)
 INDEX_SQ4_FLAT, INDEX_IVF_SQ4, INDEX_DISKANN = 7, 8, 9
-STORAGE_FP32, STORAGE_FP16 = 1, 2
+STORAGE_FP32, STORAGE_FP16, STORAGE_BF16 = 1, 2, 3  # BF16: the learned adapters only
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 
 STATUS_NAMES = {
     0: "OK", 1: "INVALID_ARGUMENT", 2: "OUT_OF_MEMORY", 3: "CANCELLED", 4: "TIMEOUT",
@@ -66,6 +67,8 @@ EXPORTED_SYMBOLS = (
     "xvec_gpu_set_wait_limit_ns",
     "xvec_gpu_rotation_signs", "xvec_gpu_rotate", "xvec_gpu_rotate_device",
     "xvec_gpu_rabitq_set_graph", "xvec_gpu_diskann_set_model", "xvec_gpu_diskann_set_graph",
+    "xvec_gpu_linear_device", "xvec_gpu_linear_backward_device", "xvec_gpu_gated_device",
+    "xvec_gpu_gated_backward_device", "xvec_gpu_clip_gradients_device",
 )
 
 
@@ -88,6 +91,37 @@ class SearchOpts(ctypes.Structure):
                 ("filter_bitmap", ctypes.c_void_p), ("filter_words", ctypes.c_int64),
                 ("stream", ctypes.c_void_p), ("cancel_flag", ctypes.c_void_p),
                 ("linear", ctypes.c_int32)]
+
+
+def _fields(text: str):
+    """ctypes fields from "type name name ...; ..." with i (int32), l (int64)
+    and p (pointer)."""
+    kinds = {"i": ctypes.c_int32, "l": ctypes.c_int64, "p": ctypes.c_void_p}
+    return [(name, kinds[part.split()[0]]) for part in text.split(";")
+            for name in part.split()[1:]]
+
+
+_SHAPE = "i device storage activation in_dim out_dim reserved; l n; "
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = _fields(_SHAPE + "p x weight bias residual y preact; l ldx ldw ldr ldy ldz; "
+                       "p status stream")
+
+
+class LinearBackwardArgs(ctypes.Structure):
+    _fields_ = _fields(_SHAPE + "p dy x weight preact dx dweight dbias; "
+                       "l lddy ldx ldw ldz lddx lddw; p status stream")
+
+
+class GatedArgs(ctypes.Structure):
+    _fields_ = _fields(_SHAPE + "p x gate_weight up_weight gate_bias up_bias h gate up; "
+                       "l ldx ldw ldh ldg; p status stream")
+
+
+class GatedBackwardArgs(ctypes.Structure):
+    _fields_ = _fields(_SHAPE + "p dh x gate_weight up_weight gate up dx dgate_weight dup_weight "
+                       "dgate_bias dup_bias; l lddh ldx ldw ldg lddx lddw; p status stream")
 
 
 class Stats(ctypes.Structure):
@@ -166,6 +200,10 @@ def _load() -> ctypes.CDLL:
     lib.xvec_gpu_rotation_signs.argtypes = [ctypes.c_char_p, ctypes.c_char_p, i32, i32, i32, vp,
                                             i64]
     lib.xvec_gpu_rotate.argtypes = [i32, vp, i64, i32, vp, i64, vp, i32]
+    for name, args in (("linear", LinearArgs), ("linear_backward", LinearBackwardArgs),
+                       ("gated", GatedArgs), ("gated_backward", GatedBackwardArgs)):
+        getattr(lib, f"xvec_gpu_{name}_device").argtypes = [ctypes.POINTER(args)]
+    lib.xvec_gpu_clip_gradients_device.argtypes = [i32, vp, i32, ctypes.c_double, vp, vp]
     lib.xvec_gpu_rotate_device.argtypes = [i32, vp, i64, i32, vp, i64, vp, i32, vp, vp]
     lib.xvec_gpu_set_wait_limit_ns.restype = i64
     lib.xvec_gpu_set_wait_limit_ns.argtypes = [i64]
@@ -258,6 +296,74 @@ class RotationReformer:
         _check(_lib.xvec_gpu_rotate_device(self.device, self.signs.ctypes.data, self.signs.size,
                                            self.dimension, d_vectors, n, d_out, 1 if inverse else 0,
                                            d_failed, stream or None))
+
+
+def linear_device(device: int, storage: int, n: int, in_dim: int, out_dim: int, x_ptr: int,
+                  weight_ptr: int, y_ptr: int, *, bias_ptr: int = 0, residual_ptr: int = 0,
+                  activation: int = ACT_NONE, preact_ptr: int = 0, ldx: int = 0, ldw: int = 0,
+                  ldr: int = 0, ldy: int = 0, ldz: int = 0, status_ptr: int = 0,
+                  stream: int = 0) -> None:
+    """y = act(x weight' + bias) + residual on device memory (xvec_gpu_linear_device):
+    x [n, in_dim], weight [out_dim, in_dim], y [n, out_dim] of one storage type;
+    preact receives x weight' + bias.  Zero pointers: not given; zero leading
+    dimensions: contiguous."""
+    _check(_lib.xvec_gpu_linear_device(ctypes.byref(LinearArgs(
+        device, storage, activation, in_dim, out_dim, 0, n, x_ptr, weight_ptr, bias_ptr,
+        residual_ptr, y_ptr, preact_ptr, ldx, ldw, ldr, ldy, ldz, status_ptr, stream))))
+
+
+def linear_backward_device(device: int, storage: int, n: int, in_dim: int, out_dim: int,
+                           dy_ptr: int, x_ptr: int, weight_ptr: int, *, preact_ptr: int = 0,
+                           activation: int = ACT_NONE, dx_ptr: int = 0, dw_ptr: int = 0,
+                           db_ptr: int = 0, lddy: int = 0, ldx: int = 0, ldw: int = 0,
+                           ldz: int = 0, lddx: int = 0, lddw: int = 0, status_ptr: int = 0,
+                           stream: int = 0) -> None:
+    """Gradients of linear_device (xvec_gpu_linear_backward_device): dx [n, in_dim],
+    dw [out_dim, in_dim] and db [out_dim], each if its pointer is given, from dy
+    [n, out_dim] and the saved preact (activations other than ACT_NONE)."""
+    _check(_lib.xvec_gpu_linear_backward_device(ctypes.byref(LinearBackwardArgs(
+        device, storage, activation, in_dim, out_dim, 0, n, dy_ptr, x_ptr, weight_ptr, preact_ptr,
+        dx_ptr, dw_ptr, db_ptr, lddy, ldx, ldw, ldz, lddx, lddw, status_ptr, stream))))
+
+
+def gated_device(device: int, storage: int, n: int, in_dim: int, out_dim: int, x_ptr: int,
+                 gate_weight_ptr: int, up_weight_ptr: int, h_ptr: int, *, gate_bias_ptr: int = 0,
+                 up_bias_ptr: int = 0, activation: int = ACT_SILU, gate_ptr: int = 0,
+                 up_ptr: int = 0, ldx: int = 0, ldw: int = 0, ldh: int = 0, ldg: int = 0,
+                 status_ptr: int = 0, stream: int = 0) -> None:
+    """h = act(x gate_weight' + gate_bias) * (x up_weight' + up_bias) on device
+    memory in one kernel (xvec_gpu_gated_device); gate and up receive the two
+    affine results, which gated_backward_device needs."""
+    _check(_lib.xvec_gpu_gated_device(ctypes.byref(GatedArgs(
+        device, storage, activation, in_dim, out_dim, 0, n, x_ptr, gate_weight_ptr, up_weight_ptr,
+        gate_bias_ptr, up_bias_ptr, h_ptr, gate_ptr, up_ptr, ldx, ldw, ldh, ldg, status_ptr,
+        stream))))
+
+
+def gated_backward_device(device: int, storage: int, n: int, in_dim: int, out_dim: int,
+                          dh_ptr: int, x_ptr: int, gate_weight_ptr: int, up_weight_ptr: int,
+                          gate_ptr: int, up_ptr: int, *, activation: int = ACT_SILU,
+                          dx_ptr: int = 0, dgate_weight_ptr: int = 0, dup_weight_ptr: int = 0,
+                          dgate_bias_ptr: int = 0, dup_bias_ptr: int = 0, lddh: int = 0,
+                          ldx: int = 0, ldw: int = 0, ldg: int = 0, lddx: int = 0, lddw: int = 0,
+                          status_ptr: int = 0, stream: int = 0) -> None:
+    """Gradients of gated_device (xvec_gpu_gated_backward_device) from dh and the
+    saved gate and up, each output if its pointer is given."""
+    _check(_lib.xvec_gpu_gated_backward_device(ctypes.byref(GatedBackwardArgs(
+        device, storage, activation, in_dim, out_dim, 0, n, dh_ptr, x_ptr, gate_weight_ptr,
+        up_weight_ptr, gate_ptr, up_ptr, dx_ptr, dgate_weight_ptr, dup_weight_ptr, dgate_bias_ptr,
+        dup_bias_ptr, lddh, ldx, ldw, ldg, lddx, lddw, status_ptr, stream))))
+
+
+def clip_gradients_device(device: int, tensors: Sequence[tuple], max_norm: float, norm_ptr: int,
+                          stream: int = 0) -> None:
+    """Clips gradients to a global norm (xvec_gpu_clip_gradients_device): tensors
+    is a sequence of (storage, in_ptr, out_ptr, count), out_ptr = in_ptr in place;
+    out = in * min(1, max_norm / norm), the float32 norm at norm_ptr."""
+    flat = [v for storage, src, dst, count in tensors for v in (src, dst, count, storage)]
+    table = (ctypes.c_int64 * max(1, len(flat)))(*flat)
+    _check(_lib.xvec_gpu_clip_gradients_device(device, table, len(flat) // 4, max_norm,
+                                               norm_ptr or None, stream or None))
 
 
 def device_count() -> int:
