@@ -587,3 +587,32 @@ def test_train_an_adapter_and_search_with_it(oracle, xb):
     assert np.array_equal(okeys.cpu().numpy().astype(np.uint64), want)
     assert np.array_equal(oscores.cpu().numpy().view(np.uint32), scores.view(np.uint32))
     idx.close()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n", [100, 1500])
+def test_expired_device_wait(xb, kind, n):
+    """A wait bound of 1 ns runs out in the matrix kernel: it sets the status, frees what it holds
+    and returns; afterwards the same call is right and leaves the status alone."""
+    k, m = 512, 384
+    mk = Maker(kind, 6)
+    x, w = mk.matrix(n, k), mk.matrix(m, k, k ** -0.5)
+    y, _ = mk.out(n, m)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def call():
+        xb.linear_device(0, STORAGE[kind], n, k, m, ptr(x), ptr(w), ptr(y), status_ptr=ptr(status),
+                         stream=stream())
+        torch.cuda.synchronize()
+
+    assert xb.set_wait_limit_ns(1) == 2_000_000_000
+    try:
+        call()
+        assert status.item() == 4  # XVEC_GPU_TIMEOUT
+    finally:
+        xb.set_wait_limit_ns(0)
+    status.zero_()
+    call()
+    assert status.item() == 0
+    want = x.double() @ w.double().t()
+    close(y, want, sum_error(x.double(), w.double(), want), "y")

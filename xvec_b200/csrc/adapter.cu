@@ -23,206 +23,257 @@ namespace {
 constexpr int64_t kMaxDim = 1 << 20;
 constexpr int kMaxDevices = 64;
 
-// --- products: one 64 x 64 tile per block, float32 sums in registers ------
-constexpr int kTile = 64, kDepth = 16;
-
+// --- operands -----------------------------------------------------------------
+// Eight elements of a row as floats, from an address that may be unaligned
+// (vec = false) and of which only `count` exist (the rest 0).
 template <typename T>
-struct Operand {
-  const T* p[2];
-  int64_t outer, inner;  // strides of the row (or column) index and of the depth index
-};
-
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256)
-    product_kernel(Product p, Operand<T> a, Operand<T> b, int z_parts) {
-  __shared__ float as[kDepth][kTile + 1], bs[2][kDepth][kTile + 1];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t r0 = (int64_t)blockIdx.x * kTile, c0 = (int64_t)blockIdx.y * kTile;
-  const int z = blockIdx.z;
-  constexpr int kSums = MODE == kGated ? 2 : 1;
-  // Two levels of sums (every 256 terms), so that long ones keep float32 accuracy.
-  float acc[kSums][4][4] = {}, total[kSums][4][4] = {};
-  for (int seg = 0; seg < z_parts; ++seg) {
-    const T* ap = a.p[MODE == kDw ? z : MODE == kDx ? seg : 0];
-    for (int64_t k0 = 0; k0 < p.depth; k0 += kDepth) {
-      for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-        // The faster index follows the operand's contiguous direction.
-        const int kk = a.inner == 1 ? i % kDepth : i / kTile;
-        const int rr = a.inner == 1 ? i / kDepth : i % kTile;
-        const bool in = r0 + rr < p.rows && k0 + kk < p.depth;
-        as[kk][rr] = in ? to_f(ap[(r0 + rr) * a.outer + (k0 + kk) * a.inner]) : 0.f;
-      }
-      for (int s = 0; s < kSums; ++s) {
-        const T* bp = b.p[MODE == kGated ? s : MODE == kDx ? seg : 0];
-        for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-          const int kk = b.inner == 1 ? i % kDepth : i / kTile;
-          const int cc = b.inner == 1 ? i / kDepth : i % kTile;
-          const bool in = c0 + cc < p.cols && k0 + kk < p.depth;
-          bs[s][kk][cc] = in ? to_f(bp[(c0 + cc) * b.outer + (k0 + kk) * b.inner]) : 0.f;
-        }
-      }
-      __syncthreads();
+__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
+  if (vec && count >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0];
+      const float4 b = reinterpret_cast<const float4*>(p)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
-      for (int kk = 0; kk < kDepth; ++kk)
-#pragma unroll
-        for (int s = 0; s < kSums; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[s][i][j] = fmaf(as[kk][ty + 16 * i], bs[s][kk][tx + 16 * j], acc[s][i][j]);
-      __syncthreads();
-      if (k0 % 256 == 256 - kDepth || k0 + kDepth >= p.depth)
-#pragma unroll
-        for (int s = 0; s < kSums; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) total[s][i][j] += acc[s][i][j], acc[s][i][j] = 0.f;
+      for (int j = 0; j < 8; ++j) v[j] = to_f(t[j]);
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_f(p[j]) : 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = r0 + ty + 16 * i, c = c0 + tx + 16 * j;
-      if (r >= p.rows || c >= p.cols) continue;
-      float v = total[0][i][j];
-      if (MODE == kLinear || MODE == kGated) {
-        if (p.bias[0]) v += to_f(static_cast<const T*>(p.bias[0])[c]);
-        if (p.save[0]) static_cast<T*>(p.save[0])[r * p.lds + c] = from_f<T>(v);
-        v = activate(p.act, v);
-      }
-      if constexpr (MODE == kGated) {
-        float u = total[1][i][j];
-        if (p.bias[1]) u += to_f(static_cast<const T*>(p.bias[1])[c]);
-        if (p.save[1]) static_cast<T*>(p.save[1])[r * p.lds + c] = from_f<T>(u);
-        v *= u;
-      }
-      if (MODE == kLinear && p.residual)
-        v += to_f(static_cast<const T*>(p.residual)[r * p.ldr + c]);
-      static_cast<T*>(p.out[MODE == kDw ? z : 0])[r * p.ldo + c] = from_f<T>(v);
-    }
 }
 
-template <typename T, int MODE>
-xvec_gpu_status launch_product(const Product& p, cudaStream_t s) {
-  Operand<T> a{{static_cast<const T*>(p.a[0]), static_cast<const T*>(p.a[1])}, p.lda, 1};
-  Operand<T> b{{static_cast<const T*>(p.b[0]), static_cast<const T*>(p.b[1])}, p.ldb, 1};
-  if (MODE == kDw) std::swap(a.outer, a.inner);
-  if (MODE == kDw || MODE == kDx) std::swap(b.outer, b.inner);
-  const dim3 grid((unsigned)((p.rows + kTile - 1) / kTile), (unsigned)((p.cols + kTile - 1) / kTile),
-                  MODE == kDw ? p.parts : 1);
-  product_kernel<T, MODE><<<grid, 256, 0, s>>>(p, a, b, MODE == kDx ? p.parts : 1);
+// Eight values as operand elements at dst: 16-bit types as they are; float32
+// as three bfloat16 parts x = h + m + l in planes `plane` elements apart, each
+// the nearest to what is left (exact: 8 bits each and the parts' signs).
+template <typename T>
+__device__ __forceinline__ void store_operand(void* dst, int64_t plane, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    __align__(16) T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = from_f<T>(v[j]);
+    *static_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(t);
+  } else {
+    __align__(16) bf16 t[3][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float x = v[j];
+      bf16 h = __float2bfloat16_rn(x);
+      // Next to the largest float32 the nearest bfloat16 is an infinity.
+      if (isinf(to_f(h)) && !isinf(x)) h = __float2bfloat16_rz(x);
+      const bool finite = isfinite(x);
+      x = finite ? x - to_f(h) : 0.f;
+      const bf16 m = __float2bfloat16_rn(x);
+      t[0][j] = h, t[1][j] = m, t[2][j] = __float2bfloat16_rn(x - to_f(m));
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      *reinterpret_cast<uint4*>(static_cast<bf16*>(dst) + i * plane) =
+          *reinterpret_cast<uint4*>(t[i]);
+  }
+}
+
+// src [rows][cols] as an operand: contiguous rows of ld (a multiple of 8)
+// elements, zeros behind the columns.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    pack_kernel(const T* src, int64_t lds, int64_t rows, int cols, bool vec, void* dst, int64_t ld) {
+  const int64_t groups = ld / 8, total = groups * rows;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups;
+    const int c = (int)(i - r * groups) * 8;
+    float v[8];
+    load8(src + r * lds + c, cols - c, vec, v);
+    store_operand<T>(static_cast<uint16_t*>(dst) + r * ld + c, rows * ld, v);
+  }
+}
+
+size_t elem_bytes(int storage) { return storage == XVEC_STORAGE_FP32 ? 4 : 2; }
+bool aligned16(const void* p, int64_t ld, size_t size) {
+  return (uintptr_t)p % 16 == 0 && ld * (int64_t)size % 16 == 0;
+}
+int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
+int planes_of(int storage) { return storage == XVEC_STORAGE_FP32 ? 3 : 1; }
+
+unsigned grid_of(int64_t threads) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 148 * 16));
+}
+
+// The operand for a [rows][cols] matrix: in place where the copies into shared
+// memory can start on 16 bytes, else packed into `room`.
+xvec_gpu_status operand(int storage, const void* p, int64_t rows, int64_t cols, int64_t ld,
+                        Scratch* room, GemmOperand* out, cudaStream_t s) {
+  out->inner = cols, out->outer = rows;
+  if (storage != XVEC_STORAGE_FP32 && aligned16(p, ld, 2)) {
+    out->p = p, out->ld = ld, out->planes = 1;
+    return XVEC_GPU_OK;
+  }
+  out->ld = round8(cols);
+  out->plane = rows * out->ld;
+  out->planes = planes_of(storage);
+  if (xvec_gpu_status st = room->alloc((size_t)out->planes * out->plane * 2, s)) return st;
+  out->p = room->ptr;
+  const unsigned grid = grid_of(rows * out->ld / 8);
+  const bool vec = aligned16(p, ld, elem_bytes(storage));
+  if (storage == XVEC_STORAGE_FP32)
+    pack_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(p), ld, rows, (int)cols, vec,
+                                            room->ptr, out->ld);
+  else  // either 16-bit type: the bits are copied through float and back, exactly but
+        // for the payload of a NaN
+    storage == XVEC_STORAGE_FP16
+        ? pack_kernel<__half><<<grid, 256, 0, s>>>(static_cast<const __half*>(p), ld, rows,
+                                                   (int)cols, vec, room->ptr, out->ld)
+        : pack_kernel<bf16><<<grid, 256, 0, s>>>(static_cast<const bf16*>(p), ld, rows, (int)cols,
+                                                 vec, room->ptr, out->ld);
   XVEC_LAUNCHED();
   XVEC_CUDA(cudaGetLastError());
   return XVEC_GPU_OK;
 }
 
-template <typename T>
-xvec_gpu_status run_product_t(const Product& p, cudaStream_t s) {
-  switch (p.mode) {
-    case kLinear: return launch_product<T, kLinear>(p, s);
-    case kGated: return launch_product<T, kGated>(p, s);
-    case kDx: return launch_product<T, kDx>(p, s);
-    default: return launch_product<T, kDw>(p, s);
-  }
-}
-
-xvec_gpu_status run_product(const Product& p, cudaStream_t s) {
-  if (p.rows == 0 || p.cols == 0) return XVEC_GPU_OK;
-  switch (p.storage) {
-    case XVEC_STORAGE_FP32: return run_product_t<float>(p, s);
-    case XVEC_STORAGE_FP16: return run_product_t<__half>(p, s);
-    default: return run_product_t<bf16>(p, s);
-  }
+xvec_gpu_status gemm(int storage, GemmCall& c, cudaStream_t s) {
+  c.bf16 = storage != XVEC_STORAGE_FP16;
+  c.p.wait_ns = (uint64_t)wait_limit_ns();
+  return storage == XVEC_STORAGE_FP32   ? gemm_fp32(c, s)
+         : storage == XVEC_STORAGE_FP16 ? gemm_fp16(c, s)
+                                        : gemm_bf16(c, s);
 }
 
 // --- pre-activation gradients and their column sums -----------------------
-// dz = dy act'(z), or (GATED) dg = dh u act'(g) and du = dh act(g), rounded to
-// T; partial [2][chunks][m]: the column sums of each row chunk in float32,
-// before the rounding.
+// dz = dy act'(z), or (GATED) dg = dh u act'(g) and du = dh act(g), as operands
+// [2][planes][n][ld] (out may be NULL: column sums only); partial
+// [2][chunks][m]: the column sums of each row chunk in float32, before any
+// rounding.  A block owns 256 columns of a row chunk: 32 threads of 8 columns,
+// 8 rows at a time.  Bound by memory.
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256)
     slope_kernel(const T* dy, int64_t lddy, const T* z, const T* u, int64_t ldz, int64_t n, int m,
-                 int act, int64_t rows_per_chunk, T* out0, T* out1, float* partial) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= m) return;
+                 int act, int vec, int64_t rows_per_chunk, uint16_t* out, int64_t ld,
+                 float* partial) {
+  constexpr int kOuts = GATED ? 2 : 1;
+  constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 256 + tx * 8;
   const int64_t r0 = blockIdx.y * rows_per_chunk;
   const int64_t r1 = min(n, r0 + rows_per_chunk);
-  float s0 = 0.f, s1 = 0.f;
-  for (int64_t r = r0; r < r1; ++r) {
-    const float d = to_f(dy[r * lddy + c]);
-    if (GATED) {
-      const float g = to_f(z[r * ldz + c]), v = to_f(u[r * ldz + c]);
-      const float dg = d * v * slope(act, g), du = d * activate(act, g);
-      out0[r * m + c] = from_f<T>(dg);
-      out1[r * m + c] = from_f<T>(du);
-      s0 += dg;
-      s1 += du;
-    } else {
-      const float v = act == XVEC_ACT_NONE ? d : d * slope(act, to_f(z[r * ldz + c]));
-      out0[r * m + c] = from_f<T>(v);
-      s0 += v;
+  float sum[kOuts][8] = {};
+  if (c < m) {
+    for (int64_t r = r0 + ty; r < r1; r += 8) {
+      float d[kOuts][8];
+      load8(dy + r * lddy + c, m - c, vec & 1, d[0]);
+      if constexpr (GATED) {
+        float g[8], v[8];
+        load8(z + r * ldz + c, m - c, vec & 2, g);
+        load8(u + r * ldz + c, m - c, vec & 4, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          d[1][j] = d[0][j] * activate(act, g[j]);
+          d[0][j] = d[0][j] * v[j] * slope(act, g[j]);
+        }
+      } else if (act != XVEC_ACT_NONE) {
+        float v[8];
+        load8(z + r * ldz + c, m - c, vec & 2, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[0][j] *= slope(act, v[j]);
+      }
+#pragma unroll
+      for (int o = 0; o < kOuts; ++o) {
+        if (out) store_operand<T>(out + (o * kPlanes * n + r) * ld + c, n * ld, d[o]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[o][j] += d[o][j];
+      }
     }
   }
   if (partial) {
-    partial[(int64_t)blockIdx.y * m + c] = s0;
-    if (GATED) partial[((int64_t)gridDim.y + blockIdx.y) * m + c] = s1;
+    __shared__ float part[8][256];
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[ty][tx * 8 + j] = sum[o][j];
+      __syncthreads();
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
+      const int col = blockIdx.x * 256 + threadIdx.x;
+      if (col < m) partial[((int64_t)o * gridDim.y + blockIdx.y) * m + col] = s;
+    }
   }
 }
 
-// out[c] = the sum over the chunks, in their order.
+// out[c] = the sum over the chunks in a fixed order: 8 interleaved runs, then
+// those.
 template <typename T>
 __global__ void __launch_bounds__(256)
     column_sum_kernel(const float* partial, int chunks, int m, T* out0, T* out1) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
   T* out = blockIdx.y ? out1 : out0;
-  if (c >= m || !out) return;
+  if (!out) return;
   const float* p = partial + (int64_t)blockIdx.y * chunks * m + c;
-  double s = 0;
-  for (int i = 0; i < chunks; ++i) s += p[(int64_t)i * m];
-  out[c] = from_f<T>((float)s);
+  float s = 0.f;
+  if (c < m)
+    for (int i = ty; i < chunks; i += 8) s += p[(int64_t)i * m];
+  __shared__ float part[8][33];
+  part[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < m) {
+    for (int i = 1; i < 8; ++i) s += part[i][tx];
+    out[c] = from_f<T>(s);
+  }
 }
 
+// The pre-activation gradients of one backward call.
+struct Slopes {
+  const void *dy, *z, *u;  // u: gated only
+  int64_t lddy, ldz, n;
+  int m, act;
+  void* out;  // NULL: not wanted
+  int64_t ld;
+  void* db[2];
+};
+
 template <typename T>
-xvec_gpu_status slopes_t(const void* dy, int64_t lddy, const void* z, const void* u, int64_t ldz,
-                         int64_t n, int m, int act, void* out0, void* out1, void* db0, void* db1,
-                         cudaStream_t s) {
-  const int chunks = (int)std::max<int64_t>(1, std::min<int64_t>(64, (n + 31) / 32));
-  const int64_t per = (n + chunks - 1) / chunks;
+xvec_gpu_status slopes_t(const Slopes& a, cudaStream_t s) {
+  const int cols = (a.m + 255) / 256;
+  const bool sums = a.db[0] || a.db[1];
+  // About eight blocks per SM, of at least 32 rows.
+  const int64_t chunks =
+      std::max<int64_t>(1, std::min<int64_t>((a.n + 31) / 32, std::max(1, 148 * 8 / cols)));
+  const int64_t per = ((a.n + chunks - 1) / chunks + 7) / 8 * 8;
+  const int used = (int)((a.n + per - 1) / per);
   Scratch partial;
-  xvec_gpu_status st;
-  if (db0 || db1)
-    if ((st = partial.alloc((size_t)2 * chunks * m * 4, s))) return st;
-  const dim3 grid((m + 255) / 256, chunks);
-  auto* kern = u ? slope_kernel<T, true> : slope_kernel<T, false>;
-  kern<<<grid, 256, 0, s>>>(static_cast<const T*>(dy), lddy, static_cast<const T*>(z),
-                            static_cast<const T*>(u), ldz, n, m, act, per,
-                            static_cast<T*>(out0), static_cast<T*>(out1), partial.as<float>());
+  if (sums)
+    if (xvec_gpu_status st = partial.alloc((size_t)2 * used * a.m * 4, s)) return st;
+  const int vec = (aligned16(a.dy, a.lddy, sizeof(T)) ? 1 : 0) |
+                  (aligned16(a.z, a.ldz, sizeof(T)) ? 2 : 0) |
+                  (aligned16(a.u, a.ldz, sizeof(T)) ? 4 : 0);
+  auto* kern = a.u ? slope_kernel<T, true> : slope_kernel<T, false>;
+  kern<<<dim3(cols, used), 256, 0, s>>>(static_cast<const T*>(a.dy), a.lddy,
+                                        static_cast<const T*>(a.z), static_cast<const T*>(a.u),
+                                        a.ldz, a.n, a.m, a.act, vec, per,
+                                        static_cast<uint16_t*>(a.out), a.ld, partial.as<float>());
   XVEC_LAUNCHED();
   XVEC_CUDA(cudaGetLastError());
-  if (db0 || db1) {
-    column_sum_kernel<T><<<dim3((m + 255) / 256, 2), 256, 0, s>>>(
-        partial.as<float>(), chunks, m, static_cast<T*>(db0), static_cast<T*>(db1));
+  if (sums) {
+    column_sum_kernel<T><<<dim3((a.m + 31) / 32, 2), 256, 0, s>>>(
+        partial.as<float>(), used, a.m, static_cast<T*>(a.db[0]), static_cast<T*>(a.db[1]));
     XVEC_LAUNCHED();
     XVEC_CUDA(cudaGetLastError());
   }
   return XVEC_GPU_OK;
 }
 
-xvec_gpu_status slopes(int storage, const void* dy, int64_t lddy, const void* z, const void* u,
-                       int64_t ldz, int64_t n, int m, int act, void* out0, void* out1, void* db0,
-                       void* db1, cudaStream_t s) {
-  auto* f = storage == XVEC_STORAGE_FP32   ? slopes_t<float>
-            : storage == XVEC_STORAGE_FP16 ? slopes_t<__half>
-                                           : slopes_t<bf16>;
-  return f(dy, lddy, z, u, ldz, n, m, act, out0, out1, db0, db1, s);
+xvec_gpu_status slopes(int storage, const Slopes& a, cudaStream_t s) {
+  return storage == XVEC_STORAGE_FP32   ? slopes_t<float>(a, s)
+         : storage == XVEC_STORAGE_FP16 ? slopes_t<__half>(a, s)
+                                        : slopes_t<bf16>(a, s);
 }
 
 // --- argument checks --------------------------------------------------------
-size_t elem_bytes(int storage) { return storage == XVEC_STORAGE_FP32 ? 4 : 2; }
-
 xvec_gpu_status invalid(const char* what) {
   set_error("adapter: %s", what);
   return XVEC_GPU_INVALID_ARGUMENT;
@@ -390,18 +441,26 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   if (a.n == 0) return XVEC_GPU_OK;
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
-  Product p;
-  p.mode = kLinear;
-  p.storage = a.storage;
-  p.rows = a.n, p.cols = a.out_dim, p.depth = a.in_dim;
-  p.a[0] = a.x, p.lda = a.ldx;
-  p.b[0] = a.weight, p.ldb = a.ldw;
+  cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+  GemmCall g;
+  g.mode = kLinear;
+  g.depth = a.in_dim;
+  Scratch room[2];
+  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, s)) ||
+      (st = operand(a.storage, a.weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0], s)))
+    return st;
+  GemmParams& p = g.p;
+  p.rows = a.n, p.cols = a.out_dim, p.segs = p.batches = 1;
   p.bias[0] = a.bias;
   p.residual = a.residual, p.ldr = a.ldr;
   p.out[0] = a.y, p.ldo = a.ldy;
   p.save[0] = a.preact, p.lds = a.ldz;
   p.act = a.activation;
-  return run_product(p, static_cast<cudaStream_t>(a.stream));
+  p.status = a.status;
+  const size_t size = elem_bytes(a.storage);
+  p.vec = aligned16(a.y, a.ldy, size) && aligned16(a.residual, a.ldr, size) &&
+          aligned16(a.preact, a.ldz, size);
+  return gemm(a.storage, g, s);
 }
 
 extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args) {
@@ -428,17 +487,26 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   if (a.n == 0) return XVEC_GPU_OK;
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
-  Product p;
-  p.mode = kGated;
-  p.storage = a.storage;
-  p.rows = a.n, p.cols = a.out_dim, p.depth = a.in_dim;
-  p.a[0] = a.x, p.lda = a.ldx;
-  p.b[0] = a.gate_weight, p.b[1] = a.up_weight, p.ldb = a.ldw;
+  cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+  GemmCall g;
+  g.mode = kGated;
+  g.depth = a.in_dim;
+  Scratch room[3];
+  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, s)) ||
+      (st = operand(a.storage, a.gate_weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0], s)) ||
+      (st = operand(a.storage, a.up_weight, a.out_dim, a.in_dim, a.ldw, &room[2], &g.b[1], s)))
+    return st;
+  GemmParams& p = g.p;
+  p.rows = a.n, p.cols = a.out_dim, p.segs = p.batches = 1;
   p.bias[0] = a.gate_bias, p.bias[1] = a.up_bias;
   p.out[0] = a.h, p.ldo = a.ldh;
   p.save[0] = a.gate, p.save[1] = a.up, p.lds = a.ldg;
   p.act = a.activation;
-  return run_product(p, static_cast<cudaStream_t>(a.stream));
+  p.status = a.status;
+  const size_t size = elem_bytes(a.storage);
+  p.vec = aligned16(a.h, a.ldh, size) && aligned16(a.gate, a.ldg, size) &&
+          aligned16(a.up, a.ldg, size);
+  return gemm(a.storage, g, s);
 }
 
 namespace xvec {
@@ -461,7 +529,6 @@ xvec_gpu_status run_backward(const Backward& b) {
   cudaStream_t s = b.stream;
   const size_t size = elem_bytes(b.storage);
   xvec_gpu_status st;
-  const bool products = b.dx || b.dw[0] || b.dw[1];
   if (b.n == 0) {
     for (int i = 0; i < b.parts; ++i) {
       if (b.dw[i])
@@ -470,36 +537,71 @@ xvec_gpu_status run_backward(const Backward& b) {
     }
     return XVEC_GPU_OK;
   }
-  if (!products && !b.db[0] && !b.db[1]) return XVEC_GPU_OK;
-  Scratch dz[2];
-  for (int i = 0; i < b.parts; ++i)
-    if ((st = dz[i].alloc((size_t)b.n * b.out_dim * size, s))) return st;
-  if ((st = slopes(b.storage, b.dy, b.lddy, b.pre[0], b.parts == 2 ? b.pre[1] : nullptr, b.ldpre,
-                   b.n, b.out_dim, b.act, dz[0].ptr, dz[1].ptr, b.db[0], b.db[1], s)))
-    return st;
+  const bool products = b.dx || b.dw[0] || b.dw[1], sums = b.db[0] || b.db[1];
+  if (!products && !sums) return XVEC_GPU_OK;
+  // The pre-activation gradients as one operand of `parts` matrices.  dy itself
+  // where no activation changes it and it can be read in place.
+  Scratch dz;
+  GemmOperand grad;
+  grad.inner = b.out_dim, grad.outer = b.n;
+  const bool direct = b.parts == 1 && b.act == XVEC_ACT_NONE && size == 2 &&
+                      aligned16(b.dy, b.lddy, size);
+  if (direct) {
+    grad.p = b.dy, grad.ld = b.lddy;
+  } else {
+    grad.ld = round8(b.out_dim);
+    grad.plane = b.n * grad.ld;
+    grad.planes = planes_of(b.storage) * b.parts;
+    if (products) {
+      if ((st = dz.alloc((size_t)grad.planes * grad.plane * 2, s))) return st;
+      grad.p = dz.ptr;
+    }
+  }
+  if (!direct || sums) {
+    Slopes a{};
+    a.dy = b.dy, a.z = b.pre[0], a.u = b.pre[1];
+    a.lddy = b.lddy, a.ldz = b.ldpre, a.n = b.n, a.m = b.out_dim, a.act = b.act;
+    a.out = dz.ptr, a.ld = grad.ld;
+    a.db[0] = b.db[0], a.db[1] = b.db[1];
+    if ((st = slopes(b.storage, a, s))) return st;
+  }
   if (b.dx) {
-    Product p;
-    p.mode = kDx;
-    p.storage = b.storage;
-    p.rows = b.n, p.cols = b.in_dim, p.depth = b.out_dim;
-    p.parts = b.parts;
-    for (int i = 0; i < b.parts; ++i) p.a[i] = dz[i].ptr, p.b[i] = b.w[i];
-    p.lda = b.out_dim, p.ldb = b.ldw;
-    p.out[0] = b.dx, p.ldo = b.lddx;
-    if ((st = run_product(p, s))) return st;
+    GemmCall g;
+    g.mode = kDx;
+    g.depth = b.out_dim;
+    g.a = grad;
+    Scratch room[2];
+    for (int i = 0; i < b.parts; ++i)
+      if ((st = operand(b.storage, b.w[i], b.out_dim, b.in_dim, b.ldw, &room[i], &g.b[i], s)))
+        return st;
+    g.p.rows = b.n, g.p.cols = b.in_dim, g.p.segs = b.parts, g.p.batches = 1;
+    g.p.out[0] = b.dx, g.p.ldo = b.lddx;
+    g.p.vec = aligned16(b.dx, b.lddx, size);
+    g.p.status = b.status;
+    if ((st = gemm(b.storage, g, s))) return st;
   }
   if (b.dw[0] || b.dw[1]) {
-    Product p;
-    p.mode = kDw;
-    p.storage = b.storage;
-    p.rows = b.out_dim, p.cols = b.in_dim, p.depth = b.n;
-    p.parts = 0;
-    for (int i = 0; i < b.parts; ++i)
-      if (b.dw[i]) p.a[p.parts] = dz[i].ptr, p.out[p.parts] = b.dw[i], ++p.parts;
-    p.b[0] = b.x;
-    p.lda = b.out_dim, p.ldb = b.ldx;
-    p.ldo = b.lddw;
-    if ((st = run_product(p, s))) return st;
+    GemmCall g;
+    g.mode = kDw;
+    g.depth = b.n;
+    g.a = grad;
+    Scratch room;
+    if ((st = operand(b.storage, b.x, b.n, b.in_dim, b.ldx, &room, &g.b[0], s))) return st;
+    g.p.rows = b.out_dim, g.p.cols = b.in_dim, g.p.segs = 1;
+    g.p.vec = 1;
+    // Only the second weight's gradient: start at its matrix.
+    const int first = b.dw[0] ? 0 : 1;
+    if (first) {
+      g.a.p = static_cast<const uint16_t*>(grad.p) + planes_of(b.storage) * grad.plane;
+      g.a.planes = planes_of(b.storage);
+    }
+    for (int i = first; i < b.parts && b.dw[i]; ++i) {
+      g.p.out[g.p.batches++] = b.dw[i];
+      g.p.vec &= aligned16(b.dw[i], b.lddw, size);
+    }
+    g.p.ldo = b.lddw;
+    g.p.status = b.status;
+    if ((st = gemm(b.storage, g, s))) return st;
   }
   return XVEC_GPU_OK;
 }

@@ -66,30 +66,55 @@ struct DeviceGuard {
   xvec_gpu_status set(int device);
 };
 
-// What a product does with its sums.
+// A product and what is done with its sums.
 //   kLinear: out = act(A B' + bias) + residual, save = A B' + bias
 //   kGated:  out = act(A B0' + bias0) * (A B1' + bias1), save0 / save1 the two
 //   kDx:     out = A0 B0 (+ A1 B1): gradients of the inputs
 //   kDw:     out0 = A0' B, out1 = A1' B: gradients of the weights
 enum Mode { kLinear = 0, kGated = 1, kDx = 2, kDw = 3 };
 
-// out [rows][cols] of one product, sums over `depth` terms.  a and b are the
-// operands (two where the mode names two); their leading dimensions.
-struct Product {
-  int mode = kLinear;
-  int storage = 0;
-  int64_t rows = 0, cols = 0, depth = 0;
-  int parts = 1;  // kDx: products added; kDw: outputs
-  const void* a[2] = {};
-  const void* b[2] = {};
-  int64_t lda = 0, ldb = 0;
-  const void* bias[2] = {};
-  const void* residual = nullptr;
-  void* out[2] = {};
-  void* save[2] = {};
-  int64_t ldr = 0, ldo = 0, lds = 0;
-  int act = 0;
+// One launch's parameters (adapter_gemm.cuh); the launch fills in the tiling.
+struct GemmParams {
+  int64_t rows, cols;    // of the output
+  int tiles_m, tiles_n;  // tiles of the whole output
+  int blocks;            // depth blocks of one product
+  int segs;              // products added (kDx)
+  int batches;           // outputs (kDw)
+  int splits, blocks_per_split;  // of the segs * blocks depth blocks
+  float* partial;        // splits > 1: [splits][batches or halves][rows][ldp] float sums
+  int64_t ldp;
+  uint32_t idesc;
+  int vec;               // outputs, saves and residual allow 16-byte accesses
+  const void* bias[2];
+  const void* residual;
+  void* out[2];
+  void* save[2];
+  int64_t ldr, ldo, lds;
+  int act;
+  int* status;
+  uint64_t wait_ns;
 };
+
+// An operand in 16-bit elements: [planes][outer][inner], ld elements between
+// rows (16 bytes or a multiple), plane elements between planes.
+struct GemmOperand {
+  const void* p = nullptr;
+  int64_t inner = 0, outer = 0, ld = 0, plane = 0;
+  int planes = 1;
+};
+
+// One product: rows, cols and the epilogue in p, sums over `depth` terms.
+struct GemmCall {
+  int mode = kLinear;
+  bool bf16 = false;  // operands are bfloat16 (else binary16)
+  int64_t depth = 0;
+  GemmOperand a, b[2];
+  GemmParams p{};
+};
+// By the storage type of the outputs; float32: operands are three bfloat16 planes.
+xvec_gpu_status gemm_fp32(const GemmCall& c, cudaStream_t s);
+xvec_gpu_status gemm_fp16(const GemmCall& c, cudaStream_t s);
+xvec_gpu_status gemm_bf16(const GemmCall& c, cudaStream_t s);
 
 }  // namespace adapter
 }  // namespace xvec

@@ -1,0 +1,729 @@
+// adapter_gemm.cuh — the learned adapter's products on the tensor cores.
+//
+// Every product of the adapter is D [rows][cols] = sum over depth of A x B with
+// its own operand order and epilogue (adapter.cuh, Mode):
+//   kLinear  x W'            A and B contiguous along depth
+//   kGated   x Wg', x Wu'    the same, two B's in one tile's two column halves
+//   kDx      dz W            A contiguous along depth, B along the columns
+//   kDw      dz' x           A contiguous along the rows, B along the columns
+// so no operand is ever transposed in memory: the matrix instruction reads
+// either order from shared memory.
+//
+//   CTA = 10 warps, persistent over tiles, one CTA per SM:
+//     warp 0    TMA producer: 64 deep blocks of A (128 rows) and B into a ring of
+//               stages (128-byte swizzle)
+//     warp 1    tensor memory; one thread issues tcgen05.mma (fp32 accumulators,
+//               two of them, so that a tile's epilogue overlaps the next tile)
+//     warps 2-9 epilogue: tcgen05.ld, bias, activation, product, residual
+//   PAIR: two CTAs (cta_group::2) share a tile of 256 rows x BN columns, each
+//   loading half of A's rows and half of B's columns.
+//
+// 16-bit storage multiplies its elements as they are.  float32 storage comes
+// as three bfloat16 planes h + m + l (24 bits, x exactly); a stage holds one
+// plane of A and of B, and the six products hh, hm, mh, mm, hl, lh are issued
+// (what is left out is below 2^-24 of the product).  The accumulator's own
+// additions truncate (measured: 48 of them leave 1.1e-6 of the 2-norm at depth
+// 960), so hh has an accumulator of its own, the five small products another,
+// and both leave tensor memory every kRound blocks to be added in registers
+// (8 truncations of the large sum instead of 48).
+//
+// Every mbarrier wait is bounded; on expiry the kernel sets *status, stops
+// issuing work, drains its own copies and frees its tensor memory.
+#pragma once
+
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "adapter.cuh"
+#include "tcgen05.cuh"
+
+namespace xvec {
+namespace adapter {
+
+constexpr int kBM = 128;      // rows per CTA (TMEM lanes)
+constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
+constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, one per column half
+constexpr int kGemmThreads = 64 + kEpiWarps * 32;
+constexpr uint32_t kABytes = kBM * kBK * 2;
+constexpr int kRound = 2;     // float32: depth blocks per accumulation in tensor memory
+
+template <typename T, bool PAIR, int BN>
+struct GemmShape {
+  // Accumulators of one round: the sums, and for float32 the small products'.
+  static constexpr int kAccCols = std::is_same<T, float>::value ? 2 * BN : BN;
+  static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B columns loaded per CTA
+  static constexpr uint32_t kBBytes = kBRows * kBK * 2;
+  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+  static constexpr uint32_t kBiasBytes = kEpiWarps * 128 * 4;
+  static constexpr int kFit = (int)((232448 - 1024 - 512 - kBiasBytes) / kStageBytes);
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kBiasBytes + 1024 + 512;
+  static constexpr int kTmemCols = 2 * kAccCols;
+  static_assert(kStages >= 4, "shared memory too small for the stage ring");
+};
+
+// --- operand access -------------------------------------------------------------
+// One box of a [plane][outer][inner] operand.  PAIR: it completes on the barrier at
+// the cluster address `bar`, which may belong to the other CTA.
+template <bool PAIR>
+__device__ __forceinline__ void load_box(const CUtensorMap* map, uint32_t bar, void* dst, int x,
+                                         int y, int z) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::smem_u32(dst)),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::smem_u32(dst)),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+// Matrix descriptor of an operand tile in 128-byte swizzle.
+//   along depth (K-major): rows of 128 bytes, 8-row groups 1024 bytes apart;
+//     16 deep = 32 bytes further.
+//   along rows (MN-major): blocks of 64 rows x 64 deep (8 KB, the leading
+//     offset), in a block 8-deep groups 1024 bytes apart; 16 deep = 2048 bytes
+//     further.
+template <bool MN>
+__device__ __forceinline__ uint64_t tile_desc(const void* tile) {
+  const uint64_t addr = tc::smem_u32(tile);
+  const uint64_t lead = MN ? 8192 >> 4 : 1;
+  return ((addr & 0x3FFFFull) >> 4) | (lead << 16) | ((1024ull >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+template <bool MN>
+constexpr uint64_t kDepthStep = MN ? 2048 >> 4 : 32 >> 4;
+
+template <bool PAIR>
+__device__ __forceinline__ void mma_16bit(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t acc) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// --- epilogue rows: 32 consecutive elements of one row ---------------------------
+template <typename T>
+__device__ __forceinline__ void store32(T* p, const float (&v)[32], int count, bool vec) {
+  if (vec && count >= 32) {
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        reinterpret_cast<float4*>(p)[i] =
+            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __align__(16) T t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = from_f<T>(v[8 * i + j]);
+        reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<uint4*>(t);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < count) p[i] = from_f<T>(v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void add32(const T* p, float (&v)[32], int count, bool vec) {
+  if (vec && count >= 32) {
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 t = reinterpret_cast<const float4*>(p)[i];
+        v[4 * i] += t.x, v[4 * i + 1] += t.y, v[4 * i + 2] += t.z, v[4 * i + 3] += t.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+        const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[8 * i + j] += to_f(t[j]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < count) v[i] += to_f(p[i]);
+  }
+}
+
+// --- the kernel ---------------------------------------------------------------
+template <int MODE, typename T, bool PAIR, int BN>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap0,
+                const __grid_constant__ CUtensorMap bmap1, const __grid_constant__ GemmParams p) {
+  using namespace tc;
+  using S = GemmShape<T, PAIR, BN>;
+  constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
+  constexpr int P = std::is_same<T, float>::value ? 3 : 1;  // planes
+  constexpr int kStages = S::kStages;
+  constexpr int kTileRows = PAIR ? 256 : 128;
+  constexpr int kTileCols = MODE == kGated ? BN / 2 : BN;
+  constexpr int kWarpCols = BN / 2;  // accumulator columns per epilogue warp
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  float* bias_all = reinterpret_cast<float*>(tiles + kStages * S::kStageBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * 128);
+  uint64_t* empty = full + kStages;   // the MMAs have read the stage
+  uint64_t* tfull = empty + kStages;  // [2] accumulator ready
+  uint64_t* tempty = tfull + 2;       // [2] accumulator drained (issuing CTA's count)
+  uint64_t* mdone = tempty + 2;       // all issued MMAs retired
+  uint32_t* issued = reinterpret_cast<uint32_t*>(mdone + 1);  // [kStages] copies per stage
+  uint32_t* tmem_slot = issued + kStages;
+  __shared__ int s_abort_storage;
+  volatile int* s_abort = &s_abort_storage;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;
+  const bool issuer = rank == 0;
+  const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+  const int workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int tiles_mn = p.tiles_m * p.tiles_n;
+  const int items = tiles_mn * p.batches * p.splits;
+  const int all_blocks = p.segs * p.blocks;
+  auto fail = [&] {
+    if (p.status) atomicExch(p.status, (int)XVEC_GPU_TIMEOUT);
+    *s_abort = 1;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      issued[s] = 0;
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], (PAIR ? 2 : 1) * kEpiWarps);
+    }
+    mbar_init(mdone, 1);
+    *s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(tmem_slot)),
+                   "n"(S::kTmemCols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(tmem_slot)),
+                   "n"(S::kTmemCols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tmem_fence_before();
+  }
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();
+  tmem_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // Work item -> split, batch, tile (columns fastest: the CTAs running at a
+  // time share A's rows and find B in L2).
+  struct Item {
+    int batch, tm, tn, k0, k1, split;
+  };
+  auto item_of = [&](int i) {
+    Item it;
+    const int t = i % tiles_mn, g = i / tiles_mn;
+    it.batch = g % p.batches;
+    it.split = g / p.batches;
+    it.tm = t / p.tiles_n;
+    it.tn = t % p.tiles_n;
+    it.k0 = it.split * p.blocks_per_split;
+    it.k1 = min(all_blocks, it.k0 + p.blocks_per_split);
+    return it;
+  };
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      const uint32_t full0 = PAIR ? cluster_addr(&full[0], 0) : smem_u32(&full[0]);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t count[kStages];
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) count[s] = 0;
+      for (int i = worker; i < items && !*s_abort; i += workers) {
+        const Item it = item_of(i);
+        const int row0 = it.tm * kTileRows + (int)rank * kBM;
+        const int col0 = it.tn * kTileCols;
+        for (int kb = it.k0; kb < it.k1 && !*s_abort; ++kb) {
+          const int seg = kb / p.blocks;
+          const int k = (kb - seg * p.blocks) * kBK;
+          const int az = (MODE == kDw ? it.batch : MODE == kDx ? seg : 0) * P;
+          const CUtensorMap* bm = (MODE == kDx && seg) ? &bmap1 : &bmap0;
+#pragma unroll 1
+          for (int pl = 0; pl < P; ++pl) {
+            if (!mbar_wait(&empty[stage], phase ^ 1, s_abort, p.wait_ns)) {
+              fail();
+              break;
+            }
+            unsigned char* a = tiles + stage * S::kStageBytes;
+            unsigned char* b = a + kABytes;
+            const uint32_t bar = full0 + stage * 8;
+            if (issuer) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * S::kStageBytes);
+            if constexpr (A_MN) {
+              load_box<PAIR>(&amap, bar, a, row0, k, az + pl);
+              load_box<PAIR>(&amap, bar, a + 8192, row0 + 64, k, az + pl);
+            } else {
+              load_box<PAIR>(&amap, bar, a, k, row0, az + pl);
+            }
+            if constexpr (MODE == kGated) {
+              // Columns of the tile: the gate's half, then the up's half.
+              if constexpr (PAIR) {
+                load_box<PAIR>(rank ? &bmap1 : &bmap0, bar, b, k, col0, pl);
+              } else {
+                load_box<PAIR>(&bmap0, bar, b, k, col0, pl);
+                load_box<PAIR>(&bmap1, bar, b + S::kBBytes / 2, k, col0, pl);
+              }
+            } else if constexpr (B_MN) {
+#pragma unroll
+              for (int c = 0; c < S::kBRows / 64; ++c)
+                load_box<PAIR>(bm, bar, b + c * 8192, col0 + (int)rank * S::kBRows + c * 64, k, pl);
+            } else {
+              load_box<PAIR>(bm, bar, b, k, col0 + (int)rank * S::kBRows, pl);
+            }
+#pragma unroll
+            for (int s = 0; s < kStages; ++s) count[s] += s == stage;
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) issued[s] = count[s];
+    }
+  } else if (warp == 1 && issuer) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      const uint32_t own_empty0 = smem_u32(&empty[0]), own_tfull0 = smem_u32(&tfull[0]);
+      const uint32_t peer_empty0 = PAIR ? cluster_addr(&empty[0], 1) : 0u;
+      const uint32_t peer_tfull0 = PAIR ? cluster_addr(&tfull[0], 1) : 0u;
+      int stage = 0;
+      uint32_t phase = 0, round = 0;
+      // Waits for the stage and moves on; the stage's tile address.
+      auto next = [&](const unsigned char** tile) {
+        const bool ok = mbar_wait(&full[stage], phase, s_abort, p.wait_ns);
+        *tile = tiles + stage * S::kStageBytes;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+        return ok;
+      };
+      auto release = [&](const unsigned char* tile) {
+        const uint32_t s = (uint32_t)(tile - tiles) / S::kStageBytes;
+        mma_commit<PAIR>(own_empty0 + s * 8);
+        if (PAIR) mma_commit<PAIR>(peer_empty0 + s * 8);
+      };
+      for (int i = worker; i < items && !*s_abort; i += workers) {
+        const Item it = item_of(i);
+        const int per = P == 1 ? it.k1 - it.k0 : kRound;
+        for (int r0 = it.k0; r0 < it.k1 && !*s_abort; r0 += per, ++round) {
+          const int acc = round & 1;
+          if (!mbar_wait(&tempty[acc], ((round >> 1) & 1) ^ 1, s_abort, p.wait_ns)) {
+            fail();
+            break;
+          }
+          tmem_fence_after();
+          const uint32_t d = tmem_base + acc * S::kAccCols;
+          const int r1 = min(it.k1, r0 + per);
+          for (int kb = r0; kb < r1; ++kb) {
+            const unsigned char* t[P];
+            bool ok = true;
+            auto multiply = [&](int i, int j, uint32_t d, bool first) {
+              const uint64_t a = tile_desc<A_MN>(t[i]), b = tile_desc<B_MN>(t[j] + kABytes);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_16bit<PAIR>(d, a + k * kDepthStep<A_MN>, b + k * kDepthStep<B_MN>, p.idesc,
+                                (first && k == 0) ? 0u : 1u);
+            };
+#pragma unroll
+            for (int pl = 0; pl < P; ++pl) {
+              if (!(ok = ok && next(&t[pl]))) break;
+              tmem_fence_after();
+              if (pl == 0) multiply(0, 0, d, kb == r0);
+              if constexpr (P == 3) {
+                if (pl == 1) {
+                  multiply(1, 1, d + BN, kb == r0);
+                  multiply(0, 1, d + BN, false);
+                  multiply(1, 0, d + BN, false);
+                }
+                if (pl == 2) multiply(0, 2, d + BN, false), multiply(2, 0, d + BN, false);
+              }
+            }
+            if (!ok) {
+              fail();
+              break;
+            }
+#pragma unroll
+            for (int pl = 0; pl < P; ++pl) release(t[pl]);
+          }
+          mma_commit<PAIR>(own_tfull0 + acc * 8);
+          if (PAIR) mma_commit<PAIR>(peer_tfull0 + acc * 8);
+        }
+      }
+      // Retire every issued MMA before tensor memory is released.
+      mma_commit<PAIR>(smem_u32(mdone));
+      if (!mbar_wait(mdone, 0, nullptr)) fail();
+    }
+  } else if (warp >= 2) {
+    // ---------------- epilogue ----------------
+    const int quarter = warp & 3, ew = warp - 2, half = ew >> 2;
+    float* bias_s = bias_all + ew * 128;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    uint32_t round = 0;
+    auto wait_round = [&] {
+      const bool ok = mbar_wait(&tfull[round & 1], (round >> 1) & 1, s_abort, p.wait_ns);
+      tmem_fence_after();
+      if (!ok) fail();
+      return __all_sync(0xffffffffu, ok);
+    };
+    auto release_round = [&] {
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_remote(cluster_addr(&tempty[round & 1], 0));
+        else mbar_arrive(&tempty[round & 1]);
+      }
+      ++round;
+    };
+    // Accumulator column of chunk c: plain modes take the warp's half from left
+    // to right; the gated mode alternates gate and up of the same outputs.
+    constexpr int kChunks = kWarpCols / 32;
+    auto acc_col = [&](int c) {
+      return MODE == kGated ? (c & 1) * (BN / 2) + half * (BN / 4) + (c >> 1) * 32
+                            : half * kWarpCols + c * 32;
+    };
+    for (int i = worker; i < items; i += workers) {
+      const Item it = item_of(i);
+      const int64_t row = (int64_t)it.tm * kTileRows + rank * kBM + quarter * 32 + lane;
+      const int64_t warp_col =
+          (int64_t)it.tn * kTileCols + half * (MODE == kGated ? BN / 4 : kWarpCols);
+      if constexpr (MODE == kLinear || MODE == kGated) {
+        // The warp's biases: its columns' in order (gated: gate, then up).
+        __syncwarp();
+        constexpr int kBiases = MODE == kGated ? BN / 4 : kWarpCols;
+        for (int c = lane; c < kBiases; c += 32) {
+          const bool in = warp_col + c < p.cols;
+          bias_s[c] = in && p.bias[0] ? to_f(static_cast<const T*>(p.bias[0])[warp_col + c]) : 0.f;
+          if constexpr (MODE == kGated)
+            bias_s[kBiases + c] =
+                in && p.bias[1] ? to_f(static_cast<const T*>(p.bias[1])[warp_col + c]) : 0.f;
+        }
+        __syncwarp();
+      }
+      // Finishes 32 columns (gated: v the gate's, u the up's sums).
+      auto finish = [&](int c, float (&v)[32], float (&u)[32]) {
+        const int64_t col = warp_col + (MODE == kGated ? c >> 1 : c) * 32;
+        if (row >= p.rows || col >= p.cols) return;
+        const int count = (int)min((int64_t)32, p.cols - col);
+        const bool vec = p.vec != 0;
+        if (p.splits > 1) {
+          constexpr int kPlanes = MODE == kGated ? 2 : 1;
+          float* dst = p.partial +
+                       ((int64_t)(it.split * p.batches + it.batch) * kPlanes * p.rows + row) *
+                           p.ldp + col;
+          store32<float>(dst, v, 32, true);
+          if constexpr (MODE == kGated) store32<float>(dst + p.rows * p.ldp, u, 32, true);
+          return;
+        }
+        if constexpr (MODE == kLinear || MODE == kGated) {
+          const float* b = bias_s + (MODE == kGated ? c >> 1 : c) * 32;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += b[j];
+          if (p.save[0]) store32(static_cast<T*>(p.save[0]) + row * p.lds + col, v, count, vec);
+          if constexpr (MODE == kGated) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] += b[BN / 4 + j];
+            if (p.save[1]) store32(static_cast<T*>(p.save[1]) + row * p.lds + col, u, count, vec);
+          }
+          if (p.act != XVEC_ACT_NONE) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = activate(p.act, v[j]);
+          }
+          if constexpr (MODE == kGated) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= u[j];
+          } else if (p.residual) {
+            add32(static_cast<const T*>(p.residual) + row * p.ldr + col, v, count, vec);
+          }
+        }
+        store32(static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row * p.ldo + col, v, count,
+                vec);
+      };
+      constexpr int kStep = MODE == kGated ? 2 : 1;
+      if constexpr (P == 1) {
+        if (!wait_round()) break;
+        const uint32_t t = tmem_base + (round & 1) * S::kAccCols + lanes;
+#pragma unroll 1
+        for (int c = 0; c < kChunks; c += kStep) {
+          uint32_t raw[kStep][32];
+#pragma unroll
+          for (int s = 0; s < kStep; ++s) tmem_ld32(t + acc_col(c + s), raw[s]);
+          tmem_wait_ld();
+          if (c + kStep >= kChunks) release_round();
+          float v[kStep][32];
+#pragma unroll
+          for (int s = 0; s < kStep; ++s)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[s][j] = __uint_as_float(raw[s][j]);
+          finish(c, v[0], v[kStep - 1]);
+        }
+      } else {
+        float sum[kChunks][32];
+        bool ok = true;
+        for (int r0 = it.k0; r0 < it.k1; r0 += kRound) {
+          if (!(ok = wait_round())) break;
+          const uint32_t t = tmem_base + (round & 1) * S::kAccCols + lanes;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t raw[32], small[32];
+            tmem_ld32(t + acc_col(c), raw);
+            tmem_ld32(t + BN + acc_col(c), small);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float v = __uint_as_float(raw[j]) + __uint_as_float(small[j]);
+              sum[c][j] = r0 == it.k0 ? v : sum[c][j] + v;
+            }
+          }
+          release_round();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < kChunks; c += kStep) finish(c, sum[c], sum[c + kStep - 1]);
+      }
+    }
+  }
+
+  __syncthreads();
+  // Drain: every copy either CTA issued has landed before either leaves
+  // (already true unless a role gave up).  The first CTA's barriers count
+  // both CTAs' copies; a stage phase that the second CTA issued but the first
+  // never armed is armed here for its half.
+  if constexpr (PAIR) cluster_sync_all();
+  if (threadIdx.x == 0 && issuer) {
+    for (int s = 0; s < kStages; ++s) {
+      const uint32_t mine = issued[s];
+      const uint32_t other = PAIR ? ld_cluster_u32(cluster_addr(&issued[s], 1)) : mine;
+      // Where the second CTA gave up before the first, its half never comes: the
+      // wait then only gives the first's own copies ample time.
+      if (mine > 0 &&
+          !mbar_wait(&full[s], (mine - 1) & 1, nullptr, other < mine ? 20000000ull : kWaitLimitNs))
+        fail();
+      if (PAIR && other > mine) {
+        mbar_expect_tx(&full[s], S::kStageBytes);
+        if (!mbar_wait(&full[s], mine & 1, nullptr)) fail();
+      }
+    }
+  }
+  if constexpr (PAIR) cluster_sync_all();
+  if (warp == 1) {
+    tmem_fence_after();
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                   "n"(S::kTmemCols));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                   "n"(S::kTmemCols));
+  }
+}
+
+// --- split sums ------------------------------------------------------------------
+// Adds the splits' partial sums in their order and finishes as the kernel would.
+template <int MODE, typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ GemmParams p) {
+  const int64_t groups = (p.cols + 3) / 4;
+  const int64_t total = groups * p.rows;
+  const int batch = blockIdx.y;
+  constexpr int kPlanes = MODE == kGated ? 2 : 1;
+  const int64_t step = (int64_t)p.batches * kPlanes * p.rows * p.ldp;  // between splits
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / groups, col = (i - row * groups) * 4;
+    float v[kPlanes][4] = {};
+#pragma unroll
+    for (int h = 0; h < kPlanes; ++h) {
+      const float* src = p.partial + ((int64_t)(batch * kPlanes + h) * p.rows + row) * p.ldp + col;
+      for (int s = 0; s < p.splits; ++s) {
+        const float4 t = *reinterpret_cast<const float4*>(src + s * step);
+        v[h][0] += t.x, v[h][1] += t.y, v[h][2] += t.z, v[h][3] += t.w;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = col + j;
+      if (c >= p.cols) break;
+      float y = v[0][j];
+      if (MODE == kLinear || MODE == kGated) {
+        if (p.bias[0]) y += to_f(static_cast<const T*>(p.bias[0])[c]);
+        if (p.save[0]) static_cast<T*>(p.save[0])[row * p.lds + c] = from_f<T>(y);
+        y = activate(p.act, y);
+      }
+      if constexpr (MODE == kGated) {
+        float u = v[1][j];
+        if (p.bias[1]) u += to_f(static_cast<const T*>(p.bias[1])[c]);
+        if (p.save[1]) static_cast<T*>(p.save[1])[row * p.lds + c] = from_f<T>(u);
+        y *= u;
+      }
+      if (MODE == kLinear && p.residual) y += to_f(static_cast<const T*>(p.residual)[row * p.ldr + c]);
+      static_cast<T*>(p.out[batch])[row * p.ldo + c] = from_f<T>(y);
+    }
+  }
+}
+
+// --- host side -----------------------------------------------------------------
+inline PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+  static const auto fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// The operand as [planes][outer][inner] 16-bit elements, boxes of [box_outer][64].
+inline bool operand_map(CUtensorMap* map, const GemmOperand& o, int box_outer) {
+  auto fn = encode_tiled();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.outer, (cuuint64_t)o.planes};
+  cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.planes > 1 ? o.plane : o.ld) * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_outer, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(o.p), dims, strides, box,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int MODE, typename T, bool PAIR, int BN>
+xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaStream_t s) {
+  using S = GemmShape<T, PAIR, BN>;
+  constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
+  CUtensorMap a, b0, b1;
+  const int b_box = B_MN ? kBK : (MODE == kGated && !PAIR) ? S::kBRows / 2 : S::kBRows;
+  if (!operand_map(&a, c.a, A_MN ? kBK : kBM) || !operand_map(&b0, c.b[0], b_box) ||
+      !operand_map(&b1, c.b[1].p ? c.b[1] : c.b[0], b_box)) {
+    set_error("adapter: no tensor map for an operand");
+    return XVEC_GPU_CUDA_ERROR;
+  }
+  // Accumulator float32, operands binary16 (0) or bfloat16 (1), their orders, N, M.
+  const uint32_t f = c.bf16 ? 1u : 0u;
+  p.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
+            ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
+  auto kern = gemm_kernel<MODE, T, PAIR, BN>;
+  XVEC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)S::kSmemBytes));
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.batches * p.splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(items, workers) * (PAIR ? 2 : 1));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = S::kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  XVEC_CUDA(cudaLaunchKernelEx(&cfg, kern, a, b0, b1, p));
+  XVEC_LAUNCHED();
+  if (p.splits > 1) {
+    const int64_t groups = (p.cols + 3) / 4 * p.rows;
+    finish_kernel<MODE, T><<<dim3((unsigned)std::min<int64_t>((groups + 255) / 256, 1184),
+                                  (unsigned)p.batches), 256, 0, s>>>(p);
+    XVEC_LAUNCHED();
+    XVEC_CUDA(cudaGetLastError());
+  }
+  return XVEC_GPU_OK;
+}
+
+// Tile shape and depth splits by a cost estimate in SM clocks: a tile's blocks
+// and its start and epilogue, in waves over the SMs; splits pay for their
+// partial sums' traffic and a second launch.
+template <int MODE, typename T>
+xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
+  constexpr bool F32 = std::is_same<T, float>::value;
+  constexpr double kProducts = F32 ? 6 : 1;
+  // Pair tiles: 256 columns, for float32 128 (its sums also live in registers,
+  // and 256 columns of them spill).
+  constexpr int kPairCols = F32 ? 128 : 256;
+  int device = 0, sms = 0;
+  XVEC_CUDA(cudaGetDevice(&device));
+  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  GemmParams p = c.p;
+  p.blocks = (int)((c.depth + kBK - 1) / kBK);
+  const int all = p.blocks * p.segs;
+  p.ldp = (p.cols + 31) / 32 * 32;
+  struct Config {
+    bool pair;
+    int rows, cols, workers;
+    double block;  // clocks per depth block
+  };
+  constexpr int kHalf = MODE == kGated ? 2 : 1;  // accumulator columns per output column
+  const Config configs[] = {{true, 256, kPairCols / kHalf, sms / 2, 2.0 * kPairCols * kProducts},
+                            {false, 128, 128 / kHalf, sms, 400.0 * kProducts}};
+  double best = 0;
+  const Config* pick = nullptr;
+  for (const Config& k : configs) {
+    const int64_t tm = (p.rows + k.rows - 1) / k.rows, tn = (p.cols + k.cols - 1) / k.cols;
+    for (int splits = 1; splits <= 32; ++splits) {
+      const int per = (all + splits - 1) / splits;
+      if (splits > 1 && (per < 4 || (int64_t)per * (splits - 1) >= all)) continue;
+      const double waves = (double)((tm * tn * p.batches * splits + k.workers - 1) / k.workers);
+      double cost = waves * (per * k.block + 2500);
+      if (splits > 1)
+        cost += 6000 + (double)splits * p.rows * p.ldp * p.batches * kHalf * 8 / 2000;
+      if (!pick || cost < best) {
+        best = cost, pick = &k;
+        p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.splits = splits, p.blocks_per_split = per;
+      }
+    }
+  }
+  Scratch partial;
+  if (p.splits > 1) {
+    const int64_t sums = (int64_t)p.splits * p.batches * kHalf * p.rows * p.ldp;
+    if (xvec_gpu_status st = partial.alloc((size_t)sums * 4, s)) return st;
+    p.partial = partial.as<float>();
+  }
+  return pick->pair ? launch_shape<MODE, T, true, kPairCols>(c, p, pick->workers, s)
+                    : launch_shape<MODE, T, false, 128>(c, p, pick->workers, s);
+}
+
+template <typename T>
+xvec_gpu_status gemm_by_mode(const GemmCall& c, cudaStream_t s) {
+  switch (c.mode) {
+    case kLinear: return launch_gemm<kLinear, T>(c, s);
+    case kGated: return launch_gemm<kGated, T>(c, s);
+    case kDx: return launch_gemm<kDx, T>(c, s);
+    default: return launch_gemm<kDw, T>(c, s);
+  }
+}
+
+}  // namespace adapter
+}  // namespace xvec

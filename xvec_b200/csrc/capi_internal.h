@@ -131,6 +131,9 @@ xvec_gpu_status tc_seeded_scan(int device, int nq, int64_t n, int kp, cudaStream
                                Scratch& psat, int* lists_out, Scratch* gthr_out = nullptr,
                                const TcPreseed& preseed = TcPreseed());
 
+// Limit of the tensor-core kernels' main-loop waits (xvec_gpu_set_wait_limit_ns).
+int64_t wait_limit_ns();
+
 // Streaming Flat candidate scan for a few queries (flat_stream.cu): a sample
 // pass over every 64th row for the starting thresholds, the pass over all
 // rows, and one candidate list per query (lkeys [nq][flat_stream_list_stride(kp)],

@@ -1107,6 +1107,8 @@ bool sq8_tc_supported(int d, const void* codes, const void* qcodes) {
 
 }  // namespace xvec
 
+int64_t xvec::wait_limit_ns() { return g_tc_wait_ns.load(std::memory_order_relaxed); }
+
 extern "C" int64_t xvec_gpu_set_wait_limit_ns(int64_t ns) {
   return xvec::g_tc_wait_ns.exchange(ns > 0 ? ns : (int64_t)xvec::tc::kWaitLimitNs);
 }
