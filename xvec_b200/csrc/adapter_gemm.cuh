@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const CUtensorMap* bm = (MODE == kDx && seg) ? &bmap1 : &bmap0;
 #pragma unroll 1
           for (int pl = 0; pl < P; ++pl) {
-            if (!mbar_wait(&empty[stage], phase ^ 1, s_abort, p.wait_ns)) {
+            if (!mbar_wait<1>(&empty[stage], phase ^ 1, s_abort, p.wait_ns)) {
               fail();
               break;
             }
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       uint32_t phase = 0, round = 0;
       // Waits for the stage and moves on; the stage's tile address.
       auto next = [&](const unsigned char** tile) {
-        const bool ok = mbar_wait(&full[stage], phase, s_abort, p.wait_ns);
+        const bool ok = mbar_wait<1>(&full[stage], phase, s_abort, p.wait_ns);
         *tile = tiles + stage * S::kStageBytes;
         if (++stage == kStages) {
           stage = 0;
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int per = P == 1 ? it.k1 - it.k0 : kRound;
         for (int r0 = it.k0; r0 < it.k1 && !*s_abort; r0 += per, ++round) {
           const int acc = round & 1;
-          if (!mbar_wait(&tempty[acc], ((round >> 1) & 1) ^ 1, s_abort, p.wait_ns)) {
+          if (!mbar_wait<1>(&tempty[acc], ((round >> 1) & 1) ^ 1, s_abort, p.wait_ns)) {
             fail();
             break;
           }
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       // Retire every issued MMA before tensor memory is released.
       mma_commit<PAIR>(smem_u32(mdone));
-      if (!mbar_wait(mdone, 0, nullptr)) fail();
+      if (!mbar_wait<1>(mdone, 0, nullptr)) fail();
     }
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     uint32_t round = 0;
     auto wait_round = [&] {
-      const bool ok = mbar_wait(&tfull[round & 1], (round >> 1) & 1, s_abort, p.wait_ns);
+      const bool ok = mbar_wait<1>(&tfull[round & 1], (round >> 1) & 1, s_abort, p.wait_ns);
       tmem_fence_after();
       if (!ok) fail();
       return __all_sync(0xffffffffu, ok);
@@ -531,11 +531,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // Where the second CTA gave up before the first, its half never comes: the
       // wait then only gives the first's own copies ample time.
       if (mine > 0 &&
-          !mbar_wait(&full[s], (mine - 1) & 1, nullptr, other < mine ? 20000000ull : kWaitLimitNs))
+          !mbar_wait<1>(&full[s], (mine - 1) & 1, nullptr, other < mine ? 20000000ull : kWaitLimitNs))
         fail();
       if (PAIR && other > mine) {
         mbar_expect_tx(&full[s], S::kStageBytes);
-        if (!mbar_wait(&full[s], mine & 1, nullptr)) fail();
+        if (!mbar_wait<1>(&full[s], mine & 1, nullptr)) fail();
       }
     }
   }
