@@ -47,6 +47,7 @@ constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
 constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, one per column half
 constexpr int kGemmThreads = 64 + kEpiWarps * 32;
 constexpr uint32_t kABytes = kBM * kBK * 2;
+constexpr int kBand = 8;      // row tiles per band of the tile order
 constexpr int kRound = 2;     // float32: depth blocks per accumulation in tensor memory
 
 template <typename T, bool PAIR, int BN>
@@ -113,6 +114,20 @@ __device__ __forceinline__ void mma_16bit(uint32_t d, uint64_t a, uint64_t b, ui
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// Arrives on the barrier at the shared-memory address `bar` of this CTA (PAIR: of both
+// CTAs) once every MMA this thread issued so far has completed.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    tc::mma_commit<false>(bar);
 }
 
 // --- epilogue rows: 32 consecutive elements of one row ---------------------------
@@ -236,8 +251,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   tmem_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  // Work item -> split, batch, tile (columns fastest: the CTAs running at a
-  // time share A's rows and find B in L2).
+  // Work item -> split, batch, tile.  Tiles go down bands of kBand row tiles, so
+  // that those running at a time share both A's rows and B's columns in L2.
   struct Item {
     int batch, tm, tn, k0, k1, split;
   };
@@ -246,8 +261,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int t = i % tiles_mn, g = i / tiles_mn;
     it.batch = g % p.batches;
     it.split = g / p.batches;
-    it.tm = t / p.tiles_n;
-    it.tn = t % p.tiles_n;
+    const int band = t / (kBand * p.tiles_n), in = t - band * kBand * p.tiles_n;
+    const int height = min(kBand, p.tiles_m - band * kBand);
+    it.tn = in / height;
+    it.tm = band * kBand + in - it.tn * height;
     it.k0 = it.split * p.blocks_per_split;
     it.k1 = min(all_blocks, it.k0 + p.blocks_per_split);
     return it;
@@ -259,9 +276,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const uint32_t full0 = PAIR ? cluster_addr(&full[0], 0) : smem_u32(&full[0]);
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t count[kStages];
-#pragma unroll
-      for (int s = 0; s < kStages; ++s) count[s] = 0;
+      uint32_t count = 0;  // stages filled
       for (int i = worker; i < items && !*s_abort; i += workers) {
         const Item it = item_of(i);
         const int row0 = it.tm * kTileRows + (int)rank * kBM;
@@ -302,8 +317,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             } else {
               load_box<PAIR>(bm, bar, b, k, col0 + (int)rank * S::kBRows, pl);
             }
-#pragma unroll
-            for (int s = 0; s < kStages; ++s) count[s] += s == stage;
+            ++count;
             if (++stage == kStages) {
               stage = 0;
               phase ^= 1;
@@ -311,15 +325,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       }
-#pragma unroll
-      for (int s = 0; s < kStages; ++s) issued[s] = count[s];
+      for (int s = 0; s < kStages; ++s)
+        issued[s] = count / kStages + (s < (int)(count % kStages) ? 1 : 0);
     }
   } else if (warp == 1 && issuer) {
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
       const uint32_t own_empty0 = smem_u32(&empty[0]), own_tfull0 = smem_u32(&tfull[0]);
-      const uint32_t peer_empty0 = PAIR ? cluster_addr(&empty[0], 1) : 0u;
-      const uint32_t peer_tfull0 = PAIR ? cluster_addr(&tfull[0], 1) : 0u;
       int stage = 0;
       uint32_t phase = 0, round = 0;
       // Waits for the stage and moves on; the stage's tile address.
@@ -334,8 +346,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       };
       auto release = [&](const unsigned char* tile) {
         const uint32_t s = (uint32_t)(tile - tiles) / S::kStageBytes;
-        mma_commit<PAIR>(own_empty0 + s * 8);
-        if (PAIR) mma_commit<PAIR>(peer_empty0 + s * 8);
+        commit<PAIR>(own_empty0 + s * 8);
       };
       for (int i = worker; i < items && !*s_abort; i += workers) {
         const Item it = item_of(i);
@@ -380,8 +391,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
             for (int pl = 0; pl < P; ++pl) release(t[pl]);
           }
-          mma_commit<PAIR>(own_tfull0 + acc * 8);
-          if (PAIR) mma_commit<PAIR>(peer_tfull0 + acc * 8);
+          commit<PAIR>(own_tfull0 + acc * 8);
         }
       }
       // Retire every issued MMA before tensor memory is released.
@@ -394,11 +404,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     float* bias_s = bias_all + ew * 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     uint32_t round = 0;
+    // One lane polls; the others wait at the shuffle.
     auto wait_round = [&] {
-      const bool ok = mbar_wait<1>(&tfull[round & 1], (round >> 1) & 1, s_abort, p.wait_ns);
+      int ok = 1;
+      if (lane == 0 && !mbar_wait<1>(&tfull[round & 1], (round >> 1) & 1, s_abort, p.wait_ns)) {
+        fail();
+        ok = 0;
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
       tmem_fence_after();
-      if (!ok) fail();
-      return __all_sync(0xffffffffu, ok);
+      return ok != 0;
     };
     auto release_round = [&] {
       tmem_fence_before();
