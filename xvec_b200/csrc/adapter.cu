@@ -170,14 +170,19 @@ __global__ void __launch_bounds__(256)
         load8(u + r * ldz + c, m - c, vec & 4, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          d[1][j] = d[0][j] * activate(act, g[j]);
-          d[0][j] = d[0][j] * v[j] * slope(act, g[j]);
+          float slope;
+          d[1][j] = d[0][j] * activate_slope<T>(act, g[j], &slope);
+          d[0][j] = d[0][j] * v[j] * slope;
         }
       } else if (act != XVEC_ACT_NONE) {
         float v[8];
         load8(z + r * ldz + c, m - c, vec & 2, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[0][j] *= slope(act, v[j]);
+        for (int j = 0; j < 8; ++j) {
+          float slope;
+          activate_slope<T>(act, v[j], &slope);
+          d[0][j] *= slope;
+        }
       }
 #pragma unroll
       for (int o = 0; o < kOuts; ++o) {

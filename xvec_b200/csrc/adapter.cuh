@@ -35,25 +35,93 @@ __device__ __forceinline__ bf16 from_f<bf16>(float v) {
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
+// Phi(z), the standard normal distribution, and exp(-z^2 / 2).  float32 results
+// take erff and expf.  For 16-bit results (half a step: 2^-12 or more) the
+// rational approximation 7.1.26 of Abramowitz and Stegun does, off by at most
+// 7.5e-8: a reciprocal, an exponential and six multiply-adds, where erff's
+// two branches made the epilogue the longest part of a tile.
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float z, float* gauss) {
+  if constexpr (sizeof(T) == 4) {
+    *gauss = expf(-0.5f * z * z);
+    return 0.5f * (1.f + erff(z * kSqrtHalf));
+  } else {
+    const float x = fabsf(z) * kSqrtHalf;
+    const float e = __expf(-x * x);
+    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    const float tail = 0.5f * q * t * e;  // Phi(-|z|)
+    *gauss = e;
+    return z < 0.f ? tail : 1.f - tail;
+  }
+}
+// 1 / (1 + exp(-z)).  The quotient is off by at most 2 units in the last place.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+  return __fdividef(1.f, 1.f + (sizeof(T) == 4 ? expf(-z) : __expf(-z)));
+}
+
+template <typename T>
+__device__ __forceinline__ float relu(float z) {
+  return z > 0.f ? z : (z == z ? 0.f : z);
+}
+template <typename T>
+__device__ __forceinline__ float gelu(float z) {
+  float e;
+  return z * normal_cdf<T>(z, &e);
+}
+template <typename T>
+__device__ __forceinline__ float silu(float z) {
+  return z * sigmoid<T>(z);
+}
+
+// act(z) for results of type T.
+template <typename T>
 __device__ __forceinline__ float activate(int act, float z) {
   switch (act) {
-    case XVEC_ACT_RELU: return z > 0.f ? z : (z == z ? 0.f : z);
-    case XVEC_ACT_GELU: return 0.5f * z * (1.f + erff(z * kSqrtHalf));
-    case XVEC_ACT_SILU: return z / (1.f + expf(-z));
+    case XVEC_ACT_RELU: return relu<T>(z);
+    case XVEC_ACT_GELU: return gelu<T>(z);
+    case XVEC_ACT_SILU: return silu<T>(z);
     default: return z;
   }
 }
-// act'(z).
-__device__ __forceinline__ float slope(int act, float z) {
+template <typename T, int N>
+__device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
+  if (act == XVEC_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = relu<T>(v[j]);
+  } else if (act == XVEC_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = gelu<T>(v[j]);
+  } else if (act == XVEC_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = silu<T>(v[j]);
+  }
+}
+// act(z), and act'(z) in *slope.
+template <typename T>
+__device__ __forceinline__ float activate_slope(int act, float z, float* slope) {
   switch (act) {
-    case XVEC_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case XVEC_ACT_GELU:
-      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * expf(-0.5f * z * z) * kInvSqrt2Pi;
-    case XVEC_ACT_SILU: {
-      const float p = 1.f / (1.f + expf(-z));
-      return p * (1.f + z * (1.f - p));
+    case XVEC_ACT_RELU:
+      *slope = z > 0.f ? 1.f : 0.f;
+      return relu<T>(z);
+    case XVEC_ACT_GELU: {
+      float e;
+      const float cdf = normal_cdf<T>(z, &e);
+      *slope = fmaf(z * e, kInvSqrt2Pi, cdf);
+      return z * cdf;
     }
-    default: return 1.f;
+    case XVEC_ACT_SILU: {
+      const float s = sigmoid<T>(z);
+      *slope = s * (1.f + z * (1.f - s));
+      return z * s;
+    }
+    default:
+      *slope = 1.f;
+      return z;
   }
 }
 

@@ -57,47 +57,75 @@ struct GemmShape {
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B columns loaded per CTA
   static constexpr uint32_t kBBytes = kBRows * kBK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  static constexpr uint32_t kBiasBytes = kEpiWarps * 128 * 4;
-  static constexpr int kFit = (int)((232448 - 1024 - 512 - kBiasBytes) / kStageBytes);
+  // Per epilogue warp: 128 biases and a 32 x 64 byte staging block.
+  static constexpr uint32_t kEpiBytes = kEpiWarps * (128 * 4 + 2048);
+  static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
-  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kBiasBytes + 1024 + 512;
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + 512;
   static constexpr int kTmemCols = 2 * kAccCols;
   static_assert(kStages >= 4, "shared memory too small for the stage ring");
 };
 
-// --- operand access -------------------------------------------------------------
+// --- barriers, operands, matrix instructions --------------------------------------
+// The producer and the issuer are single threads whose instruction count bounds
+// the rate of the ring (at 64 deep a stage has 512 clocks), so addresses are
+// 32-bit shared ones, descriptors are kept as sums, and the limit and the abort
+// flag are looked at only after a failed try.
+__device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Bounded: false once limit_ns passed or another role of the CTA raised *abort.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const volatile int* abort,
+                                         uint64_t limit_ns) {
+  if (try_bar(bar, parity)) return true;
+  const uint64_t start = tc::global_ns();
+  for (;;) {
+    if (try_bar(bar, parity)) return true;
+    if (*abort || tc::global_ns() - start > limit_ns) return false;
+  }
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+
 // One box of a [plane][outer][inner] operand.  PAIR: it completes on the barrier at
 // the cluster address `bar`, which may belong to the other CTA.
 template <bool PAIR>
-__device__ __forceinline__ void load_box(const CUtensorMap* map, uint32_t bar, void* dst, int x,
+__device__ __forceinline__ void load_box(const CUtensorMap* map, uint32_t bar, uint32_t dst, int x,
                                          int y, int z) {
   if constexpr (PAIR)
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::smem_u32(dst)),
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
   else
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::smem_u32(dst)),
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
 
-// Matrix descriptor of an operand tile in 128-byte swizzle.
+// Matrix descriptor of an operand tile in 128-byte swizzle, without its address
+// (which is added in units of 16 bytes).
 //   along depth (K-major): rows of 128 bytes, 8-row groups 1024 bytes apart;
 //     16 deep = 32 bytes further.
 //   along rows (MN-major): blocks of 64 rows x 64 deep (8 KB, the leading
 //     offset), in a block 8-deep groups 1024 bytes apart; 16 deep = 2048 bytes
 //     further.
 template <bool MN>
-__device__ __forceinline__ uint64_t tile_desc(const void* tile) {
-  const uint64_t addr = tc::smem_u32(tile);
-  const uint64_t lead = MN ? 8192 >> 4 : 1;
-  return ((addr & 0x3FFFFull) >> 4) | (lead << 16) | ((1024ull >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
-}
+constexpr uint64_t kTileDesc = ((uint64_t)(MN ? 8192 >> 4 : 1) << 16) |
+                               ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 template <bool MN>
 constexpr uint64_t kDepthStep = MN ? 2048 >> 4 : 32 >> 4;
 
@@ -115,7 +143,6 @@ __device__ __forceinline__ void mma_16bit(uint32_t d, uint64_t a, uint64_t b, ui
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-
 // Arrives on the barrier at the shared-memory address `bar` of this CTA (PAIR: of both
 // CTAs) once every MMA this thread issued so far has completed.
 template <bool PAIR>
@@ -130,54 +157,125 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     tc::mma_commit<false>(bar);
 }
 
-// --- epilogue rows: 32 consecutive elements of one row ---------------------------
-template <typename T>
-__device__ __forceinline__ void store32(T* p, const float (&v)[32], int count, bool vec) {
-  if (vec && count >= 32) {
-    if constexpr (std::is_same<T, float>::value) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        reinterpret_cast<float4*>(p)[i] =
-            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        __align__(16) T t[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = from_f<T>(v[8 * i + j]);
-        reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<uint4*>(t);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < count) p[i] = from_f<T>(v[i]);
-  }
+// --- epilogue input and output ------------------------------------------------------
+// A warp holds 32 x 32 values, one row per lane.  They reach memory (and a
+// residual comes from it) through a staging block of 32 rows of 64 bytes, so
+// that each instruction covers whole 64-byte row segments: 4 lanes of 16 bytes
+// per row.  The 16-byte parts of row r are permuted by (r / 2) mod 4, which
+// keeps both directions free of bank conflicts.
+__device__ __forceinline__ uint32_t stage_at(uint32_t buf, int row, int part) {
+  return buf + row * 64 + ((part ^ ((row >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
 }
 template <typename T>
-__device__ __forceinline__ void add32(const T* p, float (&v)[32], int count, bool vec) {
-  if (vec && count >= 32) {
-    if constexpr (std::is_same<T, float>::value) {
+__device__ __forceinline__ uint4 pack16(const float* v) {
+  uint4 u;
+  if constexpr (std::is_same<T, float>::value) {
+    u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                   __float_as_uint(v[3]));
+  } else {
+    T* t = reinterpret_cast<T*>(&u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 t = reinterpret_cast<const float4*>(p)[i];
-        v[4 * i] += t.x, v[4 * i + 1] += t.y, v[4 * i + 2] += t.z, v[4 * i + 3] += t.w;
-      }
-    } else {
+    for (int j = 0; j < 8; ++j) t[j] = from_f<T>(v[j]);
+  }
+  return u;
+}
+
+// Writes v (this lane's row) to base[row * ld + column], rows and cols of it.
+template <typename T>
+__device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows, int cols, bool vec,
+                                     const float (&v)[32], int lane) {
+  constexpr int kCols = 64 / sizeof(T), kPart = 16 / sizeof(T);  // columns per block and part
+#pragma unroll
+  for (int h = 0; h < 32 / kCols; ++h) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sts16(stage_at(buf, lane, c), pack16<T>(v + h * kCols + c * kPart));
+    __syncwarp();
+    T* out = base + h * kCols;
+    const int left = cols - h * kCols;
+    if (vec && left >= kCols) {
+      const int part = lane & 3;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-        const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[8 * i + j] += to_f(t[j]);
+        const int r = i * 8 + (lane >> 2);
+        if (r < rows)
+          *reinterpret_cast<uint4*>(out + r * ld + part * kPart) = lds16(stage_at(buf, r, part));
       }
+    } else {
+      const int col = lane % kCols;
+      for (int r = lane / kCols; r < rows; r += 32 / kCols)
+        if (col < left) {
+          const uint32_t a = stage_at(buf, r, col / kPart) + (col % kPart) * sizeof(T);
+          if constexpr (sizeof(T) == 4) {
+            float f;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+            out[r * ld + col] = f;
+          } else {
+            uint16_t b;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(a) : "memory");
+            reinterpret_cast<uint16_t*>(out)[r * ld + col] = b;
+          }
+        }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < count) v[i] += to_f(p[i]);
+    __syncwarp();
   }
 }
+
+// A 32 x 32 block on its way in: requested early (start), added to this lane's
+// row later (add).  Rows or columns that do not exist are not read.
+template <typename T>
+struct Incoming {
+  static constexpr int kParts = 32 * sizeof(T) / 16;  // 16-byte parts of a row
+  uint4 v[kParts];
+
+  __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, bool whole, int lane) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int r = (i & 3) * 8 + (lane >> 2);
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (whole && r < rows)
+        v[i] = *reinterpret_cast<const uint4*>(base + r * ld + (i >> 2) * (64 / sizeof(T)) +
+                                               (lane & 3) * (16 / sizeof(T)));
+    }
+  }
+  __device__ __forceinline__ void add(uint32_t buf, const T* base, int64_t ld, int rows, int cols,
+                                      bool whole, float (&f)[32], int lane) {
+    if (whole) {
+#pragma unroll
+      for (int h = 0; h < kParts / 4; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sts16(stage_at(buf, i * 8 + (lane >> 2), lane & 3), v[h * 4 + i]);
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint4 u = lds16(stage_at(buf, lane, c));
+          const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+          for (int j = 0; j < 16 / (int)sizeof(T); ++j)
+            f[h * (64 / sizeof(T)) + c * (16 / sizeof(T)) + j] += to_f(t[j]);
+        }
+        __syncwarp();
+      }
+    } else if (lane < rows) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < cols) f[j] += to_f(base[lane * ld + j]);
+    }
+  }
+};
 
 // --- the kernel ---------------------------------------------------------------
 template <int MODE, typename T, bool PAIR, int BN>
@@ -194,7 +292,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   constexpr int kWarpCols = BN / 2;  // accumulator columns per epilogue warp
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* bias_all = reinterpret_cast<float*>(tiles + kStages * S::kStageBytes);
+  unsigned char* staging = tiles + kStages * S::kStageBytes;
+  float* bias_all = reinterpret_cast<float*>(staging + kEpiWarps * 2048);
   uint64_t* full = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * 128);
   uint64_t* empty = full + kStages;   // the MMAs have read the stage
   uint64_t* tfull = empty + kStages;  // [2] accumulator ready
@@ -213,6 +312,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int tiles_mn = p.tiles_m * p.tiles_n;
   const int items = tiles_mn * p.batches * p.splits;
   const int all_blocks = p.segs * p.blocks;
+  const uint64_t limit = p.wait_ns;
   auto fail = [&] {
     if (p.status) atomicExch(p.status, (int)XVEC_GPU_TIMEOUT);
     *s_abort = 1;
@@ -273,141 +373,123 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
-      const uint32_t full0 = PAIR ? cluster_addr(&full[0], 0) : smem_u32(&full[0]);
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t count = 0;  // stages filled
-      for (int i = worker; i < items && !*s_abort; i += workers) {
+      const uint32_t tiles_at = smem_u32(tiles), empty_at = smem_u32(empty);
+      const uint32_t full_at = smem_u32(full), bars = PAIR ? cluster_addr(full, 0) : full_at;
+      uint32_t stage = 0, phase = 0, count = 0;  // count: stages filled
+      bool ok = true;
+      for (int i = worker; i < items && ok; i += workers) {
         const Item it = item_of(i);
         const int row0 = it.tm * kTileRows + (int)rank * kBM;
-        const int col0 = it.tn * kTileCols;
-        for (int kb = it.k0; kb < it.k1 && !*s_abort; ++kb) {
-          const int seg = kb / p.blocks;
-          const int k = (kb - seg * p.blocks) * kBK;
+        const int col0 = it.tn * kTileCols + (MODE == kGated ? 0 : (int)rank * S::kBRows);
+        int seg = it.k0 / p.blocks;
+        int k = (it.k0 - seg * p.blocks) * kBK;
+        const int k_end = p.blocks * kBK;
+        for (int n = it.k1 - it.k0; n > 0 && ok; --n) {
           const int az = (MODE == kDw ? it.batch : MODE == kDx ? seg : 0) * P;
-          const CUtensorMap* bm = (MODE == kDx && seg) ? &bmap1 : &bmap0;
-#pragma unroll 1
+          const CUtensorMap* bm = (MODE == kDx && seg) || (MODE == kGated && PAIR && rank) ? &bmap1
+                                                                                          : &bmap0;
+#pragma unroll
           for (int pl = 0; pl < P; ++pl) {
-            if (!mbar_wait<1>(&empty[stage], phase ^ 1, s_abort, p.wait_ns)) {
-              fail();
-              break;
-            }
-            unsigned char* a = tiles + stage * S::kStageBytes;
-            unsigned char* b = a + kABytes;
-            const uint32_t bar = full0 + stage * 8;
-            if (issuer) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * S::kStageBytes);
+            if (!(ok = ok && wait_bar(empty_at + stage * 8, phase ^ 1, s_abort, limit))) break;
+            const uint32_t a = tiles_at + stage * S::kStageBytes, b = a + kABytes;
+            const uint32_t bar = bars + stage * 8;
+            if (issuer) expect_bytes(full_at + stage * 8, (PAIR ? 2 : 1) * S::kStageBytes);
             if constexpr (A_MN) {
               load_box<PAIR>(&amap, bar, a, row0, k, az + pl);
               load_box<PAIR>(&amap, bar, a + 8192, row0 + 64, k, az + pl);
             } else {
               load_box<PAIR>(&amap, bar, a, k, row0, az + pl);
             }
-            if constexpr (MODE == kGated) {
-              // Columns of the tile: the gate's half, then the up's half.
-              if constexpr (PAIR) {
-                load_box<PAIR>(rank ? &bmap1 : &bmap0, bar, b, k, col0, pl);
-              } else {
-                load_box<PAIR>(&bmap0, bar, b, k, col0, pl);
-                load_box<PAIR>(&bmap1, bar, b + S::kBBytes / 2, k, col0, pl);
-              }
-            } else if constexpr (B_MN) {
+            if constexpr (B_MN) {
 #pragma unroll
               for (int c = 0; c < S::kBRows / 64; ++c)
-                load_box<PAIR>(bm, bar, b + c * 8192, col0 + (int)rank * S::kBRows + c * 64, k, pl);
+                load_box<PAIR>(bm, bar, b + c * 8192, col0 + c * 64, k, pl);
             } else {
-              load_box<PAIR>(bm, bar, b, k, col0 + (int)rank * S::kBRows, pl);
+              // Gated: the gate's columns, then the up's (PAIR: one in each CTA).
+              load_box<PAIR>(bm, bar, b, k, col0, pl);
+              if constexpr (MODE == kGated && !PAIR)
+                load_box<PAIR>(&bmap1, bar, b + S::kBBytes / 2, k, col0, pl);
             }
             ++count;
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1;
-            }
+            if (++stage == kStages) stage = 0, phase ^= 1;
           }
+          if ((k += kBK) == k_end) k = 0, ++seg;
         }
       }
-      for (int s = 0; s < kStages; ++s)
-        issued[s] = count / kStages + (s < (int)(count % kStages) ? 1 : 0);
+      if (!ok) fail();
+      for (uint32_t s = 0; s < kStages; ++s)
+        issued[s] = count / kStages + (s < count % kStages ? 1 : 0);
     }
   } else if (warp == 1 && issuer) {
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
-      const uint32_t own_empty0 = smem_u32(&empty[0]), own_tfull0 = smem_u32(&tfull[0]);
-      int stage = 0;
-      uint32_t phase = 0, round = 0;
-      // Waits for the stage and moves on; the stage's tile address.
-      auto next = [&](const unsigned char** tile) {
-        const bool ok = mbar_wait<1>(&full[stage], phase, s_abort, p.wait_ns);
-        *tile = tiles + stage * S::kStageBytes;
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-        return ok;
-      };
-      auto release = [&](const unsigned char* tile) {
-        const uint32_t s = (uint32_t)(tile - tiles) / S::kStageBytes;
-        commit<PAIR>(own_empty0 + s * 8);
-      };
-      for (int i = worker; i < items && !*s_abort; i += workers) {
+      const uint32_t full_at = smem_u32(full), empty_at = smem_u32(empty);
+      const uint32_t tfull_at = smem_u32(tfull), tempty_at = smem_u32(tempty);
+      const uint64_t a0 = kTileDesc<A_MN> + (smem_u32(tiles) >> 4);
+      const uint64_t b0 = kTileDesc<B_MN> + ((smem_u32(tiles) + kABytes) >> 4);
+      uint32_t stage = 0, phase = 0, round = 0;
+      bool ok = true;
+      for (int i = worker; i < items && ok; i += workers) {
         const Item it = item_of(i);
         const int per = P == 1 ? it.k1 - it.k0 : kRound;
-        for (int r0 = it.k0; r0 < it.k1 && !*s_abort; r0 += per, ++round) {
-          const int acc = round & 1;
-          if (!mbar_wait<1>(&tempty[acc], ((round >> 1) & 1) ^ 1, s_abort, p.wait_ns)) {
-            fail();
-            break;
-          }
+        for (int r0 = it.k0; r0 < it.k1 && ok; r0 += per, ++round) {
+          const uint32_t acc = round & 1;
+          if (!(ok = wait_bar(tempty_at + acc * 8, ((round >> 1) & 1) ^ 1, s_abort, limit))) break;
           tmem_fence_after();
           const uint32_t d = tmem_base + acc * S::kAccCols;
-          const int r1 = min(it.k1, r0 + per);
-          for (int kb = r0; kb < r1; ++kb) {
-            const unsigned char* t[P];
-            bool ok = true;
-            auto multiply = [&](int i, int j, uint32_t d, bool first) {
-              const uint64_t a = tile_desc<A_MN>(t[i]), b = tile_desc<B_MN>(t[j] + kABytes);
+          uint32_t first = 0;  // 0: the accumulators are overwritten
+          for (int n = min(it.k1 - r0, per); n > 0 && ok; --n) {
+            uint32_t at[P];
+            auto multiply = [&](int i, int j, uint32_t d, uint32_t keep) {
+              const uint64_t a = a0 + at[i] * (S::kStageBytes >> 4);
+              const uint64_t b = b0 + at[j] * (S::kStageBytes >> 4);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 mma_16bit<PAIR>(d, a + k * kDepthStep<A_MN>, b + k * kDepthStep<B_MN>, p.idesc,
-                                (first && k == 0) ? 0u : 1u);
+                                k == 0 ? keep : 1u);
             };
 #pragma unroll
             for (int pl = 0; pl < P; ++pl) {
-              if (!(ok = ok && next(&t[pl]))) break;
+              at[pl] = stage;
+              if (!(ok = ok && wait_bar(full_at + stage * 8, phase, s_abort, limit))) break;
+              if (++stage == kStages) stage = 0, phase ^= 1;
               tmem_fence_after();
-              if (pl == 0) multiply(0, 0, d, kb == r0);
+              if (pl == 0) multiply(0, 0, d, first);
               if constexpr (P == 3) {
                 if (pl == 1) {
-                  multiply(1, 1, d + BN, kb == r0);
-                  multiply(0, 1, d + BN, false);
-                  multiply(1, 0, d + BN, false);
+                  multiply(1, 1, d + BN, first);
+                  multiply(0, 1, d + BN, 1);
+                  multiply(1, 0, d + BN, 1);
                 }
-                if (pl == 2) multiply(0, 2, d + BN, false), multiply(2, 0, d + BN, false);
+                if (pl == 2) multiply(0, 2, d + BN, 1), multiply(2, 0, d + BN, 1);
               }
             }
-            if (!ok) {
-              fail();
-              break;
-            }
+            first = 1;
+            if (ok)
 #pragma unroll
-            for (int pl = 0; pl < P; ++pl) release(t[pl]);
+              for (int pl = 0; pl < P; ++pl) commit<PAIR>(empty_at + at[pl] * 8);
           }
-          commit<PAIR>(own_tfull0 + acc * 8);
+          commit<PAIR>(tfull_at + acc * 8);
         }
       }
+      if (!ok) fail();
       // Retire every issued MMA before tensor memory is released.
       mma_commit<PAIR>(smem_u32(mdone));
-      if (!mbar_wait<1>(mdone, 0, nullptr)) fail();
+      if (!mbar_wait(mdone, 0, nullptr)) fail();
     }
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3, ew = warp - 2, half = ew >> 2;
     float* bias_s = bias_all + ew * 128;
+    const uint32_t buf = smem_u32(staging + ew * 2048);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tfull_at = smem_u32(tfull);
+    const bool vec = p.vec != 0;
     uint32_t round = 0;
     // One lane polls; the others wait at the shuffle.
     auto wait_round = [&] {
       int ok = 1;
-      if (lane == 0 && !mbar_wait<1>(&tfull[round & 1], (round >> 1) & 1, s_abort, p.wait_ns)) {
+      if (lane == 0 && !wait_bar(tfull_at + (round & 1) * 8, (round >> 1) & 1, s_abort, limit)) {
         fail();
         ok = 0;
       }
@@ -431,64 +513,80 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       return MODE == kGated ? (c & 1) * (BN / 2) + half * (BN / 4) + (c >> 1) * 32
                             : half * kWarpCols + c * 32;
     };
+    constexpr int kStep = MODE == kGated ? 2 : 1;
     for (int i = worker; i < items; i += workers) {
       const Item it = item_of(i);
-      const int64_t row = (int64_t)it.tm * kTileRows + rank * kBM + quarter * 32 + lane;
+      const int64_t row0 = (int64_t)it.tm * kTileRows + rank * kBM + quarter * 32;
+      const int rows = (int)max((int64_t)0, min((int64_t)32, p.rows - row0));
       const int64_t warp_col =
           (int64_t)it.tn * kTileCols + half * (MODE == kGated ? BN / 4 : kWarpCols);
+      const int64_t cols = p.cols - warp_col;  // from the warp's first one (may be negative)
+      const T* res = MODE == kLinear && p.splits == 1 && p.residual
+                         ? static_cast<const T*>(p.residual) + row0 * p.ldr + warp_col
+                         : nullptr;
+      Incoming<T> in;
+      if (MODE == kLinear && res) in.start(res, p.ldr, rows, vec && cols >= 32, lane);
       if constexpr (MODE == kLinear || MODE == kGated) {
         // The warp's biases: its columns' in order (gated: gate, then up).
         __syncwarp();
         constexpr int kBiases = MODE == kGated ? BN / 4 : kWarpCols;
         for (int c = lane; c < kBiases; c += 32) {
-          const bool in = warp_col + c < p.cols;
-          bias_s[c] = in && p.bias[0] ? to_f(static_cast<const T*>(p.bias[0])[warp_col + c]) : 0.f;
+          const bool has = c < cols;
+          bias_s[c] = has && p.bias[0] ? to_f(static_cast<const T*>(p.bias[0])[warp_col + c]) : 0.f;
           if constexpr (MODE == kGated)
             bias_s[kBiases + c] =
-                in && p.bias[1] ? to_f(static_cast<const T*>(p.bias[1])[warp_col + c]) : 0.f;
+                has && p.bias[1] ? to_f(static_cast<const T*>(p.bias[1])[warp_col + c]) : 0.f;
         }
         __syncwarp();
       }
       // Finishes 32 columns (gated: v the gate's, u the up's sums).
       auto finish = [&](int c, float (&v)[32], float (&u)[32]) {
-        const int64_t col = warp_col + (MODE == kGated ? c >> 1 : c) * 32;
-        if (row >= p.rows || col >= p.cols) return;
-        const int count = (int)min((int64_t)32, p.cols - col);
-        const bool vec = p.vec != 0;
+        const int at = (MODE == kGated ? c >> 1 : c) * 32;
+        const int n = (int)min((int64_t)32, cols - at);
+        if (n <= 0) return;
+        const int64_t col = warp_col + at;
         if (p.splits > 1) {
           constexpr int kPlanes = MODE == kGated ? 2 : 1;
           float* dst = p.partial +
-                       ((int64_t)(it.split * p.batches + it.batch) * kPlanes * p.rows + row) *
+                       ((int64_t)(it.split * p.batches + it.batch) * kPlanes * p.rows + row0) *
                            p.ldp + col;
-          store32<float>(dst, v, 32, true);
-          if constexpr (MODE == kGated) store32<float>(dst + p.rows * p.ldp, u, 32, true);
+          emit(buf, dst, p.ldp, rows, 32, true, v, lane);
+          if constexpr (MODE == kGated)
+            emit(buf, dst + p.rows * p.ldp, p.ldp, rows, 32, true, u, lane);
           return;
         }
         if constexpr (MODE == kLinear || MODE == kGated) {
-          const float* b = bias_s + (MODE == kGated ? c >> 1 : c) * 32;
+          const float4* b = reinterpret_cast<const float4*>(bias_s + at);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += b[j];
-          if (p.save[0]) store32(static_cast<T*>(p.save[0]) + row * p.lds + col, v, count, vec);
+          for (int j = 0; j < 8; ++j) {
+            const float4 t = b[j];
+            v[4 * j] += t.x, v[4 * j + 1] += t.y, v[4 * j + 2] += t.z, v[4 * j + 3] += t.w;
+          }
+          const int64_t save = row0 * p.lds + col;
+          if (p.save[0])
+            emit(buf, static_cast<T*>(p.save[0]) + save, p.lds, rows, n, vec, v, lane);
           if constexpr (MODE == kGated) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] += b[BN / 4 + j];
-            if (p.save[1]) store32(static_cast<T*>(p.save[1]) + row * p.lds + col, u, count, vec);
+            for (int j = 0; j < 8; ++j) {
+              const float4 t = b[BN / 16 + j];
+              u[4 * j] += t.x, u[4 * j + 1] += t.y, u[4 * j + 2] += t.z, u[4 * j + 3] += t.w;
+            }
+            if (p.save[1])
+              emit(buf, static_cast<T*>(p.save[1]) + save, p.lds, rows, n, vec, u, lane);
           }
-          if (p.act != XVEC_ACT_NONE) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = activate(p.act, v[j]);
-          }
+          activate_all<T>(p.act, v);
           if constexpr (MODE == kGated) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= u[j];
-          } else if (p.residual) {
-            add32(static_cast<const T*>(p.residual) + row * p.ldr + col, v, count, vec);
+          } else if (res) {
+            in.add(buf, res + at, p.ldr, rows, n, vec && n == 32, v, lane);
+            if (c + 1 < kChunks)
+              in.start(res + at + 32, p.ldr, rows, vec && cols >= at + 64, lane);
           }
         }
-        store32(static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row * p.ldo + col, v, count,
-                vec);
+        emit(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col, p.ldo,
+             rows, n, vec, v, lane);
       };
-      constexpr int kStep = MODE == kGated ? 2 : 1;
       if constexpr (P == 1) {
         if (!wait_round()) break;
         const uint32_t t = tmem_base + (round & 1) * S::kAccCols + lanes;
@@ -514,15 +612,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t t = tmem_base + (round & 1) * S::kAccCols + lanes;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
-            uint32_t raw[32], small[32];
+            uint32_t raw[32];
             tmem_ld32(t + acc_col(c), raw);
-            tmem_ld32(t + BN + acc_col(c), small);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float v = __uint_as_float(raw[j]) + __uint_as_float(small[j]);
-              sum[c][j] = r0 == it.k0 ? v : sum[c][j] + v;
-            }
+            for (int j = 0; j < 32; ++j)
+              sum[c][j] = r0 == it.k0 ? __uint_as_float(raw[j]) : sum[c][j] + __uint_as_float(raw[j]);
+            tmem_ld32(t + BN + acc_col(c), raw);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[c][j] += __uint_as_float(raw[j]);
           }
           release_round();
         }
@@ -546,11 +645,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // Where the second CTA gave up before the first, its half never comes: the
       // wait then only gives the first's own copies ample time.
       if (mine > 0 &&
-          !mbar_wait<1>(&full[s], (mine - 1) & 1, nullptr, other < mine ? 20000000ull : kWaitLimitNs))
+          !mbar_wait(&full[s], (mine - 1) & 1, nullptr, other < mine ? 20000000ull : kWaitLimitNs))
         fail();
       if (PAIR && other > mine) {
         mbar_expect_tx(&full[s], S::kStageBytes);
-        if (!mbar_wait<1>(&full[s], mine & 1, nullptr)) fail();
+        if (!mbar_wait(&full[s], mine & 1, nullptr)) fail();
       }
     }
   }
@@ -595,7 +694,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Gem
       if (MODE == kLinear || MODE == kGated) {
         if (p.bias[0]) y += to_f(static_cast<const T*>(p.bias[0])[c]);
         if (p.save[0]) static_cast<T*>(p.save[0])[row * p.lds + c] = from_f<T>(y);
-        y = activate(p.act, y);
+        y = activate<T>(p.act, y);
       }
       if constexpr (MODE == kGated) {
         float u = v[1][j];

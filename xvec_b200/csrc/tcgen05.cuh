@@ -59,8 +59,7 @@ __device__ __forceinline__ uint64_t global_ns() {
 }
 
 // Bounded parity wait: false once limit_ns passed or another role of the
-// CTA raised *abort, both looked at every kEvery failed tries.
-template <int kEvery = 256>
+// CTA raised *abort.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
                                           const volatile int* abort,
                                           uint64_t limit_ns = kWaitLimitNs) {
@@ -76,7 +75,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
         : "r"(addr), "r"(parity)
         : "memory");
     if (done) return true;
-    if ((i & (kEvery - 1)) == 0) {
+    if ((i & 255) == 0) {
       if (abort && *abort) return false;
       const uint64_t now = global_ns();
       if (start == 0) start = now;
