@@ -6,6 +6,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "capi_internal.h"
 
@@ -30,6 +33,21 @@ __device__ __forceinline__ __half from_f<__half>(float v) {
 template <>
 __device__ __forceinline__ bf16 from_f<bf16>(float v) {
   return __float2bfloat16_rn(v);
+}
+
+// Two values side by side, each rounded to T.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (sizeof(T) != 2) return 0;
+  uint32_t u;
+  if constexpr (std::is_same<T, bf16>::value) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    memcpy(&u, &t, 4);
+  } else {
+    const __half2 t = __floats2half2_rn(a, b);
+    memcpy(&u, &t, 4);
+  }
+  return u;
 }
 
 constexpr float kSqrtHalf = 0.70710678118654752f;

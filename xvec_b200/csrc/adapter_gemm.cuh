@@ -44,21 +44,24 @@ namespace adapter {
 
 constexpr int kBM = 128;      // rows per CTA (TMEM lanes)
 constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
-constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, one per column half
-constexpr int kGemmThreads = 64 + kEpiWarps * 32;
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr int kBand = 8;      // row tiles per band of the tile order
 constexpr int kRound = 2;     // float32: depth blocks per accumulation in tensor memory
 
 template <typename T, bool PAIR, int BN>
 struct GemmShape {
+  // Two epilogue warps per TMEM lane quarter, one per half of the columns.  (Four
+  // on 256 columns cost a stage of the ring and were slower: 131072 x 1024 -> 1024
+  // fp16 with silu and residual 360 us against 336.)
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 64 + kEpiWarps * 32;
   // Accumulators of one round: the sums, and for float32 the small products'.
   static constexpr int kAccCols = std::is_same<T, float>::value ? 2 * BN : BN;
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B columns loaded per CTA
   static constexpr uint32_t kBBytes = kBRows * kBK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  // Per epilogue warp: 128 biases and a 32 x 64 byte staging block.
-  static constexpr uint32_t kEpiBytes = kEpiWarps * (128 * 4 + 2048);
+  // Per epilogue warp: a bias per column and a 32 x 64 byte staging block.
+  static constexpr uint32_t kEpiBytes = kEpiWarps * (BN / 2 * 4 + 2048);
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + 512;
@@ -186,9 +189,9 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
     u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
                    __float_as_uint(v[3]));
   } else {
-    T* t = reinterpret_cast<T*>(&u);
+    uint32_t* t = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = from_f<T>(v[j]);
+    for (int j = 0; j < 4; ++j) t[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
   }
   return u;
 }
@@ -279,14 +282,14 @@ struct Incoming {
 
 // --- the kernel ---------------------------------------------------------------
 template <int MODE, typename T, bool PAIR, int BN>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap0,
                 const __grid_constant__ CUtensorMap bmap1, const __grid_constant__ GemmParams p) {
   using namespace tc;
   using S = GemmShape<T, PAIR, BN>;
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   constexpr int P = std::is_same<T, float>::value ? 3 : 1;  // planes
-  constexpr int kStages = S::kStages;
+  constexpr int kStages = S::kStages, kEpiWarps = S::kEpiWarps;
   constexpr int kTileRows = PAIR ? 256 : 128;
   constexpr int kTileCols = MODE == kGated ? BN / 2 : BN;
   constexpr int kWarpCols = BN / 2;  // accumulator columns per epilogue warp
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* staging = tiles + kStages * S::kStageBytes;
   float* bias_all = reinterpret_cast<float*>(staging + kEpiWarps * 2048);
-  uint64_t* full = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * 128);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * kWarpCols);
   uint64_t* empty = full + kStages;   // the MMAs have read the stage
   uint64_t* tfull = empty + kStages;  // [2] accumulator ready
   uint64_t* tempty = tfull + 2;       // [2] accumulator drained (issuing CTA's count)
@@ -479,8 +482,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
-    const int quarter = warp & 3, ew = warp - 2, half = ew >> 2;
-    float* bias_s = bias_all + ew * 128;
+    const int quarter = warp & 3, ew = warp - 2, group = ew >> 2;
+    float* bias_s = bias_all + ew * kWarpCols;
     const uint32_t buf = smem_u32(staging + ew * 2048);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tfull_at = smem_u32(tfull);
@@ -509,17 +512,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // Accumulator column of chunk c: plain modes take the warp's half from left
     // to right; the gated mode alternates gate and up of the same outputs.
     constexpr int kChunks = kWarpCols / 32;
+    constexpr int kOutCols = MODE == kGated ? kWarpCols / 2 : kWarpCols;  // output columns
     auto acc_col = [&](int c) {
-      return MODE == kGated ? (c & 1) * (BN / 2) + half * (BN / 4) + (c >> 1) * 32
-                            : half * kWarpCols + c * 32;
+      return MODE == kGated ? (c & 1) * (BN / 2) + group * kOutCols + (c >> 1) * 32
+                            : group * kWarpCols + c * 32;
     };
     constexpr int kStep = MODE == kGated ? 2 : 1;
     for (int i = worker; i < items; i += workers) {
       const Item it = item_of(i);
       const int64_t row0 = (int64_t)it.tm * kTileRows + rank * kBM + quarter * 32;
       const int rows = (int)max((int64_t)0, min((int64_t)32, p.rows - row0));
-      const int64_t warp_col =
-          (int64_t)it.tn * kTileCols + half * (MODE == kGated ? BN / 4 : kWarpCols);
+      const int64_t warp_col = (int64_t)it.tn * kTileCols + group * kOutCols;
       const int64_t cols = p.cols - warp_col;  // from the warp's first one (may be negative)
       const T* res = MODE == kLinear && p.splits == 1 && p.residual
                          ? static_cast<const T*>(p.residual) + row0 * p.ldr + warp_col
@@ -529,80 +532,81 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       if constexpr (MODE == kLinear || MODE == kGated) {
         // The warp's biases: its columns' in order (gated: gate, then up).
         __syncwarp();
-        constexpr int kBiases = MODE == kGated ? BN / 4 : kWarpCols;
-        for (int c = lane; c < kBiases; c += 32) {
+        for (int c = lane; c < kOutCols; c += 32) {
           const bool has = c < cols;
           bias_s[c] = has && p.bias[0] ? to_f(static_cast<const T*>(p.bias[0])[warp_col + c]) : 0.f;
           if constexpr (MODE == kGated)
-            bias_s[kBiases + c] =
+            bias_s[kOutCols + c] =
                 has && p.bias[1] ? to_f(static_cast<const T*>(p.bias[1])[warp_col + c]) : 0.f;
         }
         __syncwarp();
       }
-      // Finishes 32 columns (gated: v the gate's, u the up's sums).
-      auto finish = [&](int c, float (&v)[32], float (&u)[32]) {
+      // Finishes 32 columns: v the sums (gated: the gate's; up() then gives the
+      // up's, late, so that both are not held at once).
+      auto finish = [&](int c, float (&v)[32], auto&& up) {
         const int at = (MODE == kGated ? c >> 1 : c) * 32;
         const int n = (int)min((int64_t)32, cols - at);
-        if (n <= 0) return;
         const int64_t col = warp_col + at;
         if (p.splits > 1) {
           constexpr int kPlanes = MODE == kGated ? 2 : 1;
           float* dst = p.partial +
                        ((int64_t)(it.split * p.batches + it.batch) * kPlanes * p.rows + row0) *
                            p.ldp + col;
-          emit(buf, dst, p.ldp, rows, 32, true, v, lane);
-          if constexpr (MODE == kGated)
-            emit(buf, dst + p.rows * p.ldp, p.ldp, rows, 32, true, u, lane);
+          if (n > 0) emit(buf, dst, p.ldp, rows, 32, true, v, lane);
+          if constexpr (MODE == kGated) {
+            up(v);
+            if (n > 0) emit(buf, dst + p.rows * p.ldp, p.ldp, rows, 32, true, v, lane);
+          }
           return;
         }
-        if constexpr (MODE == kLinear || MODE == kGated) {
-          const float4* b = reinterpret_cast<const float4*>(bias_s + at);
+        // Bias and the saved pre-activation of the first or second sums.
+        auto affine = [&](int which, float (&x)[32]) {
+          const float4* b = reinterpret_cast<const float4*>(bias_s + which * kOutCols + at);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float4 t = b[j];
-            v[4 * j] += t.x, v[4 * j + 1] += t.y, v[4 * j + 2] += t.z, v[4 * j + 3] += t.w;
+            x[4 * j] += t.x, x[4 * j + 1] += t.y, x[4 * j + 2] += t.z, x[4 * j + 3] += t.w;
           }
-          const int64_t save = row0 * p.lds + col;
-          if (p.save[0])
-            emit(buf, static_cast<T*>(p.save[0]) + save, p.lds, rows, n, vec, v, lane);
-          if constexpr (MODE == kGated) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 t = b[BN / 16 + j];
-              u[4 * j] += t.x, u[4 * j + 1] += t.y, u[4 * j + 2] += t.z, u[4 * j + 3] += t.w;
-            }
-            if (p.save[1])
-              emit(buf, static_cast<T*>(p.save[1]) + save, p.lds, rows, n, vec, u, lane);
-          }
+          if (p.save[which] && n > 0)
+            emit(buf, static_cast<T*>(p.save[which]) + row0 * p.lds + col, p.lds, rows, n, vec, x,
+                 lane);
+        };
+        if constexpr (MODE == kLinear || MODE == kGated) {
+          affine(0, v);
           activate_all<T>(p.act, v);
-          if constexpr (MODE == kGated) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= u[j];
-          } else if (res) {
-            in.add(buf, res + at, p.ldr, rows, n, vec && n == 32, v, lane);
-            if (c + 1 < kChunks)
-              in.start(res + at + 32, p.ldr, rows, vec && cols >= at + 64, lane);
-          }
         }
-        emit(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col, p.ldo,
-             rows, n, vec, v, lane);
+        if constexpr (MODE == kGated) {
+          float u[32];
+          up(u);
+          affine(1, u);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= u[j];
+        }
+        if (MODE == kLinear && res && n > 0) {
+          in.add(buf, res + at, p.ldr, rows, n, vec && n == 32, v, lane);
+          if (c + 1 < kChunks) in.start(res + at + 32, p.ldr, rows, vec && cols >= at + 64, lane);
+        }
+        if (n > 0)
+          emit(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col, p.ldo,
+               rows, n, vec, v, lane);
       };
       if constexpr (P == 1) {
         if (!wait_round()) break;
         const uint32_t t = tmem_base + (round & 1) * S::kAccCols + lanes;
 #pragma unroll 1
         for (int c = 0; c < kChunks; c += kStep) {
-          uint32_t raw[kStep][32];
+          // One accumulator chunk; the last one frees the accumulator.
+          auto chunk = [&](int c, float (&v)[32]) {
+            uint32_t raw[32];
+            tmem_ld32(t + acc_col(c), raw);
+            tmem_wait_ld();
+            if (c == kChunks - 1) release_round();
 #pragma unroll
-          for (int s = 0; s < kStep; ++s) tmem_ld32(t + acc_col(c + s), raw[s]);
-          tmem_wait_ld();
-          if (c + kStep >= kChunks) release_round();
-          float v[kStep][32];
-#pragma unroll
-          for (int s = 0; s < kStep; ++s)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[s][j] = __uint_as_float(raw[s][j]);
-          finish(c, v[0], v[kStep - 1]);
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+          };
+          float v[32];
+          chunk(c, v);
+          finish(c, v, [&](float (&u)[32]) { chunk(c + 1, u); });
         }
       } else {
         float sum[kChunks][32];
@@ -627,7 +631,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < kChunks; c += kStep) finish(c, sum[c], sum[c + kStep - 1]);
+        for (int c = 0; c < kChunks; c += kStep)
+          finish(c, sum[c], [&](float (&u)[32]) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] = sum[c + kStep - 1][j];
+          });
       }
     }
   }
@@ -756,7 +764,7 @@ xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaS
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.batches * p.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)std::min<int64_t>(items, workers) * (PAIR ? 2 : 1));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmemBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

@@ -2,10 +2,17 @@
 //
 //   norm = sqrt(sum over all tensors of x^2),  out = x min(1, max_norm / norm)
 //
-// Bound by memory: every element is read once for the norm and once for the
-// scaling, and written once.  The tensors are cut into chunks of kChunk
-// elements; a block owns whole chunks, so the order of the sums depends on the
-// sizes alone and results repeat.
+// Two launches, both bound by memory.  The tensors are cut into chunks of 32 KB;
+// block b takes chunks b, b + blocks, ...: the first launch leaves one float64 sum
+// of squares per block, the second adds them (every block for itself, which
+// saves a launch) and scales, its chunks in the opposite order, so that the
+// last ones that the first launch read still lie in L2.  Which block adds
+// what depends on the sizes alone, so results repeat.
+//
+// Squares: a 16-byte vector's are summed in float32 and added up in float64; a
+// vector whose sum leaves float32's comfortable range (values around 1e-19 or
+// 1e19, and what is not finite) is squared in float64, so that neither overflow
+// nor underflow of a square matters.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -16,9 +23,9 @@ namespace xvec {
 namespace adapter {
 namespace {
 
-constexpr int kChunk = 16384;  // elements
+constexpr int kChunkBytes = 32768;
 constexpr int kThreads = 256;
-constexpr int kMaxEntries = 500;  // per launch: the table travels as a kernel parameter
+constexpr int kBlocksPerSm = 6;
 
 struct Entry {
   const void* in;
@@ -27,29 +34,22 @@ struct Entry {
   int32_t storage;
   uint32_t first_chunk;  // of this launch
 };
+// Travels as a kernel parameter; two sizes, since a launch pays for its bytes.
+template <int N>
 struct Table {
   int entries;
   uint32_t chunks;
-  Entry e[kMaxEntries];
+  Entry e[N];
 };
+constexpr int kFew = 32, kMany = 500;
 
-__device__ __forceinline__ float load_as_float(const Entry& e, int64_t i) {
-  switch (e.storage) {
-    case XVEC_STORAGE_FP32: return static_cast<const float*>(e.in)[i];
-    case XVEC_STORAGE_FP16: return to_f(static_cast<const __half*>(e.in)[i]);
-    default: return to_f(static_cast<const bf16*>(e.in)[i]);
-  }
-}
-__device__ __forceinline__ void store_from_float(const Entry& e, int64_t i, float v) {
-  switch (e.storage) {
-    case XVEC_STORAGE_FP32: static_cast<float*>(e.out)[i] = v; break;
-    case XVEC_STORAGE_FP16: static_cast<__half*>(e.out)[i] = from_f<__half>(v); break;
-    default: static_cast<bf16*>(e.out)[i] = from_f<bf16>(v);
-  }
+__host__ __device__ constexpr int chunk_elems(int storage) {
+  return storage == XVEC_STORAGE_FP32 ? kChunkBytes / 4 : kChunkBytes / 2;
 }
 
 // The entry of a chunk: the last whose first chunk is at or before it.
-__device__ __forceinline__ int entry_of(const Table& t, uint32_t chunk) {
+template <int N>
+__device__ __forceinline__ int entry_of(const Table<N>& t, uint32_t chunk) {
   int lo = 0, hi = t.entries - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -59,94 +59,199 @@ __device__ __forceinline__ int entry_of(const Table& t, uint32_t chunk) {
   return lo;
 }
 
-// Sum of v over the block, on thread 0.
+// Sum of v over the block in a fixed order, on every thread.
 __device__ __forceinline__ double block_sum(double v) {
   __shared__ double part[kThreads / 32];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_down_sync(0xffffffffu, v, o);
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
-  if (threadIdx.x == 0)
-    for (int i = 1; i < kThreads / 32; ++i) v += part[i];
+  v = part[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) v += part[i];
   return v;
 }
 
-// sums[chunk] = the chunk's sum of squares, in float64.
-__global__ void __launch_bounds__(kThreads)
-    square_sum_kernel(const __grid_constant__ Table t, double* sums) {
-  const Entry& e = t.e[entry_of(t, blockIdx.x)];
-  const int64_t i0 = (int64_t)(blockIdx.x - e.first_chunk) * kChunk;
-  const int64_t i1 = min(e.count, i0 + kChunk);
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& u, float (&v)[16 / sizeof(T)]) {
+  const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int j = 0; j < 16 / (int)sizeof(T); ++j) v[j] = to_f(t[j]);
+}
+
+// Sum of the squares of one 16-byte vector.
+template <typename T>
+__device__ __forceinline__ double vector_squares(const uint4& u) {
+  constexpr int N = 16 / sizeof(T);
+  float v[N];
+  unpack<T>(u, v);
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) s = fmaf(v[j], v[j], s);
+  if constexpr (!std::is_same<T, __half>::value) {
+    if (!(s >= 1e-30f && s <= 1e37f)) {
+      double d = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) d = fma((double)v[j], (double)v[j], d);
+      return d;
+    }
+  }
+  return s;
+}
+
+// Elements [i0, i1) of a tensor: the vectors between 16-byte boundaries, and
+// the few elements before and after them one by one.
+template <typename T>
+__device__ __forceinline__ double square_range(const T* in, int64_t i0, int64_t i1) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t head = min(i1, i0 + (int64_t)((16 - (uintptr_t)(in + i0) % 16) % 16 / sizeof(T)));
+  const int vectors = (int)((i1 - head) / N);
+  const uint4* p = reinterpret_cast<const uint4*>(in + head);
+  double s0 = 0, s1 = 0;
+  int i = threadIdx.x;
+  for (; i + 3 * kThreads < vectors; i += 4 * kThreads) {
+    const uint4 a = __ldg(p + i), b = __ldg(p + i + kThreads);
+    const uint4 c = __ldg(p + i + 2 * kThreads), d = __ldg(p + i + 3 * kThreads);
+    s0 += vector_squares<T>(a);
+    s1 += vector_squares<T>(b);
+    s0 += vector_squares<T>(c);
+    s1 += vector_squares<T>(d);
+  }
+  for (; i < vectors; i += kThreads) s0 += vector_squares<T>(__ldg(p + i));
+  const int64_t tail = head + (int64_t)vectors * N;
+  const int64_t e = threadIdx.x < head - i0 ? i0 + threadIdx.x : tail + threadIdx.x - (head - i0);
+  if (e < i1) {
+    const double v = to_f(in[e]);
+    s1 = fma(v, v, s1);
+  }
+  return s0 + s1;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 scaled(const uint4& u, float f) {
+  constexpr int N = 16 / sizeof(T);
+  float v[N];
+  unpack<T>(u, v);
+  uint4 r;
+  T* t = reinterpret_cast<T*>(&r);
+#pragma unroll
+  for (int j = 0; j < N; ++j) t[j] = from_f<T>(v[j] * f);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_range(const T* in, T* out, int64_t i0, int64_t i1, float f) {
+  constexpr int N = 16 / sizeof(T);
+  if (((uintptr_t)in ^ (uintptr_t)out) % 16) {  // no common 16-byte boundaries
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads) out[i] = from_f<T>(to_f(in[i]) * f);
+    return;
+  }
+  const int64_t head = min(i1, i0 + (int64_t)((16 - (uintptr_t)(in + i0) % 16) % 16 / sizeof(T)));
+  const int vectors = (int)((i1 - head) / N);
+  const uint4* p = reinterpret_cast<const uint4*>(in + head);
+  uint4* q = reinterpret_cast<uint4*>(out + head);
+  int i = threadIdx.x;
+  for (; i + 3 * kThreads < vectors; i += 4 * kThreads) {
+    const uint4 a = p[i], b = p[i + kThreads], c = p[i + 2 * kThreads], d = p[i + 3 * kThreads];
+    q[i] = scaled<T>(a, f);
+    q[i + kThreads] = scaled<T>(b, f);
+    q[i + 2 * kThreads] = scaled<T>(c, f);
+    q[i + 3 * kThreads] = scaled<T>(d, f);
+  }
+  for (; i < vectors; i += kThreads) q[i] = scaled<T>(p[i], f);
+  const int64_t tail = head + (int64_t)vectors * N;
+  const int64_t e = threadIdx.x < head - i0 ? i0 + threadIdx.x : tail + threadIdx.x - (head - i0);
+  if (e < i1) out[e] = from_f<T>(to_f(in[e]) * f);
+}
+
+// sums[block] = the sum of squares of the block's chunks.
+template <int N>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+    square_sum_kernel(const __grid_constant__ Table<N> t, double* sums) {
   double s = 0;
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads) {
-    const double v = load_as_float(e, i);
-    s += v * v;
+  for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const Entry& e = t.e[entry_of(t, c)];
+    const int64_t i0 = (int64_t)(c - e.first_chunk) * chunk_elems(e.storage);
+    const int64_t i1 = min(e.count, i0 + chunk_elems(e.storage));
+    if (e.storage == XVEC_STORAGE_FP32)
+      s += square_range(static_cast<const float*>(e.in), i0, i1);
+    else if (e.storage == XVEC_STORAGE_FP16)
+      s += square_range(static_cast<const __half*>(e.in), i0, i1);
+    else
+      s += square_range(static_cast<const bf16*>(e.in), i0, i1);
   }
   s = block_sum(s);
   if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
-// norm and the scale, from all chunks' sums.
-__global__ void __launch_bounds__(kThreads)
-    norm_kernel(const double* sums, int64_t chunks, double max_norm, float* norm, float* scale) {
+template <int N>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+    scale_kernel(const __grid_constant__ Table<N> t, const double* sums, int num_sums,
+                 double max_norm, float* norm) {
   double s = 0;
-  for (int64_t i = threadIdx.x; i < chunks; i += kThreads) s += sums[i];
-  s = block_sum(s);
-  if (threadIdx.x == 0) {
-    const double n = sqrt(s);
-    *norm = (float)n;
-    *scale = isfinite(n) && n > max_norm ? (float)(max_norm / n) : 1.f;
+  for (int i = threadIdx.x; i < num_sums; i += kThreads) s += sums[i];
+  const double n = sqrt(block_sum(s));
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  const float f = isfinite(n) && n > max_norm ? (float)(max_norm / n) : 1.f;
+  if (blockIdx.x >= t.chunks) return;
+  for (uint32_t c = blockIdx.x + (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x;;
+       c -= gridDim.x) {
+    const Entry& e = t.e[entry_of(t, c)];
+    if (f != 1.f || e.in != e.out) {
+      const int64_t i0 = (int64_t)(c - e.first_chunk) * chunk_elems(e.storage);
+      const int64_t i1 = min(e.count, i0 + chunk_elems(e.storage));
+      if (e.storage == XVEC_STORAGE_FP32)
+        scale_range(static_cast<const float*>(e.in), static_cast<float*>(e.out), i0, i1, f);
+      else if (e.storage == XVEC_STORAGE_FP16)
+        scale_range(static_cast<const __half*>(e.in), static_cast<__half*>(e.out), i0, i1, f);
+      else
+        scale_range(static_cast<const bf16*>(e.in), static_cast<bf16*>(e.out), i0, i1, f);
+    }
+    if (c < gridDim.x) break;
   }
 }
 
-__global__ void __launch_bounds__(kThreads)
-    scale_kernel(const __grid_constant__ Table t, const float* scale) {
-  const Entry& e = t.e[entry_of(t, blockIdx.x)];
-  const float f = *scale;
-  if (f == 1.f && e.in == e.out) return;
-  const int64_t i0 = (int64_t)(blockIdx.x - e.first_chunk) * kChunk;
-  const int64_t i1 = min(e.count, i0 + kChunk);
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads)
-    store_from_float(e, i, load_as_float(e, i) * f);
-}
-
+// Launches over all tensors, N at a time: sums (pass 0) and scaling (pass 1).
+template <int N>
 xvec_gpu_status clip(const xvec_gpu_tensor* tensors, int num, double max_norm, float* d_norm,
-                     cudaStream_t s) {
-  int64_t chunks = 0;
-  for (int i = 0; i < num; ++i) chunks += (tensors[i].count + kChunk - 1) / kChunk;
-  Scratch sums, scale;
-  xvec_gpu_status st;
-  if ((st = sums.alloc((size_t)chunks * 8, s)) || (st = scale.alloc(4, s))) return st;
-  Table t;
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t done = 0;
-    for (int i = 0; i < num;) {
-      t.entries = 0;
-      t.chunks = 0;
-      for (; i < num && t.entries < kMaxEntries; ++i) {
-        const int64_t c = (tensors[i].count + kChunk - 1) / kChunk;
-        if (c == 0) continue;
-        if (t.chunks + c > 0x7fffffff) break;
-        t.e[t.entries++] = {tensors[i].in, tensors[i].out, tensors[i].count, tensors[i].storage,
-                            t.chunks};
-        t.chunks += (uint32_t)c;
-      }
-      if (t.entries == 0) continue;
-      if (pass == 0)
-        square_sum_kernel<<<t.chunks, kThreads, 0, s>>>(t, sums.as<double>() + done);
-      else
-        scale_kernel<<<t.chunks, kThreads, 0, s>>>(t, scale.as<float>());
-      XVEC_LAUNCHED();
-      XVEC_CUDA(cudaGetLastError());
-      done += t.chunks;
+                     int sms, cudaStream_t s) {
+  const int max_blocks = sms * kBlocksPerSm;
+  Table<N> t;
+  // Fills t from tensor *i on; false when nothing is left.
+  auto fill = [&](int* i) {
+    t.entries = 0;
+    t.chunks = 0;
+    for (; *i < num && t.entries < N; ++*i) {
+      const xvec_gpu_tensor& x = tensors[*i];
+      const int64_t c = (x.count + chunk_elems(x.storage) - 1) / chunk_elems(x.storage);
+      if (c == 0) continue;
+      if (t.chunks + c > 0x7fffffff) break;
+      t.e[t.entries++] = {x.in, x.out, x.count, x.storage, t.chunks};
+      t.chunks += (uint32_t)c;
     }
-    if (pass == 0) {
-      norm_kernel<<<1, kThreads, 0, s>>>(sums.as<double>(), chunks, max_norm, d_norm,
-                                         scale.as<float>());
-      XVEC_LAUNCHED();
-      XVEC_CUDA(cudaGetLastError());
-    }
+    return t.entries > 0;
+  };
+  int blocks = 0;
+  for (int i = 0; fill(&i);) blocks += (int)std::min<uint32_t>(t.chunks, max_blocks);
+  Scratch sums;
+  if (xvec_gpu_status st = sums.alloc((size_t)blocks * 8, s)) return st;
+  int done = 0;
+  for (int i = 0; fill(&i);) {
+    const int b = (int)std::min<uint32_t>(t.chunks, max_blocks);
+    square_sum_kernel<N><<<b, kThreads, 0, s>>>(t, sums.as<double>() + done);
+    XVEC_LAUNCHED();
+    XVEC_CUDA(cudaGetLastError());
+    done += b;
+  }
+  int i = 0;
+  for (int pass = 0; fill(&i) || pass == 0; ++pass) {
+    const int b = std::max(1, (int)std::min<uint32_t>(t.chunks, max_blocks));
+    scale_kernel<N><<<b, kThreads, 0, s>>>(t, sums.as<double>(), blocks, max_norm,
+                                           pass == 0 ? d_norm : nullptr);
+    XVEC_LAUNCHED();
+    XVEC_CUDA(cudaGetLastError());
+    if (t.entries == 0) break;
   }
   return XVEC_GPU_OK;
 }
@@ -215,5 +320,9 @@ extern "C" xvec_gpu_status xvec_gpu_clip_gradients_device(int32_t device,
   if (bad) return invalid("an output overlaps another tensor");
   DeviceGuard guard;
   if (xvec_gpu_status st = guard.set(device)) return st;
-  return clip(tensors, num_tensors, max_norm, d_norm, static_cast<cudaStream_t>(stream));
+  int sms = 0;
+  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return num_tensors <= kFew ? clip<kFew>(tensors, num_tensors, max_norm, d_norm, sms, s)
+                             : clip<kMany>(tensors, num_tensors, max_norm, d_norm, sms, s);
 }
