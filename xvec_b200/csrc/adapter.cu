@@ -24,28 +24,6 @@ constexpr int64_t kMaxDim = 1 << 20;
 constexpr int kMaxDevices = 64;
 
 // --- operands -----------------------------------------------------------------
-// Eight elements of a row as floats, from an address that may be unaligned
-// (vec = false) and of which only `count` exist (the rest 0).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
-  if (vec && count >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0];
-      const float4 b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f(t[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_f(p[j]) : 0.f;
-  }
-}
-
 // Eight values as operand elements at dst: 16-bit types as they are; float32
 // as three bfloat16 parts x = h + m + l in planes `plane` elements apart, each
 // the nearest to what is left (exact: 8 bits each and the parts' signs).
@@ -93,9 +71,6 @@ __global__ void __launch_bounds__(256)
 }
 
 size_t elem_bytes(int storage) { return storage == XVEC_STORAGE_FP32 ? 4 : 2; }
-bool aligned16(const void* p, int64_t ld, size_t size) {
-  return (uintptr_t)p % 16 == 0 && ld * (int64_t)size % 16 == 0;
-}
 int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
 int planes_of(int storage) { return storage == XVEC_STORAGE_FP32 ? 3 : 1; }
 
@@ -447,6 +422,14 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
   cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+  if (a.n <= kFewRows) {
+    FewRows f{};
+    f.n = (int)a.n, f.in_dim = a.in_dim, f.out_dim = a.out_dim, f.act = a.activation;
+    f.x = a.x, f.w[0] = a.weight, f.bias[0] = a.bias, f.residual = a.residual;
+    f.out = a.y, f.save[0] = a.preact;
+    f.ldx = a.ldx, f.ldw = a.ldw, f.ldr = a.ldr, f.ldo = a.ldy, f.lds = a.ldz;
+    return few_rows(a.storage, f, s);
+  }
   GemmCall g;
   g.mode = kLinear;
   g.depth = a.in_dim;
@@ -493,6 +476,15 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
   cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+  if (a.n <= kFewRows) {
+    FewRows f{};
+    f.n = (int)a.n, f.in_dim = a.in_dim, f.out_dim = a.out_dim, f.act = a.activation;
+    f.x = a.x, f.w[0] = a.gate_weight, f.w[1] = a.up_weight;
+    f.bias[0] = a.gate_bias, f.bias[1] = a.up_bias;
+    f.out = a.h, f.save[0] = a.gate, f.save[1] = a.up;
+    f.ldx = a.ldx, f.ldw = a.ldw, f.ldo = a.ldh, f.lds = a.ldg;
+    return few_rows(a.storage, f, s);
+  }
   GemmCall g;
   g.mode = kGated;
   g.depth = a.in_dim;

@@ -143,6 +143,28 @@ __device__ __forceinline__ float activate_slope(int act, float z, float* slope) 
   }
 }
 
+// Eight elements of a row as floats, from an address that may be unaligned
+// (vec = false) and of which only `count` exist (the rest 0).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
+  if (vec && count >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0];
+      const float4 b = reinterpret_cast<const float4*>(p)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_f(t[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_f(p[j]) : 0.f;
+  }
+}
+
 // Makes `device` current for one call and restores the caller's.
 struct DeviceGuard {
   int before = -1;
@@ -201,6 +223,21 @@ struct GemmCall {
 xvec_gpu_status gemm_fp32(const GemmCall& c, cudaStream_t s);
 xvec_gpu_status gemm_fp16(const GemmCall& c, cudaStream_t s);
 xvec_gpu_status gemm_bf16(const GemmCall& c, cudaStream_t s);
+
+// Rows read in place with 16-byte accesses.
+inline bool aligned16(const void* p, int64_t ld, size_t size) {
+  return (uintptr_t)p % 16 == 0 && ld * (int64_t)size % 16 == 0;
+}
+
+// The forward calls for a few rows (adapter_few.cu): kLinear, or with two weights kGated.
+constexpr int kFewRows = 8;
+struct FewRows {
+  int n, in_dim, out_dim, act;
+  const void *x, *w[2], *bias[2], *residual;
+  void *out, *save[2];
+  int64_t ldx, ldw, ldr, ldo, lds;
+};
+xvec_gpu_status few_rows(int storage, const FewRows& f, cudaStream_t s);
 
 }  // namespace adapter
 }  // namespace xvec
