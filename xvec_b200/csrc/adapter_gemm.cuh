@@ -9,12 +9,12 @@
 // so no operand is ever transposed in memory: the matrix instruction reads
 // either order from shared memory.
 //
-//   CTA = 10 warps, persistent over tiles, one CTA per SM:
-//     warp 0    TMA producer: 64 deep blocks of A (128 rows) and B into a ring of
-//               stages (128-byte swizzle)
-//     warp 1    tensor memory; one thread issues tcgen05.mma (fp32 accumulators,
-//               two of them, so that a tile's epilogue overlaps the next tile)
-//     warps 2-9 epilogue: tcgen05.ld, bias, activation, product, residual
+//   CTA = 12 warps, persistent over tiles, one CTA per SM:
+//     warp 0     TMA producer: 64 deep blocks of A (128 rows) and B into a ring of
+//                stages (128-byte swizzle)
+//     warp 1     tensor memory; one thread issues tcgen05.mma (fp32 accumulators,
+//                two of them, so that a tile's epilogue overlaps the next tile)
+//     warps 4-11 epilogue: tcgen05.ld, bias, activation, product, residual
 //   PAIR: two CTAs (cta_group::2) share a tile of 256 rows x BN columns, each
 //   loading half of A's rows and half of B's columns.
 //
@@ -23,9 +23,13 @@
 // plane of A and of B, and the six products hh, hm, mh, mm, hl, lh are issued
 // (what is left out is below 2^-24 of the product).  The accumulator's own
 // additions truncate (measured: 48 of them leave 1.1e-6 of the 2-norm at depth
-// 960), so hh has an accumulator of its own, the five small products another,
-// and both leave tensor memory every kRound blocks to be added in registers
-// (8 truncations of the large sum instead of 48).
+// 960), so hh has an accumulator of its own that leaves tensor memory every
+// kRound blocks to be added in registers (8 truncations instead of 48), and the
+// five products that are 2^8 times smaller have another that leaves at the end.
+// hh is drained while the small products of the same block are issued, so one
+// accumulator of each suffices and the tile keeps 256 columns: at 128 an
+// instruction waits for its operands in shared memory (105 clocks, not 64).
+// The drained sums take the registers that the other warps give up (setmaxnreg).
 //
 // Every mbarrier wait is bounded; on expiry the kernel sets *status, stops
 // issuing work, drains its own copies and frees its tensor memory.
@@ -46,6 +50,7 @@ constexpr int kBM = 128;      // rows per CTA (TMEM lanes)
 constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr int kBand = 8;      // row tiles per band of the tile order
+constexpr int kFewRegs = 40, kManyRegs = 232;
 constexpr int kRound = 2;     // float32: depth blocks per accumulation in tensor memory
 
 template <typename T, bool PAIR, int BN>
@@ -54,9 +59,7 @@ struct GemmShape {
   // on 256 columns cost a stage of the ring and were slower: 131072 x 1024 -> 1024
   // fp16 with silu and residual 360 us against 336.)
   static constexpr int kEpiWarps = 8;
-  static constexpr int kThreads = 64 + kEpiWarps * 32;
-  // Accumulators of one round: the sums, and for float32 the small products'.
-  static constexpr int kAccCols = std::is_same<T, float>::value ? 2 * BN : BN;
+  static constexpr int kThreads = 128 + kEpiWarps * 32;
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B columns loaded per CTA
   static constexpr uint32_t kBBytes = kBRows * kBK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
@@ -65,7 +68,7 @@ struct GemmShape {
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + 512;
-  static constexpr int kTmemCols = 2 * kAccCols;
+  static constexpr int kTmemCols = 2 * BN;  // two accumulators
   static_assert(kStages >= 4, "shared memory too small for the stage ring");
 };
 
@@ -158,6 +161,16 @@ __device__ __forceinline__ void commit(uint32_t bar) {
         : "memory");
   else
     tc::mma_commit<false>(bar);
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
 }
 
 // --- epilogue input and output ------------------------------------------------------
@@ -299,7 +312,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
   float* bias_all = reinterpret_cast<float*>(staging + kEpiWarps * 2048);
   uint64_t* full = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * kWarpCols);
   uint64_t* empty = full + kStages;   // the MMAs have read the stage
-  uint64_t* tfull = empty + kStages;  // [2] accumulator ready
+  uint64_t* tfull = empty + kStages;  // [2] accumulator ready (float32: hh, small)
   uint64_t* tempty = tfull + 2;       // [2] accumulator drained (issuing CTA's count)
   uint64_t* mdone = tempty + 2;       // all issued MMAs retired
   uint32_t* issued = reinterpret_cast<uint32_t*>(mdone + 1);  // [kStages] copies per stage
@@ -373,9 +386,11 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
     return it;
   };
 
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
-    if (lane == 0) {
+  // float32: 384 threads of 168 registers become 128 of kFewRegs and 256 of kManyRegs.
+  if (warp < 4) {
+    if constexpr (P == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    if (warp == 0 && lane == 0) {
+      // ---------------- TMA producer ----------------
       const uint32_t tiles_at = smem_u32(tiles), empty_at = smem_u32(empty);
       const uint32_t full_at = smem_u32(full), bars = PAIR ? cluster_addr(full, 0) : full_at;
       uint32_t stage = 0, phase = 0, count = 0;  // count: stages filled
@@ -422,57 +437,70 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
       if (!ok) fail();
       for (uint32_t s = 0; s < kStages; ++s)
         issued[s] = count / kStages + (s < count % kStages ? 1 : 0);
-    }
-  } else if (warp == 1 && issuer) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    } else if (warp == 1 && lane == 0 && issuer) {
+      // ---------------- MMA issuer ----------------
       const uint32_t full_at = smem_u32(full), empty_at = smem_u32(empty);
       const uint32_t tfull_at = smem_u32(tfull), tempty_at = smem_u32(tempty);
       const uint64_t a0 = kTileDesc<A_MN> + (smem_u32(tiles) >> 4);
       const uint64_t b0 = kTileDesc<B_MN> + ((smem_u32(tiles) + kABytes) >> 4);
-      uint32_t stage = 0, phase = 0, round = 0;
+      uint32_t stage = 0, phase = 0;
       bool ok = true;
-      for (int i = worker; i < items && ok; i += workers) {
+      // Waits for the next stage; its number.
+      auto next = [&](uint32_t* at) {
+        *at = stage;
+        const bool got = wait_bar(full_at + stage * 8, phase, s_abort, limit);
+        if (++stage == kStages) stage = 0, phase ^= 1;
+        tmem_fence_after();
+        return got;
+      };
+      // A's plane in stage i times B's in stage j, into d; keep = 0 overwrites it.
+      auto multiply = [&](uint32_t i, uint32_t j, uint32_t d, uint32_t keep) {
+        const uint64_t a = a0 + i * (S::kStageBytes >> 4), b = b0 + j * (S::kStageBytes >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_16bit<PAIR>(d, a + k * kDepthStep<A_MN>, b + k * kDepthStep<B_MN>, p.idesc,
+                          k == 0 ? keep : 1u);
+      };
+      uint32_t round = 0, tile = 0;
+      for (int i = worker; i < items && ok; i += workers, ++tile) {
         const Item it = item_of(i);
-        const int per = P == 1 ? it.k1 - it.k0 : kRound;
-        for (int r0 = it.k0; r0 < it.k1 && ok; r0 += per, ++round) {
-          const uint32_t acc = round & 1;
-          if (!(ok = wait_bar(tempty_at + acc * 8, ((round >> 1) & 1) ^ 1, s_abort, limit))) break;
+        if constexpr (P == 1) {
+          const uint32_t acc = tile & 1, d = tmem_base + acc * BN;
+          if (!(ok = wait_bar(tempty_at + acc * 8, ((tile >> 1) & 1) ^ 1, s_abort, limit))) break;
           tmem_fence_after();
-          const uint32_t d = tmem_base + acc * S::kAccCols;
-          uint32_t first = 0;  // 0: the accumulators are overwritten
-          for (int n = min(it.k1 - r0, per); n > 0 && ok; --n) {
-            uint32_t at[P];
-            auto multiply = [&](int i, int j, uint32_t d, uint32_t keep) {
-              const uint64_t a = a0 + at[i] * (S::kStageBytes >> 4);
-              const uint64_t b = b0 + at[j] * (S::kStageBytes >> 4);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_16bit<PAIR>(d, a + k * kDepthStep<A_MN>, b + k * kDepthStep<B_MN>, p.idesc,
-                                k == 0 ? keep : 1u);
-            };
-#pragma unroll
-            for (int pl = 0; pl < P; ++pl) {
-              at[pl] = stage;
-              if (!(ok = ok && wait_bar(full_at + stage * 8, phase, s_abort, limit))) break;
-              if (++stage == kStages) stage = 0, phase ^= 1;
-              tmem_fence_after();
-              if (pl == 0) multiply(0, 0, d, first);
-              if constexpr (P == 3) {
-                if (pl == 1) {
-                  multiply(1, 1, d + BN, first);
-                  multiply(0, 1, d + BN, 1);
-                  multiply(1, 0, d + BN, 1);
-                }
-                if (pl == 2) multiply(0, 2, d + BN, 1), multiply(2, 0, d + BN, 1);
-              }
-            }
-            first = 1;
-            if (ok)
-#pragma unroll
-              for (int pl = 0; pl < P; ++pl) commit<PAIR>(empty_at + at[pl] * 8);
+          for (int k = it.k0; k < it.k1; ++k) {
+            uint32_t at;
+            if (!(ok = next(&at))) break;
+            multiply(at, at, d, k > it.k0);
+            commit<PAIR>(empty_at + at * 8);
           }
           commit<PAIR>(tfull_at + acc * 8);
+        } else {
+          const uint32_t d = tmem_base, small = tmem_base + BN;
+          for (int k = it.k0; k < it.k1; ++k) {
+            const bool opens = (k - it.k0) % kRound == 0;
+            const bool closes = (k - it.k0) % kRound == kRound - 1 || k + 1 == it.k1;
+            uint32_t h, m, l;
+            if (opens) {
+              if (!(ok = wait_bar(tempty_at, (round & 1) ^ 1, s_abort, limit))) break;
+              ++round;
+            }
+            if (!(ok = next(&h))) break;
+            multiply(h, h, d, !opens);
+            if (closes) commit<PAIR>(tfull_at);
+            if (k == it.k0 && !(ok = wait_bar(tempty_at + 8, (tile & 1) ^ 1, s_abort, limit))) break;
+            if (!(ok = next(&m))) break;
+            multiply(m, m, small, k > it.k0);
+            multiply(h, m, small, 1);
+            multiply(m, h, small, 1);
+            if (!(ok = next(&l))) break;
+            multiply(h, l, small, 1);
+            multiply(l, h, small, 1);
+            commit<PAIR>(empty_at + h * 8);
+            commit<PAIR>(empty_at + m * 8);
+            commit<PAIR>(empty_at + l * 8);
+          }
+          commit<PAIR>(tfull_at + 8);
         }
       }
       if (!ok) fail();
@@ -480,19 +508,19 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
       mma_commit<PAIR>(smem_u32(mdone));
       if (!mbar_wait(mdone, 0, nullptr)) fail();
     }
-  } else if (warp >= 2) {
+  } else {
     // ---------------- epilogue ----------------
-    const int quarter = warp & 3, ew = warp - 2, group = ew >> 2;
+    if constexpr (P == 3) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
+    const int quarter = warp & 3, ew = warp - 4, group = ew >> 2;
     float* bias_s = bias_all + ew * kWarpCols;
     const uint32_t buf = smem_u32(staging + ew * 2048);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tfull_at = smem_u32(tfull);
     const bool vec = p.vec != 0;
-    uint32_t round = 0;
-    // One lane polls; the others wait at the shuffle.
-    auto wait_round = [&] {
+    // Waits for accumulator `acc`.  One lane polls; the others wait at the shuffle.
+    auto wait_acc = [&](uint32_t acc, uint32_t parity) {
       int ok = 1;
-      if (lane == 0 && !wait_bar(tfull_at + (round & 1) * 8, (round >> 1) & 1, s_abort, limit)) {
+      if (lane == 0 && !wait_bar(tfull_at + acc * 8, parity, s_abort, limit)) {
         fail();
         ok = 0;
       }
@@ -500,14 +528,13 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
       tmem_fence_after();
       return ok != 0;
     };
-    auto release_round = [&] {
+    auto release_acc = [&](uint32_t acc) {
       tmem_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_remote(cluster_addr(&tempty[round & 1], 0));
-        else mbar_arrive(&tempty[round & 1]);
+        if constexpr (PAIR) mbar_arrive_remote(cluster_addr(&tempty[acc], 0));
+        else mbar_arrive(&tempty[acc]);
       }
-      ++round;
     };
     // Accumulator column of chunk c: plain modes take the warp's half from left
     // to right; the gated mode alternates gate and up of the same outputs.
@@ -518,7 +545,8 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
                             : group * kWarpCols + c * 32;
     };
     constexpr int kStep = MODE == kGated ? 2 : 1;
-    for (int i = worker; i < items; i += workers) {
+    uint32_t round = 0, tile = 0;
+    for (int i = worker; i < items; i += workers, ++tile) {
       const Item it = item_of(i);
       const int64_t row0 = (int64_t)it.tm * kTileRows + rank * kBM + quarter * 32;
       const int rows = (int)max((int64_t)0, min((int64_t)32, p.rows - row0));
@@ -528,7 +556,8 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
                          ? static_cast<const T*>(p.residual) + row0 * p.ldr + warp_col
                          : nullptr;
       Incoming<T> in;
-      if (MODE == kLinear && res) in.start(res, p.ldr, rows, vec && cols >= 32, lane);
+      // (float32 has no registers for it while it drains.)
+      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, vec && cols >= 32, lane);
       if constexpr (MODE == kLinear || MODE == kGated) {
         // The warp's biases: its columns' in order (gated: gate, then up).
         __syncwarp();
@@ -583,16 +612,17 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
           for (int j = 0; j < 32; ++j) v[j] *= u[j];
         }
         if (MODE == kLinear && res && n > 0) {
+          if (P == 3) in.start(res + at, p.ldr, rows, vec && n == 32, lane);
           in.add(buf, res + at, p.ldr, rows, n, vec && n == 32, v, lane);
-          if (c + 1 < kChunks) in.start(res + at + 32, p.ldr, rows, vec && cols >= at + 64, lane);
+          if (P == 1 && c + 1 < kChunks) in.start(res + at + 32, p.ldr, rows, vec && cols >= at + 64, lane);
         }
         if (n > 0)
           emit(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col, p.ldo,
                rows, n, vec, v, lane);
       };
       if constexpr (P == 1) {
-        if (!wait_round()) break;
-        const uint32_t t = tmem_base + (round & 1) * S::kAccCols + lanes;
+        const uint32_t acc = tile & 1, t = tmem_base + acc * BN + lanes;
+        if (!wait_acc(acc, (tile >> 1) & 1)) break;
 #pragma unroll 1
         for (int c = 0; c < kChunks; c += kStep) {
           // One accumulator chunk; the last one frees the accumulator.
@@ -600,7 +630,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
             uint32_t raw[32];
             tmem_ld32(t + acc_col(c), raw);
             tmem_wait_ld();
-            if (c == kChunks - 1) release_round();
+            if (c == kChunks - 1) release_acc(acc);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
           };
@@ -610,32 +640,43 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
         }
       } else {
         float sum[kChunks][32];
-        bool ok = true;
-        for (int r0 = it.k0; r0 < it.k1; r0 += kRound) {
-          if (!(ok = wait_round())) break;
-          const uint32_t t = tmem_base + (round & 1) * S::kAccCols + lanes;
+        auto drain = [&](uint32_t t, bool first) {
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            uint32_t raw[32];
-            tmem_ld32(t + acc_col(c), raw);
+          for (int c = 0; c < 2 * kChunks; ++c) {
+            uint32_t raw[16];
+            tmem_ld16(t + lanes + acc_col(c >> 1) + (c & 1) * 16, raw);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              sum[c][j] = r0 == it.k0 ? __uint_as_float(raw[j]) : sum[c][j] + __uint_as_float(raw[j]);
-            tmem_ld32(t + BN + acc_col(c), raw);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c][j] += __uint_as_float(raw[j]);
+            for (int j = 0; j < 16; ++j) {
+              float& f = sum[c >> 1][(c & 1) * 16 + j];
+              f = first ? __uint_as_float(raw[j]) : f + __uint_as_float(raw[j]);
+            }
           }
-          release_round();
+        };
+        bool ok = true;
+        for (int k = it.k0; k < it.k1 && ok; k += kRound, ++round) {
+          if (!(ok = wait_acc(0, round & 1))) break;
+          drain(tmem_base, k == it.k0);
+          release_acc(0);
+        }
+        if (ok && (ok = wait_acc(1, tile & 1))) {
+          drain(tmem_base + BN, false);
+          release_acc(1);
         }
         if (!ok) break;
+        // A rolled loop over chunks that always takes the first sums and moves the
+        // others up: unrolled, its addresses alone made the sums spill.
+#pragma unroll 1
+        for (int c = 0; c < kChunks; c += kStep) {
+          finish(c, sum[0], [&](float (&u)[32]) {
 #pragma unroll
-        for (int c = 0; c < kChunks; c += kStep)
-          finish(c, sum[c], [&](float (&u)[32]) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] = sum[c + kStep - 1][j];
+            for (int j = 0; j < 32; ++j) u[j] = sum[kStep - 1][j];
           });
+#pragma unroll
+          for (int i = 0; i + kStep < kChunks; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[i][j] = sum[i + kStep][j];
+        }
       }
     }
   }
@@ -761,6 +802,15 @@ xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaS
   auto kern = gemm_kernel<MODE, T, PAIR, BN>;
   XVEC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)S::kSmemBytes));
+  if (std::is_same<T, float>::value) {
+    // The register split needs the whole block's share at launch, or it would wait.
+    cudaFuncAttributes fa;
+    XVEC_CUDA(cudaFuncGetAttributes(&fa, kern));
+    if (fa.numRegs * S::kThreads < 128 * kFewRegs + (S::kThreads - 128) * kManyRegs) {
+      set_error("adapter: the matrix kernel was built with %d registers", fa.numRegs);
+      return XVEC_GPU_UNSUPPORTED;
+    }
+  }
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.batches * p.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)std::min<int64_t>(items, workers) * (PAIR ? 2 : 1));
@@ -790,11 +840,7 @@ xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaS
 // partial sums' traffic and a second launch.
 template <int MODE, typename T>
 xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
-  constexpr bool F32 = std::is_same<T, float>::value;
-  constexpr double kProducts = F32 ? 6 : 1;
-  // Pair tiles: 256 columns, for float32 128 (its sums also live in registers,
-  // and 256 columns of them spill).
-  constexpr int kPairCols = F32 ? 128 : 256;
+  constexpr double kProducts = std::is_same<T, float>::value ? 6 : 1;
   int device = 0, sms = 0;
   XVEC_CUDA(cudaGetDevice(&device));
   XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
@@ -808,7 +854,7 @@ xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
     double block;  // clocks per depth block
   };
   constexpr int kHalf = MODE == kGated ? 2 : 1;  // accumulator columns per output column
-  const Config configs[] = {{true, 256, kPairCols / kHalf, sms / 2, 2.0 * kPairCols * kProducts},
+  const Config configs[] = {{true, 256, 256 / kHalf, sms / 2, 512.0 * kProducts},
                             {false, 128, 128 / kHalf, sms, 400.0 * kProducts}};
   double best = 0;
   const Config* pick = nullptr;
@@ -833,7 +879,7 @@ xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
     if (xvec_gpu_status st = partial.alloc((size_t)sums * 4, s)) return st;
     p.partial = partial.as<float>();
   }
-  return pick->pair ? launch_shape<MODE, T, true, kPairCols>(c, p, pick->workers, s)
+  return pick->pair ? launch_shape<MODE, T, true, 256>(c, p, pick->workers, s)
                     : launch_shape<MODE, T, false, 128>(c, p, pick->workers, s);
 }
 
