@@ -54,19 +54,33 @@ __device__ __forceinline__ void store_operand(void* dst, int64_t plane, const fl
   }
 }
 
-// src [rows][cols] as an operand: contiguous rows of ld (a multiple of 8)
-// elements, zeros behind the columns.  Bound by memory.
+// A [rows][cols] matrix to become an operand: contiguous rows of ld (a multiple
+// of 8) elements, zeros behind the columns.
+struct Pack {
+  const void* src;
+  void* dst;
+  int64_t lds, rows, ld;
+  int cols, vec;
+};
+struct Packs {
+  Pack p[3];
+  int n = 0;
+};
+// Packs up to three matrices (blockIdx.y) at once.  Bound by memory.
 template <typename T>
-__global__ void __launch_bounds__(256)
-    pack_kernel(const T* src, int64_t lds, int64_t rows, int cols, bool vec, void* dst, int64_t ld) {
-  const int64_t groups = ld / 8, total = groups * rows;
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs packs) {
+  pdl_begin();
+  const Pack& p = packs.p[blockIdx.y];
+  const T* src = static_cast<const T*>(p.src);
+  const int64_t groups = p.ld / 8, total = groups * p.rows;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / groups;
+    // (64-bit divisions would cost more than the copy.)
+    const int64_t r = total >> 32 ? i / groups : (uint32_t)i / (uint32_t)groups;
     const int c = (int)(i - r * groups) * 8;
     float v[8];
-    load8(src + r * lds + c, cols - c, vec, v);
-    store_operand<T>(static_cast<uint16_t*>(dst) + r * ld + c, rows * ld, v);
+    load8(src + r * p.lds + c, p.cols - c, p.vec, v);
+    store_operand<T>(static_cast<uint16_t*>(p.dst) + r * p.ld + c, p.rows * p.ld, v);
   }
 }
 
@@ -79,9 +93,9 @@ unsigned grid_of(int64_t threads) {
 }
 
 // The operand for a [rows][cols] matrix: in place where the copies into shared
-// memory can start on 16 bytes, else packed into `room`.
+// memory can start on 16 bytes, else `room`, for run_packs to fill.
 xvec_gpu_status operand(int storage, const void* p, int64_t rows, int64_t cols, int64_t ld,
-                        Scratch* room, GemmOperand* out, cudaStream_t s) {
+                        Scratch* room, GemmOperand* out, Packs* packs, cudaStream_t s) {
   out->inner = cols, out->outer = rows;
   if (storage != XVEC_STORAGE_FP32 && aligned16(p, ld, 2)) {
     out->p = p, out->ld = ld, out->planes = 1;
@@ -92,20 +106,20 @@ xvec_gpu_status operand(int storage, const void* p, int64_t rows, int64_t cols, 
   out->planes = planes_of(storage);
   if (xvec_gpu_status st = room->alloc((size_t)out->planes * out->plane * 2, s)) return st;
   out->p = room->ptr;
-  const unsigned grid = grid_of(rows * out->ld / 8);
-  const bool vec = aligned16(p, ld, elem_bytes(storage));
-  if (storage == XVEC_STORAGE_FP32)
-    pack_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(p), ld, rows, (int)cols, vec,
-                                            room->ptr, out->ld);
-  else  // either 16-bit type: the bits are copied through float and back, exactly but
-        // for the payload of a NaN
-    storage == XVEC_STORAGE_FP16
-        ? pack_kernel<__half><<<grid, 256, 0, s>>>(static_cast<const __half*>(p), ld, rows,
-                                                   (int)cols, vec, room->ptr, out->ld)
-        : pack_kernel<bf16><<<grid, 256, 0, s>>>(static_cast<const bf16*>(p), ld, rows, (int)cols,
-                                                 vec, room->ptr, out->ld);
-  XVEC_LAUNCHED();
-  XVEC_CUDA(cudaGetLastError());
+  packs->p[packs->n++] = {p, room->ptr, ld, rows, out->ld, (int)cols,
+                          aligned16(p, ld, elem_bytes(storage)) ? 1 : 0};
+  return XVEC_GPU_OK;
+}
+xvec_gpu_status run_packs(int storage, const Packs& packs, cudaStream_t s) {
+  if (packs.n == 0) return XVEC_GPU_OK;
+  int64_t most = 0;
+  for (int i = 0; i < packs.n; ++i) most = std::max(most, packs.p[i].rows * packs.p[i].ld / 8);
+  // 16-bit types: the bits pass through float and back, exactly but for the
+  // payload of a NaN.
+  auto* kern = storage == XVEC_STORAGE_FP32   ? pack_kernel<float>
+               : storage == XVEC_STORAGE_FP16 ? pack_kernel<__half>
+                                              : pack_kernel<bf16>;
+  XVEC_CUDA(launch_pdl(kern, dim3(grid_of(most), packs.n), 256, 0, s, 1, packs));
   return XVEC_GPU_OK;
 }
 
@@ -128,6 +142,7 @@ __global__ void __launch_bounds__(256)
     slope_kernel(const T* dy, int64_t lddy, const T* z, const T* u, int64_t ldz, int64_t n, int m,
                  int act, int vec, int64_t rows_per_chunk, uint16_t* out, int64_t ld,
                  float* partial) {
+  pdl_begin();
   constexpr int kOuts = GATED ? 2 : 1;
   constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -136,34 +151,38 @@ __global__ void __launch_bounds__(256)
   const int64_t r1 = min(n, r0 + rows_per_chunk);
   float sum[kOuts][8] = {};
   if (c < m) {
-    for (int64_t r = r0 + ty; r < r1; r += 8) {
-      float d[kOuts][8];
-      load8(dy + r * lddy + c, m - c, vec & 1, d[0]);
-      if constexpr (GATED) {
-        float g[8], v[8];
-        load8(z + r * ldz + c, m - c, vec & 2, g);
-        load8(u + r * ldz + c, m - c, vec & 4, v);
+    // Two rows at a time: their loads are all requested before the first is used.
+    for (int64_t r = r0 + ty; r < r1; r += 16) {
+      float d[2][kOuts][8], z8[2][8], u8[2][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float slope;
-          d[1][j] = d[0][j] * activate_slope<T>(act, g[j], &slope);
-          d[0][j] = d[0][j] * v[j] * slope;
-        }
-      } else if (act != XVEC_ACT_NONE) {
-        float v[8];
-        load8(z + r * ldz + c, m - c, vec & 2, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float slope;
-          activate_slope<T>(act, v[j], &slope);
-          d[0][j] *= slope;
-        }
+      for (int i = 0; i < 2; ++i) {
+        const int64_t q = r + 8 * i < r1 ? r + 8 * i : r;
+        load8(dy + q * lddy + c, m - c, vec & 1, d[i][0]);
+        if (GATED || act != XVEC_ACT_NONE) load8(z + q * ldz + c, m - c, vec & 2, z8[i]);
+        if (GATED) load8(u + q * ldz + c, m - c, vec & 4, u8[i]);
       }
 #pragma unroll
-      for (int o = 0; o < kOuts; ++o) {
-        if (out) store_operand<T>(out + (o * kPlanes * n + r) * ld + c, n * ld, d[o]);
+      for (int i = 0; i < 2; ++i) {
+        if (r + 8 * i >= r1) break;
+        if (GATED || act != XVEC_ACT_NONE) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[o][j] += d[o][j];
+          for (int j = 0; j < 8; ++j) {
+            float slope;
+            const float a = activate_slope<T>(act, z8[i][j], &slope);
+            if constexpr (GATED) {
+              d[i][1][j] = d[i][0][j] * a;
+              d[i][0][j] *= u8[i][j];
+            }
+            d[i][0][j] *= slope;
+          }
+        }
+#pragma unroll
+        for (int o = 0; o < kOuts; ++o) {
+          if (out)
+            store_operand<T>(out + (o * kPlanes * n + r + 8 * i) * ld + c, n * ld, d[i][o]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[o][j] += d[i][o][j];
+        }
       }
     }
   }
@@ -184,11 +203,13 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// out[c] = the sum over the chunks in a fixed order: 8 interleaved runs, then
+// out[c] = the sum over the chunks in a fixed order: 32 interleaved runs, then
 // those.
+constexpr int kSumThreads = 1024;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kSumThreads)
     column_sum_kernel(const float* partial, int chunks, int m, T* out0, T* out1) {
+  pdl_begin();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
   T* out = blockIdx.y ? out1 : out0;
@@ -196,12 +217,12 @@ __global__ void __launch_bounds__(256)
   const float* p = partial + (int64_t)blockIdx.y * chunks * m + c;
   float s = 0.f;
   if (c < m)
-    for (int i = ty; i < chunks; i += 8) s += p[(int64_t)i * m];
-  __shared__ float part[8][33];
+    for (int i = ty; i < chunks; i += 32) s += p[(int64_t)i * m];
+  __shared__ float part[32][33];
   part[ty][tx] = s;
   __syncthreads();
   if (ty == 0 && c < m) {
-    for (int i = 1; i < 8; ++i) s += part[i][tx];
+    for (int i = 1; i < 32; ++i) s += part[i][tx];
     out[c] = from_f<T>(s);
   }
 }
@@ -220,10 +241,10 @@ template <typename T>
 xvec_gpu_status slopes_t(const Slopes& a, cudaStream_t s) {
   const int cols = (a.m + 255) / 256;
   const bool sums = a.db[0] || a.db[1];
-  // About eight blocks per SM, of at least 32 rows.
+  // About four blocks per SM, of at least 16 rows.
   const int64_t chunks =
-      std::max<int64_t>(1, std::min<int64_t>((a.n + 31) / 32, std::max(1, 148 * 8 / cols)));
-  const int64_t per = ((a.n + chunks - 1) / chunks + 7) / 8 * 8;
+      std::max<int64_t>(1, std::min<int64_t>((a.n + 15) / 16, std::max(1, 148 * 4 / cols)));
+  const int64_t per = ((a.n + chunks - 1) / chunks + 15) / 16 * 16;
   const int used = (int)((a.n + per - 1) / per);
   Scratch partial;
   if (sums)
@@ -232,18 +253,13 @@ xvec_gpu_status slopes_t(const Slopes& a, cudaStream_t s) {
                   (aligned16(a.z, a.ldz, sizeof(T)) ? 2 : 0) |
                   (aligned16(a.u, a.ldz, sizeof(T)) ? 4 : 0);
   auto* kern = a.u ? slope_kernel<T, true> : slope_kernel<T, false>;
-  kern<<<dim3(cols, used), 256, 0, s>>>(static_cast<const T*>(a.dy), a.lddy,
-                                        static_cast<const T*>(a.z), static_cast<const T*>(a.u),
-                                        a.ldz, a.n, a.m, a.act, vec, per,
-                                        static_cast<uint16_t*>(a.out), a.ld, partial.as<float>());
-  XVEC_LAUNCHED();
-  XVEC_CUDA(cudaGetLastError());
-  if (sums) {
-    column_sum_kernel<T><<<dim3((a.m + 31) / 32, 2), 256, 0, s>>>(
-        partial.as<float>(), used, a.m, static_cast<T*>(a.db[0]), static_cast<T*>(a.db[1]));
-    XVEC_LAUNCHED();
-    XVEC_CUDA(cudaGetLastError());
-  }
+  XVEC_CUDA(launch_pdl(kern, dim3(cols, used), 256, 0, s, 1, static_cast<const T*>(a.dy), a.lddy,
+                       static_cast<const T*>(a.z), static_cast<const T*>(a.u), a.ldz, a.n, a.m,
+                       a.act, vec, per, static_cast<uint16_t*>(a.out), a.ld, partial.as<float>()));
+  if (sums)
+    XVEC_CUDA(launch_pdl(column_sum_kernel<T>, dim3((a.m + 31) / 32, 2), kSumThreads, 0, s, 1,
+                         partial.as<float>(), used, a.m, static_cast<T*>(a.db[0]),
+                         static_cast<T*>(a.db[1])));
   return XVEC_GPU_OK;
 }
 
@@ -434,8 +450,11 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   g.mode = kLinear;
   g.depth = a.in_dim;
   Scratch room[2];
-  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, s)) ||
-      (st = operand(a.storage, a.weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0], s)))
+  Packs packs;
+  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, &packs, s)) ||
+      (st = operand(a.storage, a.weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0], &packs,
+                    s)) ||
+      (st = run_packs(a.storage, packs, s)))
     return st;
   GemmParams& p = g.p;
   p.rows = a.n, p.cols = a.out_dim, p.segs = p.batches = 1;
@@ -489,9 +508,13 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   g.mode = kGated;
   g.depth = a.in_dim;
   Scratch room[3];
-  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, s)) ||
-      (st = operand(a.storage, a.gate_weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0], s)) ||
-      (st = operand(a.storage, a.up_weight, a.out_dim, a.in_dim, a.ldw, &room[2], &g.b[1], s)))
+  Packs packs;
+  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, &packs, s)) ||
+      (st = operand(a.storage, a.gate_weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0],
+                    &packs, s)) ||
+      (st = operand(a.storage, a.up_weight, a.out_dim, a.in_dim, a.ldw, &room[2], &g.b[1], &packs,
+                    s)) ||
+      (st = run_packs(a.storage, packs, s)))
     return st;
   GemmParams& p = g.p;
   p.rows = a.n, p.cols = a.out_dim, p.segs = p.batches = 1;
@@ -562,15 +585,22 @@ xvec_gpu_status run_backward(const Backward& b) {
     a.db[0] = b.db[0], a.db[1] = b.db[1];
     if ((st = slopes(b.storage, a, s))) return st;
   }
+  Scratch room[3];
+  GemmOperand w[2], x;
+  Packs packs;
+  if (b.dx)
+    for (int i = 0; i < b.parts; ++i)
+      if ((st = operand(b.storage, b.w[i], b.out_dim, b.in_dim, b.ldw, &room[i], &w[i], &packs, s)))
+        return st;
+  if (b.dw[0] || b.dw[1])
+    if ((st = operand(b.storage, b.x, b.n, b.in_dim, b.ldx, &room[2], &x, &packs, s))) return st;
+  if ((st = run_packs(b.storage, packs, s))) return st;
   if (b.dx) {
     GemmCall g;
     g.mode = kDx;
     g.depth = b.out_dim;
     g.a = grad;
-    Scratch room[2];
-    for (int i = 0; i < b.parts; ++i)
-      if ((st = operand(b.storage, b.w[i], b.out_dim, b.in_dim, b.ldw, &room[i], &g.b[i], s)))
-        return st;
+    for (int i = 0; i < b.parts; ++i) g.b[i] = w[i];
     g.p.rows = b.n, g.p.cols = b.in_dim, g.p.segs = b.parts, g.p.batches = 1;
     g.p.out[0] = b.dx, g.p.ldo = b.lddx;
     g.p.vec = aligned16(b.dx, b.lddx, size);
@@ -582,8 +612,7 @@ xvec_gpu_status run_backward(const Backward& b) {
     g.mode = kDw;
     g.depth = b.n;
     g.a = grad;
-    Scratch room;
-    if ((st = operand(b.storage, b.x, b.n, b.in_dim, b.ldx, &room, &g.b[0], s))) return st;
+    g.b[0] = x;
     g.p.rows = b.out_dim, g.p.cols = b.in_dim, g.p.segs = 1;
     g.p.vec = 1;
     // Only the second weight's gradient: start at its matrix.

@@ -46,6 +46,7 @@ template <typename T, bool GATED, int ROWS, int COLS>
 __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_constant__ FewRows p,
                                                                bool x_vec, bool w_vec) {
   constexpr int W = GATED ? 2 : 1;
+  pdl_begin();
   const int lane = threadIdx.x & 31;
   const int c0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * COLS;
   if (c0 >= p.out_dim) return;
@@ -96,11 +97,10 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_cons
 template <typename T, bool GATED, int ROWS, int COLS>
 xvec_gpu_status launch(const FewRows& f, cudaStream_t s) {
   constexpr int kPer = kWarps * COLS;
-  few_rows_kernel<T, GATED, ROWS, COLS><<<(f.out_dim + kPer - 1) / kPer, kWarps * 32, 0, s>>>(
-      f, aligned16(f.x, f.ldx, sizeof(T)),
-      aligned16(f.w[0], f.ldw, sizeof(T)) && aligned16(f.w[1], f.ldw, sizeof(T)));
-  XVEC_LAUNCHED();
-  XVEC_CUDA(cudaGetLastError());
+  XVEC_CUDA(launch_pdl(few_rows_kernel<T, GATED, ROWS, COLS>, dim3((f.out_dim + kPer - 1) / kPer),
+                       kWarps * 32, 0, s, 1, f, aligned16(f.x, f.ldx, sizeof(T)),
+                       aligned16(f.w[0], f.ldw, sizeof(T)) &&
+                           aligned16(f.w[1], f.ldw, sizeof(T))));
   return XVEC_GPU_OK;
 }
 

@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
     }
     tmem_fence_before();
   }
+  pdl_begin();
   __syncthreads();
   if constexpr (PAIR) cluster_sync_all();
   tmem_fence_after();
@@ -718,6 +719,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
 // Adds the splits' partial sums in their order and finishes as the kernel would.
 template <int MODE, typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ GemmParams p) {
+  pdl_begin();
   const int64_t groups = (p.cols + 3) / 4;
   const int64_t total = groups * p.rows;
   const int batch = blockIdx.y;
@@ -812,25 +814,14 @@ xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaS
     }
   }
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.batches * p.splits;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>(items, workers) * (PAIR ? 2 : 1));
-  cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = S::kSmemBytes;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  XVEC_CUDA(cudaLaunchKernelEx(&cfg, kern, a, b0, b1, p));
-  XVEC_LAUNCHED();
+  XVEC_CUDA(launch_pdl(kern, dim3((unsigned)std::min<int64_t>(items, workers) * (PAIR ? 2 : 1)),
+                       S::kThreads, S::kSmemBytes, s, PAIR ? 2 : 1, a, b0, b1, p));
   if (p.splits > 1) {
     const int64_t groups = (p.cols + 3) / 4 * p.rows;
-    finish_kernel<MODE, T><<<dim3((unsigned)std::min<int64_t>((groups + 255) / 256, 1184),
-                                  (unsigned)p.batches), 256, 0, s>>>(p);
-    XVEC_LAUNCHED();
-    XVEC_CUDA(cudaGetLastError());
+    XVEC_CUDA(launch_pdl(finish_kernel<MODE, T>,
+                         dim3((unsigned)std::min<int64_t>((groups + 255) / 256, 1184),
+                              (unsigned)p.batches),
+                         256, 0, s, 1, p));
   }
   return XVEC_GPU_OK;
 }

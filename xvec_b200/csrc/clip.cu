@@ -169,6 +169,7 @@ __device__ __forceinline__ void scale_range(const T* in, T* out, int64_t i0, int
 template <int N>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     square_sum_kernel(const __grid_constant__ Table<N> t, double* sums) {
+  pdl_begin();
   double s = 0;
   for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const Entry& e = t.e[entry_of(t, c)];
@@ -189,6 +190,7 @@ template <int N>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     scale_kernel(const __grid_constant__ Table<N> t, const double* sums, int num_sums,
                  double max_norm, float* norm) {
+  pdl_begin();
   double s = 0;
   for (int i = threadIdx.x; i < num_sums; i += kThreads) s += sums[i];
   const double n = sqrt(block_sum(s));
@@ -239,18 +241,15 @@ xvec_gpu_status clip(const xvec_gpu_tensor* tensors, int num, double max_norm, f
   int done = 0;
   for (int i = 0; fill(&i);) {
     const int b = (int)std::min<uint32_t>(t.chunks, max_blocks);
-    square_sum_kernel<N><<<b, kThreads, 0, s>>>(t, sums.as<double>() + done);
-    XVEC_LAUNCHED();
-    XVEC_CUDA(cudaGetLastError());
+    XVEC_CUDA(launch_pdl(square_sum_kernel<N>, dim3(b), kThreads, 0, s, 1, t,
+                         sums.as<double>() + done));
     done += b;
   }
   int i = 0;
   for (int pass = 0; fill(&i) || pass == 0; ++pass) {
     const int b = std::max(1, (int)std::min<uint32_t>(t.chunks, max_blocks));
-    scale_kernel<N><<<b, kThreads, 0, s>>>(t, sums.as<double>(), blocks, max_norm,
-                                           pass == 0 ? d_norm : nullptr);
-    XVEC_LAUNCHED();
-    XVEC_CUDA(cudaGetLastError());
+    XVEC_CUDA(launch_pdl(scale_kernel<N>, dim3(b), kThreads, 0, s, 1, t, sums.as<double>(), blocks,
+                         max_norm, pass == 0 ? d_norm : nullptr));
     if (t.entries == 0) break;
   }
   return XVEC_GPU_OK;
