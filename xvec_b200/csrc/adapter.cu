@@ -30,10 +30,8 @@ constexpr int kMaxDevices = 64;
 template <typename T>
 __device__ __forceinline__ void store_operand(void* dst, int64_t plane, const float (&v)[8]) {
   if constexpr (sizeof(T) == 2) {
-    __align__(16) T t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = from_f<T>(v[j]);
-    *static_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(t);
+    *static_cast<uint4*>(dst) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                           pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
   } else {
     __align__(16) bf16 t[3][8];
 #pragma unroll
@@ -137,51 +135,75 @@ xvec_gpu_status gemm(int storage, GemmCall& c, cudaStream_t s) {
 // [2][chunks][m]: the column sums of each row chunk in float32, before any
 // rounding.  A block owns 256 columns of a row chunk: 32 threads of 8 columns,
 // 8 rows at a time.  Bound by memory.
+template <typename T>
+struct Eight {
+  static constexpr int N = sizeof(T) / 2;  // 16-byte parts
+  uint4 v[N];
+  __device__ __forceinline__ void load(const T* p, int count, bool vec) {
+    if (vec && count >= 8) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+      T* t = reinterpret_cast<T*>(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = j < count ? p[j] : from_f<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    return to_f(reinterpret_cast<const T*>(v)[j]);
+  }
+};
+
+// kRows rows of a thread are requested before the first is used and held as
+// they came.  (Held as floats they took 122 registers, a quarter of the warps.)
 template <typename T, bool GATED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
     slope_kernel(const T* dy, int64_t lddy, const T* z, const T* u, int64_t ldz, int64_t n, int m,
                  int act, int vec, int64_t rows_per_chunk, uint16_t* out, int64_t ld,
                  float* partial) {
   pdl_begin();
   constexpr int kOuts = GATED ? 2 : 1;
   constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+  constexpr int kRows = 2;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 256 + tx * 8;
   const int64_t r0 = blockIdx.y * rows_per_chunk;
   const int64_t r1 = min(n, r0 + rows_per_chunk);
+  const bool act_needed = GATED || act != XVEC_ACT_NONE;
   float sum[kOuts][8] = {};
   if (c < m) {
-    // Two rows at a time: their loads are all requested before the first is used.
-    for (int64_t r = r0 + ty; r < r1; r += 16) {
-      float d[2][kOuts][8], z8[2][8], u8[2][8];
+    for (int64_t r = r0 + ty; r < r1; r += 8 * kRows) {
+      Eight<T> dr[kRows], zr[kRows], ur[kRows];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < kRows; ++i) {
         const int64_t q = r + 8 * i < r1 ? r + 8 * i : r;
-        load8(dy + q * lddy + c, m - c, vec & 1, d[i][0]);
-        if (GATED || act != XVEC_ACT_NONE) load8(z + q * ldz + c, m - c, vec & 2, z8[i]);
-        if (GATED) load8(u + q * ldz + c, m - c, vec & 4, u8[i]);
+        dr[i].load(dy + q * lddy + c, m - c, vec & 1);
+        if (act_needed) zr[i].load(z + q * ldz + c, m - c, vec & 2);
+        if (GATED) ur[i].load(u + q * ldz + c, m - c, vec & 4);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < kRows; ++i) {
         if (r + 8 * i >= r1) break;
-        if (GATED || act != XVEC_ACT_NONE) {
+        float d[kOuts][8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 8; ++j) {
+          d[0][j] = dr[i][j];
+          if (act_needed) {
             float slope;
-            const float a = activate_slope<T>(act, z8[i][j], &slope);
+            const float a = activate_slope<T>(act, zr[i][j], &slope);
             if constexpr (GATED) {
-              d[i][1][j] = d[i][0][j] * a;
-              d[i][0][j] *= u8[i][j];
+              d[1][j] = d[0][j] * a;
+              d[0][j] *= ur[i][j];
             }
-            d[i][0][j] *= slope;
+            d[0][j] *= slope;
           }
         }
 #pragma unroll
         for (int o = 0; o < kOuts; ++o) {
           if (out)
-            store_operand<T>(out + (o * kPlanes * n + r + 8 * i) * ld + c, n * ld, d[i][o]);
+            store_operand<T>(out + (o * kPlanes * n + r + 8 * i) * ld + c, n * ld, d[o]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum[o][j] += d[i][o][j];
+          for (int j = 0; j < 8; ++j) sum[o][j] += d[o][j];
         }
       }
     }
@@ -241,9 +263,9 @@ template <typename T>
 xvec_gpu_status slopes_t(const Slopes& a, cudaStream_t s) {
   const int cols = (a.m + 255) / 256;
   const bool sums = a.db[0] || a.db[1];
-  // About four blocks per SM, of at least 16 rows.
+  // About eight blocks per SM, of at least 16 rows.
   const int64_t chunks =
-      std::max<int64_t>(1, std::min<int64_t>((a.n + 15) / 16, std::max(1, 148 * 4 / cols)));
+      std::max<int64_t>(1, std::min<int64_t>((a.n + 15) / 16, std::max(1, 148 * 8 / cols)));
   const int64_t per = ((a.n + chunks - 1) / chunks + 15) / 16 * 16;
   const int used = (int)((a.n + per - 1) / per);
   Scratch partial;

@@ -68,7 +68,7 @@ struct GemmShape {
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + 512;
-  static constexpr int kTmemCols = 2 * BN;  // two accumulators
+  static constexpr int kTmemCols = BN == 192 ? 512 : 2 * BN;  // two accumulators, a power of two
   static_assert(kStages >= 4, "shared memory too small for the stage ring");
 };
 
@@ -601,6 +601,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
             emit(buf, static_cast<T*>(p.save[which]) + row0 * p.lds + col, p.lds, rows, n, vec, x,
                  lane);
         };
+        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, vec && n == 32, lane);
         if constexpr (MODE == kLinear || MODE == kGated) {
           affine(0, v);
           activate_all<T>(p.act, v);
@@ -613,7 +614,6 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
           for (int j = 0; j < 32; ++j) v[j] *= u[j];
         }
         if (MODE == kLinear && res && n > 0) {
-          if (P == 3) in.start(res + at, p.ldr, rows, vec && n == 32, lane);
           in.add(buf, res + at, p.ldr, rows, n, vec && n == 32, v, lane);
           if (P == 1 && c + 1 < kChunks) in.start(res + at + 32, p.ldr, rows, vec && cols >= at + 64, lane);
         }
@@ -826,9 +826,16 @@ xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaS
   return XVEC_GPU_OK;
 }
 
-// Tile shape and depth splits by a cost estimate in SM clocks: a tile's blocks
-// and its start and epilogue, in waves over the SMs; splits pay for their
-// partial sums' traffic and a second launch.
+// Tile shape and depth splits by a cost estimate in SM clocks.  A tile's blocks
+// overlap the epilogue of the tile before, so a wave takes the longer of the two,
+// and the last epilogue comes on top; splits pay for their partial sums' traffic
+// and a second launch.  Measured: 512 clocks a block for a pair's 256 columns
+// (the matrix rate), 400 for 192, 620 for a single CTA's 128 x 128 (twice the
+// bytes per product); about 20 clocks an epilogue column for each matrix that it
+// reads or writes and for an activation, 45 where rows do not allow 16-byte
+// accesses.  192 columns exist for one product along depth (kLinear), where they
+// can fill the last wave better: 10000 x 960 -> 960 fp32 is 200 tiles of three
+// waves instead of 160 larger ones of three.
 template <int MODE, typename T>
 xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
   constexpr double kProducts = std::is_same<T, float>::value ? 6 : 1;
@@ -840,22 +847,28 @@ xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
   const int all = p.blocks * p.segs;
   p.ldp = (p.cols + 31) / 32 * 32;
   struct Config {
-    bool pair;
     int rows, cols, workers;
     double block;  // clocks per depth block
+    bool use;
   };
   constexpr int kHalf = MODE == kGated ? 2 : 1;  // accumulator columns per output column
-  const Config configs[] = {{true, 256, 256 / kHalf, sms / 2, 512.0 * kProducts},
-                            {false, 128, 128 / kHalf, sms, 400.0 * kProducts}};
+  const Config configs[] = {{256, 256 / kHalf, sms / 2, 512.0 * kProducts, true},
+                            {256, 192, sms / 2, 400.0 * kProducts, MODE == kLinear},
+                            {128, 128 / kHalf, sms, 620.0 * kProducts, true}};
+  const int matrices = 1 + (p.save[0] != nullptr) + (p.save[1] != nullptr) +
+                       (p.residual != nullptr) + (p.act != XVEC_ACT_NONE);
   double best = 0;
   const Config* pick = nullptr;
   for (const Config& k : configs) {
+    if (!k.use) continue;
     const int64_t tm = (p.rows + k.rows - 1) / k.rows, tn = (p.cols + k.cols - 1) / k.cols;
     for (int splits = 1; splits <= 32; ++splits) {
       const int per = (all + splits - 1) / splits;
       if (splits > 1 && (per < 4 || (int64_t)per * (splits - 1) >= all)) continue;
       const double waves = (double)((tm * tn * p.batches * splits + k.workers - 1) / k.workers);
-      double cost = waves * (per * k.block + 2500);
+      const double epilogue = k.cols * (splits > 1 ? 50.0 * kHalf : matrices * (p.vec ? 20.0 : 45.0));
+      double cost = waves * std::max(per * k.block, epilogue) +
+                    std::min(per * k.block, epilogue) + 2500;
       if (splits > 1)
         cost += 6000 + (double)splits * p.rows * p.ldp * p.batches * kHalf * 8 / 2000;
       if (!pick || cost < best) {
@@ -870,8 +883,10 @@ xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
     if (xvec_gpu_status st = partial.alloc((size_t)sums * 4, s)) return st;
     p.partial = partial.as<float>();
   }
-  return pick->pair ? launch_shape<MODE, T, true, 256>(c, p, pick->workers, s)
-                    : launch_shape<MODE, T, false, 128>(c, p, pick->workers, s);
+  if (pick->rows == 128) return launch_shape<MODE, T, false, 128>(c, p, pick->workers, s);
+  if constexpr (MODE == kLinear)
+    if (pick->cols == 192) return launch_shape<MODE, T, true, 192>(c, p, pick->workers, s);
+  return launch_shape<MODE, T, true, 256>(c, p, pick->workers, s);
 }
 
 template <typename T>
