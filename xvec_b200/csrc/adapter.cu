@@ -12,7 +12,6 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cmath>
 
 #include "adapter.cuh"
 
@@ -64,15 +63,11 @@ struct Packs {
   Pack p[3];
   int n = 0;
 };
-// Packs up to three matrices (blockIdx.y) at once.  Bound by memory.
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs packs) {
-  pdl_begin();
-  const Pack& p = packs.p[blockIdx.y];
+__device__ __forceinline__ void pack(const Pack& p, int64_t thread, int64_t threads) {
   const T* src = static_cast<const T*>(p.src);
   const int64_t groups = p.ld / 8, total = groups * p.rows;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * 256) {
+  for (int64_t i = thread; i < total; i += threads) {
     // (64-bit divisions would cost more than the copy.)
     const int64_t r = total >> 32 ? i / groups : (uint32_t)i / (uint32_t)groups;
     const int c = (int)(i - r * groups) * 8;
@@ -80,6 +75,12 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs
     load8(src + r * p.lds + c, p.cols - c, p.vec, v);
     store_operand<T>(static_cast<uint16_t*>(p.dst) + r * p.ld + c, p.rows * p.ld, v);
   }
+}
+// Packs up to three matrices (blockIdx.y) at once.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs packs) {
+  pdl_begin();
+  pack<T>(packs.p[blockIdx.y], (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
 size_t elem_bytes(int storage) { return storage == XVEC_STORAGE_FP32 ? 4 : 2; }
@@ -90,30 +91,52 @@ unsigned grid_of(int64_t threads) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 148 * 16));
 }
 
-// The operand for a [rows][cols] matrix: in place where the copies into shared
-// memory can start on 16 bytes, else `room`, for run_packs to fill.
-xvec_gpu_status operand(int storage, const void* p, int64_t rows, int64_t cols, int64_t ld,
-                        Scratch* room, GemmOperand* out, Packs* packs, cudaStream_t s) {
-  out->inner = cols, out->outer = rows;
-  if (storage != XVEC_STORAGE_FP32 && aligned16(p, ld, 2)) {
-    out->p = p, out->ld = ld, out->planes = 1;
-    return XVEC_GPU_OK;
+// One call's scratch: a single stream-ordered allocation, handed out in parts.
+struct Arena {
+  Scratch room;
+  size_t used = 0;
+  size_t add(size_t bytes) {
+    const size_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    return at;
   }
-  out->ld = round8(cols);
-  out->plane = rows * out->ld;
-  out->planes = planes_of(storage);
-  if (xvec_gpu_status st = room->alloc((size_t)out->planes * out->plane * 2, s)) return st;
-  out->p = room->ptr;
-  packs->p[packs->n++] = {p, room->ptr, ld, rows, out->ld, (int)cols,
-                          aligned16(p, ld, elem_bytes(storage)) ? 1 : 0};
-  return XVEC_GPU_OK;
+  xvec_gpu_status alloc(cudaStream_t s) { return used ? room.alloc(used, s) : XVEC_GPU_OK; }
+  void* at(size_t offset) const { return room.as<char>() + offset; }
+};
+
+// The operand for a [rows][cols] matrix: in place where the copies into shared
+// memory can start on 16 bytes, else a place in the arena for the packing.
+// (16-bit types: packed bits pass through float and back, exactly but for the
+// payload of a NaN.)
+struct Operand {
+  GemmOperand g;
+  bool packed = false;
+  size_t at = 0;
+  Pack pack{};
+};
+Operand plan_operand(int storage, const void* p, int64_t rows, int64_t cols, int64_t ld,
+                     Arena* arena) {
+  Operand o;
+  o.g.p = p, o.g.inner = cols, o.g.outer = rows, o.g.ld = ld;
+  if (storage != XVEC_STORAGE_FP32 && aligned16(p, ld, 2)) return o;
+  o.packed = true;
+  o.g.ld = round8(cols);
+  o.g.plane = rows * o.g.ld;
+  o.g.planes = planes_of(storage);
+  o.at = arena->add((size_t)o.g.planes * o.g.plane * 2);
+  o.pack = {p, nullptr, ld, rows, o.g.ld, (int)cols, aligned16(p, ld, elem_bytes(storage)) ? 1 : 0};
+  return o;
+}
+// Once the arena is there.
+void place(Operand* o, const Arena& arena, Packs* packs) {
+  if (!o->packed) return;
+  o->g.p = o->pack.dst = arena.at(o->at);
+  packs->p[packs->n++] = o->pack;
 }
 xvec_gpu_status run_packs(int storage, const Packs& packs, cudaStream_t s) {
   if (packs.n == 0) return XVEC_GPU_OK;
   int64_t most = 0;
   for (int i = 0; i < packs.n; ++i) most = std::max(most, packs.p[i].rows * packs.p[i].ld / 8);
-  // 16-bit types: the bits pass through float and back, exactly but for the
-  // payload of a NaN.
   auto* kern = storage == XVEC_STORAGE_FP32   ? pack_kernel<float>
                : storage == XVEC_STORAGE_FP16 ? pack_kernel<__half>
                                               : pack_kernel<bf16>;
@@ -127,6 +150,24 @@ xvec_gpu_status gemm(int storage, GemmCall& c, cudaStream_t s) {
   return storage == XVEC_STORAGE_FP32   ? gemm_fp32(c, s)
          : storage == XVEC_STORAGE_FP16 ? gemm_fp16(c, s)
                                         : gemm_bf16(c, s);
+}
+
+// A forward product: plan, scratch, packing, launch.
+xvec_gpu_status forward(int storage, GemmCall& g, Operand* a, Operand* b0, Operand* b1, Arena& arena,
+                        cudaStream_t s) {
+  xvec_gpu_status st = plan_gemm(storage, &g);
+  if (st) return st;
+  const size_t partial = arena.add(g.partial_bytes);
+  if ((st = arena.alloc(s))) return st;
+  Packs packs;
+  place(a, arena, &packs);
+  place(b0, arena, &packs);
+  if (b1) place(b1, arena, &packs);
+  if ((st = run_packs(storage, packs, s))) return st;
+  g.a = a->g, g.b[0] = b0->g;
+  if (b1) g.b[1] = b1->g;
+  if (g.partial_bytes) g.p.partial = static_cast<float*>(arena.at(partial));
+  return gemm(storage, g, s);
 }
 
 // --- pre-activation gradients and their column sums -----------------------
@@ -154,21 +195,48 @@ struct Eight {
   }
 };
 
+// The pre-activation gradients of one backward call and its packings.
+struct Slopes {
+  const void *dy, *z, *u;  // u: gated only
+  int64_t lddy, ldz, n;
+  int m, act, vec;  // vec: 1, 2, 4 = dy, z, u allow 16-byte accesses
+  int cols, chunks;  // blocks: of 256 columns, of rows_per_chunk rows
+  int64_t rows_per_chunk;
+  uint16_t* out;
+  int64_t ld;
+  float* partial;
+  Packs packs;
+  unsigned pack_blocks;  // for each packing
+};
+
+// Blocks [0, cols chunks) are the gradients', the others the packings'.
 // kRows rows of a thread are requested before the first is used and held as
 // they came.  (Held as floats they took 122 registers, a quarter of the warps.)
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
-    slope_kernel(const T* dy, int64_t lddy, const T* z, const T* u, int64_t ldz, int64_t n, int m,
-                 int act, int vec, int64_t rows_per_chunk, uint16_t* out, int64_t ld,
-                 float* partial) {
+    slope_kernel(const __grid_constant__ Slopes p) {
   pdl_begin();
+  const unsigned slope_blocks = (unsigned)p.cols * p.chunks;
+  if (blockIdx.x >= slope_blocks) {
+    const unsigned b = blockIdx.x - slope_blocks, which = b / p.pack_blocks;
+    pack<T>(p.packs.p[which], (int64_t)(b - which * p.pack_blocks) * 256 + threadIdx.x,
+            (int64_t)p.pack_blocks * 256);
+    return;
+  }
+  const unsigned chunk = blockIdx.x / p.cols, col_block = blockIdx.x - chunk * p.cols;
+  const T* dy = static_cast<const T*>(p.dy);
+  const T* z = static_cast<const T*>(p.z);
+  const T* u = static_cast<const T*>(p.u);
+  const int64_t lddy = p.lddy, ldz = p.ldz, n = p.n, ld = p.ld;
+  const int m = p.m, act = p.act, vec = p.vec;
+  uint16_t* out = p.out;
   constexpr int kOuts = GATED ? 2 : 1;
   constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
   constexpr int kRows = 2;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c = blockIdx.x * 256 + tx * 8;
-  const int64_t r0 = blockIdx.y * rows_per_chunk;
-  const int64_t r1 = min(n, r0 + rows_per_chunk);
+  const int c = col_block * 256 + tx * 8;
+  const int64_t r0 = chunk * p.rows_per_chunk;
+  const int64_t r1 = min(n, r0 + p.rows_per_chunk);
   const bool act_needed = GATED || act != XVEC_ACT_NONE;
   float sum[kOuts][8] = {};
   if (c < m) {
@@ -208,7 +276,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
       }
     }
   }
-  if (partial) {
+  if (p.partial) {
     __shared__ float part[8][256];
 #pragma unroll
     for (int o = 0; o < kOuts; ++o) {
@@ -219,76 +287,57 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
-      const int col = blockIdx.x * 256 + threadIdx.x;
-      if (col < m) partial[((int64_t)o * gridDim.y + blockIdx.y) * m + col] = s;
+      const int col = col_block * 256 + threadIdx.x;
+      if (col < m) p.partial[((int64_t)o * p.chunks + chunk) * m + col] = s;
     }
   }
 }
 
-// out[c] = the sum over the chunks in a fixed order: 32 interleaved runs, then
-// those.
-constexpr int kSumThreads = 1024;
+// The column sums alone, where no product follows that could take them along.
 template <typename T>
-__global__ void __launch_bounds__(kSumThreads)
-    column_sum_kernel(const float* partial, int chunks, int m, T* out0, T* out1) {
+__global__ void __launch_bounds__(128)
+    column_sum_kernel(const float* sums, int chunks, int m, void* out0, void* out1) {
   pdl_begin();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + tx;
-  T* out = blockIdx.y ? out1 : out0;
-  if (!out) return;
-  const float* p = partial + (int64_t)blockIdx.y * chunks * m + c;
-  float s = 0.f;
-  if (c < m)
-    for (int i = ty; i < chunks; i += 32) s += p[(int64_t)i * m];
-  __shared__ float part[32][33];
-  part[ty][tx] = s;
-  __syncthreads();
-  if (ty == 0 && c < m) {
-    for (int i = 1; i < 32; ++i) s += part[i][tx];
-    out[c] = from_f<T>(s);
-  }
+  column_sums<T>(sums, chunks, m, out0, out1, blockIdx.x * 4 + (threadIdx.x >> 5), gridDim.x * 4,
+                 threadIdx.x & 31);
 }
 
-// The pre-activation gradients of one backward call.
-struct Slopes {
-  const void *dy, *z, *u;  // u: gated only
-  int64_t lddy, ldz, n;
-  int m, act;
-  void* out;  // NULL: not wanted
-  int64_t ld;
-  void* db[2];
-};
+// Row chunks of the gradient pass: about eight blocks per SM, of at least 16 rows.
+void plan_slopes(Slopes* a) {
+  a->cols = (a->m + 255) / 256;
+  const int64_t most =
+      std::max<int64_t>(1, std::min<int64_t>((a->n + 15) / 16, std::max(1, 148 * 8 / a->cols)));
+  a->rows_per_chunk = ((a->n + most - 1) / most + 15) / 16 * 16;
+  a->chunks = (int)((a->n + a->rows_per_chunk - 1) / a->rows_per_chunk);
+}
 
 template <typename T>
-xvec_gpu_status slopes_t(const Slopes& a, cudaStream_t s) {
-  const int cols = (a.m + 255) / 256;
-  const bool sums = a.db[0] || a.db[1];
-  // About eight blocks per SM, of at least 16 rows.
-  const int64_t chunks =
-      std::max<int64_t>(1, std::min<int64_t>((a.n + 15) / 16, std::max(1, 148 * 8 / cols)));
-  const int64_t per = ((a.n + chunks - 1) / chunks + 15) / 16 * 16;
-  const int used = (int)((a.n + per - 1) / per);
-  Scratch partial;
-  if (sums)
-    if (xvec_gpu_status st = partial.alloc((size_t)2 * used * a.m * 4, s)) return st;
-  const int vec = (aligned16(a.dy, a.lddy, sizeof(T)) ? 1 : 0) |
-                  (aligned16(a.z, a.ldz, sizeof(T)) ? 2 : 0) |
-                  (aligned16(a.u, a.ldz, sizeof(T)) ? 4 : 0);
+xvec_gpu_status slopes_t(Slopes& a, cudaStream_t s) {
+  a.vec = (aligned16(a.dy, a.lddy, sizeof(T)) ? 1 : 0) |
+          (aligned16(a.z, a.ldz, sizeof(T)) ? 2 : 0) | (aligned16(a.u, a.ldz, sizeof(T)) ? 4 : 0);
+  int64_t most = 0;
+  for (int i = 0; i < a.packs.n; ++i)
+    most = std::max(most, a.packs.p[i].rows * a.packs.p[i].ld / 8);
+  a.pack_blocks = grid_of(most);
   auto* kern = a.u ? slope_kernel<T, true> : slope_kernel<T, false>;
-  XVEC_CUDA(launch_pdl(kern, dim3(cols, used), 256, 0, s, 1, static_cast<const T*>(a.dy), a.lddy,
-                       static_cast<const T*>(a.z), static_cast<const T*>(a.u), a.ldz, a.n, a.m,
-                       a.act, vec, per, static_cast<uint16_t*>(a.out), a.ld, partial.as<float>()));
-  if (sums)
-    XVEC_CUDA(launch_pdl(column_sum_kernel<T>, dim3((a.m + 31) / 32, 2), kSumThreads, 0, s, 1,
-                         partial.as<float>(), used, a.m, static_cast<T*>(a.db[0]),
-                         static_cast<T*>(a.db[1])));
+  XVEC_CUDA(launch_pdl(kern, dim3((unsigned)a.cols * a.chunks + a.pack_blocks * a.packs.n), 256, 0,
+                       s, 1, a));
   return XVEC_GPU_OK;
 }
 
-xvec_gpu_status slopes(int storage, const Slopes& a, cudaStream_t s) {
+xvec_gpu_status slopes(int storage, Slopes& a, cudaStream_t s) {
   return storage == XVEC_STORAGE_FP32   ? slopes_t<float>(a, s)
          : storage == XVEC_STORAGE_FP16 ? slopes_t<__half>(a, s)
                                         : slopes_t<bf16>(a, s);
+}
+
+xvec_gpu_status sum_columns(int storage, const GemmParams& p, cudaStream_t s) {
+  auto* kern = storage == XVEC_STORAGE_FP32   ? column_sum_kernel<float>
+               : storage == XVEC_STORAGE_FP16 ? column_sum_kernel<__half>
+                                              : column_sum_kernel<bf16>;
+  XVEC_CUDA(launch_pdl(kern, dim3((unsigned)std::min((p.sum_cols + 15) / 16, 1184)), 128, 0, s, 1,
+                       p.sums, p.sum_chunks, p.sum_cols, p.sum_out[0], p.sum_out[1]));
+  return XVEC_GPU_OK;
 }
 
 // --- argument checks --------------------------------------------------------
@@ -395,6 +444,58 @@ xvec_gpu_status check_shape(const Args* a) {
 
 }  // namespace
 
+// Tile shape and depth splits by a cost estimate in SM clocks.  A tile's blocks
+// overlap the epilogue of the tile before, so a wave takes the longer of the two,
+// and the last epilogue comes on top; splits pay for their partial sums' traffic
+// and a second launch.  Measured: 512 clocks a block for a pair's 256 columns
+// (the matrix rate), 400 for 192, 620 for a single CTA's 128 x 128 (twice the
+// bytes per product); about 20 clocks an epilogue column for each matrix that it
+// reads or writes and for an activation, 45 where rows do not allow 16-byte
+// accesses.  192 columns exist for one product along depth (kLinear), where they
+// can fill the last wave better: 10000 x 960 -> 960 fp32 is 200 tiles of three
+// waves instead of 160 larger ones of three.
+xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
+  const double products = storage == XVEC_STORAGE_FP32 ? 6 : 1;
+  const double block[kShapes] = {512 * products, 400 * products, 620 * products};
+  int device = 0, sms = 0;
+  XVEC_CUDA(cudaGetDevice(&device));
+  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  GemmParams& p = c->p;
+  p.blocks = (int)((c->depth + 63) / 64);
+  p.ldp = (p.cols + 31) / 32 * 32;
+  const int all = p.blocks * p.segs;
+  const int half = c->mode == kGated ? 2 : 1;  // accumulator columns per output column
+  const int matrices = 1 + (p.save[0] != nullptr) + (p.save[1] != nullptr) +
+                       (p.residual != nullptr) + (p.act != XVEC_ACT_NONE);
+  double best = 0;
+  p.splits = 0;
+  for (int k = 0; k < kShapes; ++k) {
+    if (k == 1 && c->mode != kLinear) continue;
+    const int rows = kTileShapes[k].rows, cols = kTileShapes[k].cols / half;
+    const int workers = kTileShapes[k].pair ? sms / 2 : sms;
+    const int64_t tm = (p.rows + rows - 1) / rows, tn = (p.cols + cols - 1) / cols;
+    for (int splits = 1; splits <= 32; ++splits) {
+      const int per = (all + splits - 1) / splits;
+      if (splits > 1 && (per < 4 || (int64_t)per * (splits - 1) >= all)) continue;
+      const double waves = (double)((tm * tn * p.batches * splits + workers - 1) / workers);
+      const double epilogue =
+          cols * (splits > 1 ? 50.0 * half : matrices * (p.vec ? 20.0 : 45.0));
+      double cost = waves * std::max(per * block[k], epilogue) +
+                    std::min(per * block[k], epilogue) + 2500;
+      if (splits > 1)
+        cost += 6000 + (double)splits * p.rows * p.ldp * p.batches * half * 8 / 2000;
+      if (p.splits == 0 || cost < best) {
+        best = cost;
+        c->shape = k;
+        p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.splits = splits, p.blocks_per_split = per;
+      }
+    }
+  }
+  c->partial_bytes =
+      p.splits > 1 ? (size_t)p.splits * p.batches * half * p.rows * p.ldp * 4 : 0;
+  return XVEC_GPU_OK;
+}
+
 xvec_gpu_status DeviceGuard::set(int device) {
   int count = 0;
   if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
@@ -471,13 +572,9 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   GemmCall g;
   g.mode = kLinear;
   g.depth = a.in_dim;
-  Scratch room[2];
-  Packs packs;
-  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, &packs, s)) ||
-      (st = operand(a.storage, a.weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0], &packs,
-                    s)) ||
-      (st = run_packs(a.storage, packs, s)))
-    return st;
+  Arena arena;
+  Operand x = plan_operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &arena);
+  Operand w = plan_operand(a.storage, a.weight, a.out_dim, a.in_dim, a.ldw, &arena);
   GemmParams& p = g.p;
   p.rows = a.n, p.cols = a.out_dim, p.segs = p.batches = 1;
   p.bias[0] = a.bias;
@@ -489,7 +586,7 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   const size_t size = elem_bytes(a.storage);
   p.vec = aligned16(a.y, a.ldy, size) && aligned16(a.residual, a.ldr, size) &&
           aligned16(a.preact, a.ldz, size);
-  return gemm(a.storage, g, s);
+  return forward(a.storage, g, &x, &w, nullptr, arena, s);
 }
 
 extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args) {
@@ -529,15 +626,10 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   GemmCall g;
   g.mode = kGated;
   g.depth = a.in_dim;
-  Scratch room[3];
-  Packs packs;
-  if ((st = operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &room[0], &g.a, &packs, s)) ||
-      (st = operand(a.storage, a.gate_weight, a.out_dim, a.in_dim, a.ldw, &room[1], &g.b[0],
-                    &packs, s)) ||
-      (st = operand(a.storage, a.up_weight, a.out_dim, a.in_dim, a.ldw, &room[2], &g.b[1], &packs,
-                    s)) ||
-      (st = run_packs(a.storage, packs, s)))
-    return st;
+  Arena arena;
+  Operand x = plan_operand(a.storage, a.x, a.n, a.in_dim, a.ldx, &arena);
+  Operand wg = plan_operand(a.storage, a.gate_weight, a.out_dim, a.in_dim, a.ldw, &arena);
+  Operand wu = plan_operand(a.storage, a.up_weight, a.out_dim, a.in_dim, a.ldw, &arena);
   GemmParams& p = g.p;
   p.rows = a.n, p.cols = a.out_dim, p.segs = p.batches = 1;
   p.bias[0] = a.gate_bias, p.bias[1] = a.up_bias;
@@ -548,7 +640,7 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   const size_t size = elem_bytes(a.storage);
   p.vec = aligned16(a.h, a.ldh, size) && aligned16(a.gate, a.ldg, size) &&
           aligned16(a.up, a.ldg, size);
-  return gemm(a.storage, g, s);
+  return forward(a.storage, g, &x, &wg, &wu, arena, s);
 }
 
 namespace xvec {
@@ -581,75 +673,87 @@ xvec_gpu_status run_backward(const Backward& b) {
   }
   const bool products = b.dx || b.dw[0] || b.dw[1], sums = b.db[0] || b.db[1];
   if (!products && !sums) return XVEC_GPU_OK;
+  // The plan: operands, both products and their scratch.
+  Arena arena;
+  Operand w[2], x;
+  if (b.dx)
+    for (int i = 0; i < b.parts; ++i)
+      w[i] = plan_operand(b.storage, b.w[i], b.out_dim, b.in_dim, b.ldw, &arena);
+  if (b.dw[0] || b.dw[1]) x = plan_operand(b.storage, b.x, b.n, b.in_dim, b.ldx, &arena);
   // The pre-activation gradients as one operand of `parts` matrices.  dy itself
   // where no activation changes it and it can be read in place.
-  Scratch dz;
   GemmOperand grad;
   grad.inner = b.out_dim, grad.outer = b.n;
   const bool direct = b.parts == 1 && b.act == XVEC_ACT_NONE && size == 2 &&
                       aligned16(b.dy, b.lddy, size);
+  size_t grad_at = 0;
   if (direct) {
     grad.p = b.dy, grad.ld = b.lddy;
   } else {
     grad.ld = round8(b.out_dim);
     grad.plane = b.n * grad.ld;
     grad.planes = planes_of(b.storage) * b.parts;
-    if (products) {
-      if ((st = dz.alloc((size_t)grad.planes * grad.plane * 2, s))) return st;
-      grad.p = dz.ptr;
-    }
+    if (products) grad_at = arena.add((size_t)grad.planes * grad.plane * 2);
   }
+  Slopes a{};
+  a.dy = b.dy, a.z = b.pre[0], a.u = b.parts == 2 ? b.pre[1] : nullptr;
+  a.lddy = b.lddy, a.ldz = b.ldpre, a.n = b.n, a.m = b.out_dim, a.act = b.act;
+  a.ld = grad.ld;
+  plan_slopes(&a);
+  const size_t sums_at = sums ? arena.add((size_t)2 * a.chunks * a.m * 4) : 0;
+  GemmCall dx, dw;
+  dx.mode = kDx;
+  dx.depth = b.out_dim;
+  dx.p.rows = b.n, dx.p.cols = b.in_dim, dx.p.segs = b.parts, dx.p.batches = 1;
+  dx.p.out[0] = b.dx, dx.p.ldo = b.lddx;
+  dx.p.vec = aligned16(b.dx, b.lddx, size);
+  dx.p.status = b.status;
+  dw.mode = kDw;
+  dw.depth = b.n;
+  dw.p.rows = b.out_dim, dw.p.cols = b.in_dim, dw.p.segs = 1;
+  dw.p.vec = 1;
+  dw.p.ldo = b.lddw;
+  dw.p.status = b.status;
+  const int first = b.dw[0] ? 0 : 1;  // 1: only the second weight's gradient
+  for (int i = first; i < b.parts && b.dw[i]; ++i) {
+    dw.p.out[dw.p.batches++] = b.dw[i];
+    dw.p.vec &= aligned16(b.dw[i], b.lddw, size);
+  }
+  if (b.dx && (st = plan_gemm(b.storage, &dx))) return st;
+  if (dw.p.batches && (st = plan_gemm(b.storage, &dw))) return st;
+  // (One after the other: they can share the place for split sums.)
+  const size_t partial_at = arena.add(std::max(dx.partial_bytes, dw.partial_bytes));
+
+  if ((st = arena.alloc(s))) return st;
+  for (Operand* o : {&w[0], &w[1], &x}) place(o, arena, &a.packs);
+  if (!direct && products) grad.p = a.out = static_cast<uint16_t*>(arena.at(grad_at));
+  if (sums) a.partial = static_cast<float*>(arena.at(sums_at));
   if (!direct || sums) {
-    Slopes a{};
-    a.dy = b.dy, a.z = b.pre[0], a.u = b.pre[1];
-    a.lddy = b.lddy, a.ldz = b.ldpre, a.n = b.n, a.m = b.out_dim, a.act = b.act;
-    a.out = dz.ptr, a.ld = grad.ld;
-    a.db[0] = b.db[0], a.db[1] = b.db[1];
     if ((st = slopes(b.storage, a, s))) return st;
+  } else if ((st = run_packs(b.storage, a.packs, s))) {
+    return st;
   }
-  Scratch room[3];
-  GemmOperand w[2], x;
-  Packs packs;
-  if (b.dx)
-    for (int i = 0; i < b.parts; ++i)
-      if ((st = operand(b.storage, b.w[i], b.out_dim, b.in_dim, b.ldw, &room[i], &w[i], &packs, s)))
-        return st;
-  if (b.dw[0] || b.dw[1])
-    if ((st = operand(b.storage, b.x, b.n, b.in_dim, b.ldx, &room[2], &x, &packs, s))) return st;
-  if ((st = run_packs(b.storage, packs, s))) return st;
+  GemmParams& carrier = b.dx ? dx.p : dw.p;  // takes the column sums along
+  if (sums) {
+    carrier.sums = a.partial, carrier.sum_chunks = a.chunks, carrier.sum_cols = a.m;
+    carrier.sum_out[0] = b.db[0], carrier.sum_out[1] = b.db[1];
+    if (!products) return sum_columns(b.storage, carrier, s);
+  }
   if (b.dx) {
-    GemmCall g;
-    g.mode = kDx;
-    g.depth = b.out_dim;
-    g.a = grad;
-    for (int i = 0; i < b.parts; ++i) g.b[i] = w[i];
-    g.p.rows = b.n, g.p.cols = b.in_dim, g.p.segs = b.parts, g.p.batches = 1;
-    g.p.out[0] = b.dx, g.p.ldo = b.lddx;
-    g.p.vec = aligned16(b.dx, b.lddx, size);
-    g.p.status = b.status;
-    if ((st = gemm(b.storage, g, s))) return st;
+    dx.a = grad;
+    dx.b[0] = w[0].g, dx.b[1] = w[1].g;
+    if (dx.partial_bytes) dx.p.partial = static_cast<float*>(arena.at(partial_at));
+    if ((st = gemm(b.storage, dx, s))) return st;
   }
-  if (b.dw[0] || b.dw[1]) {
-    GemmCall g;
-    g.mode = kDw;
-    g.depth = b.n;
-    g.a = grad;
-    g.b[0] = x;
-    g.p.rows = b.out_dim, g.p.cols = b.in_dim, g.p.segs = 1;
-    g.p.vec = 1;
-    // Only the second weight's gradient: start at its matrix.
-    const int first = b.dw[0] ? 0 : 1;
+  if (dw.p.batches) {
+    dw.a = grad;
     if (first) {
-      g.a.p = static_cast<const uint16_t*>(grad.p) + planes_of(b.storage) * grad.plane;
-      g.a.planes = planes_of(b.storage);
+      dw.a.p = static_cast<const uint16_t*>(grad.p) + planes_of(b.storage) * grad.plane;
+      dw.a.planes = planes_of(b.storage);
     }
-    for (int i = first; i < b.parts && b.dw[i]; ++i) {
-      g.p.out[g.p.batches++] = b.dw[i];
-      g.p.vec &= aligned16(b.dw[i], b.lddw, size);
-    }
-    g.p.ldo = b.lddw;
-    g.p.status = b.status;
-    if ((st = gemm(b.storage, g, s))) return st;
+    dw.b[0] = x.g;
+    if (dw.partial_bytes) dw.p.partial = static_cast<float*>(arena.at(partial_at));
+    if ((st = gemm(b.storage, dw, s))) return st;
   }
   return XVEC_GPU_OK;
 }

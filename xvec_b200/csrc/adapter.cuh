@@ -222,6 +222,10 @@ struct GemmParams {
   void* save[2];
   int64_t ldr, ldo, lds;
   int act;
+  // Column sums for the warps that have no part in the product (column_sums).
+  const float* sums;
+  int sum_chunks, sum_cols;
+  void* sum_out[2];
   int* status;
   uint64_t wait_ns;
 };
@@ -241,11 +245,44 @@ struct GemmCall {
   int64_t depth = 0;
   GemmOperand a, b[2];
   GemmParams p{};
+  int shape = 0;              // of the tiles (plan_gemm)
+  size_t partial_bytes = 0;   // scratch for split sums, at p.partial
 };
+constexpr int kShapes = 3;
+struct TileShape {
+  int rows, cols;  // cols: of the accumulator (half as many outputs when gated)
+  bool pair;
+};
+constexpr TileShape kTileShapes[kShapes] = {{256, 256, true}, {256, 192, true}, {128, 128, false}};
+// Picks the tiles and splits: fills in c's tiling and partial_bytes.
+xvec_gpu_status plan_gemm(int storage, GemmCall* c);
 // By the storage type of the outputs; float32: operands are three bfloat16 planes.
 xvec_gpu_status gemm_fp32(const GemmCall& c, cudaStream_t s);
 xvec_gpu_status gemm_fp16(const GemmCall& c, cudaStream_t s);
 xvec_gpu_status gemm_bf16(const GemmCall& c, cudaStream_t s);
+
+// out[o][c] = the sum over the chunks of sums[o][chunk][c], o = 0, 1, in a fixed
+// order: four interleaved runs, then those.  Warp `worker` of `workers` takes
+// every workers-th group of 8 columns.
+template <typename T>
+__device__ __forceinline__ void column_sums(const float* sums, int chunks, int m, void* out0,
+                                            void* out1, int worker, int workers, int lane) {
+  const int groups = (m + 7) / 8;
+  for (int g = worker; g < 2 * groups; g += workers) {
+    T* out = static_cast<T*>(g < groups ? out0 : out1);
+    if (!out) continue;
+    const int c = (g < groups ? g : g - groups) * 8 + (lane & 7);
+    const float* p = sums + (g < groups ? 0 : (int64_t)chunks * m) + c;
+    float s = 0.f;
+    if (c < m) {
+#pragma unroll 8
+      for (int i = lane >> 3; i < chunks; i += 4) s += p[(int64_t)i * m];
+    }
+    s += __shfl_xor_sync(0xffffffffu, s, 8);
+    s += __shfl_xor_sync(0xffffffffu, s, 16);
+    if (lane < 8 && c < m) out[c] = from_f<T>(s);
+  }
+}
 
 // Rows read in place with 16-byte accesses.
 inline bool aligned16(const void* p, int64_t ld, size_t size) {

@@ -14,6 +14,7 @@
 //                stages (128-byte swizzle)
 //     warp 1     tensor memory; one thread issues tcgen05.mma (fp32 accumulators,
 //                two of them, so that a tile's epilogue overlaps the next tile)
+//     warps 2-3  column sums of an earlier launch, where the call has some
 //     warps 4-11 epilogue: tcgen05.ld, bias, activation, product, residual
 //   PAIR: two CTAs (cta_group::2) share a tile of 256 rows x BN columns, each
 //   loading half of A's rows and half of B's columns.
@@ -50,7 +51,7 @@ constexpr int kBM = 128;      // rows per CTA (TMEM lanes)
 constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr int kBand = 8;      // row tiles per band of the tile order
-constexpr int kFewRegs = 40, kManyRegs = 232;
+constexpr int kFewRegs = 56, kManyRegs = 224;
 constexpr int kRound = 2;     // float32: depth blocks per accumulation in tensor memory
 
 template <typename T, bool PAIR, int BN>
@@ -508,6 +509,9 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
       // Retire every issued MMA before tensor memory is released.
       mma_commit<PAIR>(smem_u32(mdone));
       if (!mbar_wait(mdone, 0, nullptr)) fail();
+    } else if (warp >= 2 && p.sums) {
+      column_sums<T>(p.sums, p.sum_chunks, p.sum_cols, p.sum_out[0], p.sum_out[1],
+                     (int)blockIdx.x * 2 + warp - 2, (int)gridDim.x * 2, lane);
     }
   } else {
     // ---------------- epilogue ----------------
@@ -787,7 +791,8 @@ inline bool operand_map(CUtensorMap* map, const GemmOperand& o, int box_outer) {
 }
 
 template <int MODE, typename T, bool PAIR, int BN>
-xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaStream_t s) {
+xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
+  GemmParams p = c.p;
   using S = GemmShape<T, PAIR, BN>;
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   CUtensorMap a, b0, b1;
@@ -814,8 +819,12 @@ xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaS
     }
   }
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.batches * p.splits;
-  XVEC_CUDA(launch_pdl(kern, dim3((unsigned)std::min<int64_t>(items, workers) * (PAIR ? 2 : 1)),
-                       S::kThreads, S::kSmemBytes, s, PAIR ? 2 : 1, a, b0, b1, p));
+  int device = 0, sms = 0;
+  XVEC_CUDA(cudaGetDevice(&device));
+  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  const int64_t ctas = PAIR ? std::min<int64_t>(items, sms / 2) * 2 : std::min<int64_t>(items, sms);
+  XVEC_CUDA(launch_pdl(kern, dim3((unsigned)ctas), S::kThreads, S::kSmemBytes, s,
+                       PAIR ? 2 : 1, a, b0, b1, p));
   if (p.splits > 1) {
     const int64_t groups = (p.cols + 3) / 4 * p.rows;
     XVEC_CUDA(launch_pdl(finish_kernel<MODE, T>,
@@ -826,67 +835,12 @@ xvec_gpu_status launch_shape(const GemmCall& c, GemmParams p, int workers, cudaS
   return XVEC_GPU_OK;
 }
 
-// Tile shape and depth splits by a cost estimate in SM clocks.  A tile's blocks
-// overlap the epilogue of the tile before, so a wave takes the longer of the two,
-// and the last epilogue comes on top; splits pay for their partial sums' traffic
-// and a second launch.  Measured: 512 clocks a block for a pair's 256 columns
-// (the matrix rate), 400 for 192, 620 for a single CTA's 128 x 128 (twice the
-// bytes per product); about 20 clocks an epilogue column for each matrix that it
-// reads or writes and for an activation, 45 where rows do not allow 16-byte
-// accesses.  192 columns exist for one product along depth (kLinear), where they
-// can fill the last wave better: 10000 x 960 -> 960 fp32 is 200 tiles of three
-// waves instead of 160 larger ones of three.
 template <int MODE, typename T>
 xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
-  constexpr double kProducts = std::is_same<T, float>::value ? 6 : 1;
-  int device = 0, sms = 0;
-  XVEC_CUDA(cudaGetDevice(&device));
-  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-  GemmParams p = c.p;
-  p.blocks = (int)((c.depth + kBK - 1) / kBK);
-  const int all = p.blocks * p.segs;
-  p.ldp = (p.cols + 31) / 32 * 32;
-  struct Config {
-    int rows, cols, workers;
-    double block;  // clocks per depth block
-    bool use;
-  };
-  constexpr int kHalf = MODE == kGated ? 2 : 1;  // accumulator columns per output column
-  const Config configs[] = {{256, 256 / kHalf, sms / 2, 512.0 * kProducts, true},
-                            {256, 192, sms / 2, 400.0 * kProducts, MODE == kLinear},
-                            {128, 128 / kHalf, sms, 620.0 * kProducts, true}};
-  const int matrices = 1 + (p.save[0] != nullptr) + (p.save[1] != nullptr) +
-                       (p.residual != nullptr) + (p.act != XVEC_ACT_NONE);
-  double best = 0;
-  const Config* pick = nullptr;
-  for (const Config& k : configs) {
-    if (!k.use) continue;
-    const int64_t tm = (p.rows + k.rows - 1) / k.rows, tn = (p.cols + k.cols - 1) / k.cols;
-    for (int splits = 1; splits <= 32; ++splits) {
-      const int per = (all + splits - 1) / splits;
-      if (splits > 1 && (per < 4 || (int64_t)per * (splits - 1) >= all)) continue;
-      const double waves = (double)((tm * tn * p.batches * splits + k.workers - 1) / k.workers);
-      const double epilogue = k.cols * (splits > 1 ? 50.0 * kHalf : matrices * (p.vec ? 20.0 : 45.0));
-      double cost = waves * std::max(per * k.block, epilogue) +
-                    std::min(per * k.block, epilogue) + 2500;
-      if (splits > 1)
-        cost += 6000 + (double)splits * p.rows * p.ldp * p.batches * kHalf * 8 / 2000;
-      if (!pick || cost < best) {
-        best = cost, pick = &k;
-        p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.splits = splits, p.blocks_per_split = per;
-      }
-    }
-  }
-  Scratch partial;
-  if (p.splits > 1) {
-    const int64_t sums = (int64_t)p.splits * p.batches * kHalf * p.rows * p.ldp;
-    if (xvec_gpu_status st = partial.alloc((size_t)sums * 4, s)) return st;
-    p.partial = partial.as<float>();
-  }
-  if (pick->rows == 128) return launch_shape<MODE, T, false, 128>(c, p, pick->workers, s);
+  if (c.shape == 2) return launch_shape<MODE, T, false, 128>(c, s);
   if constexpr (MODE == kLinear)
-    if (pick->cols == 192) return launch_shape<MODE, T, true, 192>(c, p, pick->workers, s);
-  return launch_shape<MODE, T, true, 256>(c, p, pick->workers, s);
+    if (c.shape == 1) return launch_shape<MODE, T, true, 192>(c, s);
+  return launch_shape<MODE, T, true, 256>(c, s);
 }
 
 template <typename T>
