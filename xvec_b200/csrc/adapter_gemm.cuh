@@ -63,21 +63,27 @@ struct GemmShape {
   static constexpr int kThreads = 128 + kEpiWarps * 32;
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B columns loaded per CTA
   static constexpr uint32_t kBBytes = kBRows * kBK * 2;
-  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+  // A stage holds one plane of a depth block (float32), or two blocks (16-bit): a
+  // stage's handshake takes its single threads about 350 clocks, one block's
+  // instructions 512 or less.
+  static constexpr int kUnits = std::is_same<T, float>::value ? 1 : 2;
+  static constexpr uint32_t kBlockBytes = kABytes + kBBytes;
+  static constexpr uint32_t kStageBytes = kUnits * kBlockBytes;
   // Per epilogue warp: a bias per column and a 32 x 64 byte staging block.
   static constexpr uint32_t kEpiBytes = kEpiWarps * (BN / 2 * 4 + 2048);
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + 512;
   static constexpr int kTmemCols = BN == 192 ? 512 : 2 * BN;  // two accumulators, a power of two
-  static_assert(kStages >= 4, "shared memory too small for the stage ring");
+  static_assert(kStages * kUnits >= 6, "shared memory too small for the stage ring");
 };
 
 // --- barriers, operands, matrix instructions --------------------------------------
-// The producer and the issuer are single threads whose instruction count bounds
-// the rate of the ring (at 64 deep a stage has 512 clocks), so addresses are
+// The producer and the issuer are single threads whose instruction count can bound
+// the rate of the ring (a block has 512 clocks or less), so addresses are
 // 32-bit shared ones, descriptors are kept as sums, and the limit and the abort
-// flag are looked at only after a failed try.
+// flag are looked at only after a failed try.  (With a generic wait, a division
+// and an abort check for each block they took 780 clocks.)
 __device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -317,7 +323,8 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
   uint64_t* tempty = tfull + 2;       // [2] accumulator drained (issuing CTA's count)
   uint64_t* mdone = tempty + 2;       // all issued MMAs retired
   uint32_t* issued = reinterpret_cast<uint32_t*>(mdone + 1);  // [kStages] copies per stage
-  uint32_t* tmem_slot = issued + kStages;
+  uint32_t* units = issued + kStages;  // [kStages] blocks of the stage's last filling
+  uint32_t* tmem_slot = units + kStages;
   __shared__ int s_abort_storage;
   volatile int* s_abort = &s_abort_storage;
 
@@ -339,7 +346,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      issued[s] = 0;
+      issued[s] = units[s] = 0;
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
@@ -404,36 +411,49 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
         int seg = it.k0 / p.blocks;
         int k = (it.k0 - seg * p.blocks) * kBK;
         const int k_end = p.blocks * kBK;
-        for (int n = it.k1 - it.k0; n > 0 && ok; --n) {
-          const int az = (MODE == kDw ? it.batch : MODE == kDx ? seg : 0) * P;
+        // One block of A and B into `a`, from depth k of product seg, plane pl.
+        auto load = [&](uint32_t bar, uint32_t a, int pl) {
+          const uint32_t b = a + kABytes;
+          const int az = (MODE == kDw ? it.batch : MODE == kDx ? seg : 0) * P + pl;
           const CUtensorMap* bm = (MODE == kDx && seg) || (MODE == kGated && PAIR && rank) ? &bmap1
                                                                                           : &bmap0;
+          if constexpr (A_MN) {
+            load_box<PAIR>(&amap, bar, a, row0, k, az);
+            load_box<PAIR>(&amap, bar, a + 8192, row0 + 64, k, az);
+          } else {
+            load_box<PAIR>(&amap, bar, a, k, row0, az);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int c = 0; c < S::kBRows / 64; ++c)
+              load_box<PAIR>(bm, bar, b + c * 8192, col0 + c * 64, k, pl);
+          } else {
+            // Gated: the gate's columns, then the up's (PAIR: one in each CTA).
+            load_box<PAIR>(bm, bar, b, k, col0, pl);
+            if constexpr (MODE == kGated && !PAIR)
+              load_box<PAIR>(&bmap1, bar, b + S::kBBytes / 2, k, col0, pl);
+          }
+        };
+        for (int n = it.k1 - it.k0; n > 0 && ok; n -= S::kUnits) {
 #pragma unroll
           for (int pl = 0; pl < P; ++pl) {
             if (!(ok = ok && wait_bar(empty_at + stage * 8, phase ^ 1, s_abort, limit))) break;
-            const uint32_t a = tiles_at + stage * S::kStageBytes, b = a + kABytes;
-            const uint32_t bar = bars + stage * 8;
-            if (issuer) expect_bytes(full_at + stage * 8, (PAIR ? 2 : 1) * S::kStageBytes);
-            if constexpr (A_MN) {
-              load_box<PAIR>(&amap, bar, a, row0, k, az + pl);
-              load_box<PAIR>(&amap, bar, a + 8192, row0 + 64, k, az + pl);
-            } else {
-              load_box<PAIR>(&amap, bar, a, k, row0, az + pl);
+            const uint32_t at = tiles_at + stage * S::kStageBytes, bar = bars + stage * 8;
+            const uint32_t blocks = min(n, S::kUnits);
+            if (issuer) expect_bytes(full_at + stage * 8, (PAIR ? 2 : 1) * blocks * S::kBlockBytes);
+            load(bar, at, pl);
+            if constexpr (P == 1) {
+              if ((k += kBK) == k_end) k = 0, ++seg;
+              if (blocks > 1) {
+                load(bar, at + S::kBlockBytes, pl);
+                if ((k += kBK) == k_end) k = 0, ++seg;
+              }
             }
-            if constexpr (B_MN) {
-#pragma unroll
-              for (int c = 0; c < S::kBRows / 64; ++c)
-                load_box<PAIR>(bm, bar, b + c * 8192, col0 + c * 64, k, pl);
-            } else {
-              // Gated: the gate's columns, then the up's (PAIR: one in each CTA).
-              load_box<PAIR>(bm, bar, b, k, col0, pl);
-              if constexpr (MODE == kGated && !PAIR)
-                load_box<PAIR>(&bmap1, bar, b + S::kBBytes / 2, k, col0, pl);
-            }
+            units[stage] = blocks;
             ++count;
             if (++stage == kStages) stage = 0, phase ^= 1;
           }
-          if ((k += kBK) == k_end) k = 0, ++seg;
+          if (P == 3 && (k += kBK) == k_end) k = 0, ++seg;
         }
       }
       if (!ok) fail();
@@ -455,9 +475,11 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
         tmem_fence_after();
         return got;
       };
-      // A's plane in stage i times B's in stage j, into d; keep = 0 overwrites it.
-      auto multiply = [&](uint32_t i, uint32_t j, uint32_t d, uint32_t keep) {
-        const uint64_t a = a0 + i * (S::kStageBytes >> 4), b = b0 + j * (S::kStageBytes >> 4);
+      // A's block in stage i times B's in stage j, both `off` further, into d; keep = 0
+      // overwrites it.
+      auto multiply = [&](uint32_t i, uint32_t j, uint32_t d, uint32_t keep, uint32_t off = 0) {
+        const uint64_t a = a0 + (i * (S::kStageBytes >> 4) + off);
+        const uint64_t b = b0 + (j * (S::kStageBytes >> 4) + off);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           mma_16bit<PAIR>(d, a + k * kDepthStep<A_MN>, b + k * kDepthStep<B_MN>, p.idesc,
@@ -470,10 +492,11 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
           const uint32_t acc = tile & 1, d = tmem_base + acc * BN;
           if (!(ok = wait_bar(tempty_at + acc * 8, ((tile >> 1) & 1) ^ 1, s_abort, limit))) break;
           tmem_fence_after();
-          for (int k = it.k0; k < it.k1; ++k) {
+          for (int k = it.k0; k < it.k1; k += S::kUnits) {
             uint32_t at;
             if (!(ok = next(&at))) break;
             multiply(at, at, d, k > it.k0);
+            if (k + 1 < it.k1) multiply(at, at, d, 1, S::kBlockBytes >> 4);
             commit<PAIR>(empty_at + at * 8);
           }
           commit<PAIR>(tfull_at + acc * 8);
@@ -702,7 +725,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
           !mbar_wait(&full[s], (mine - 1) & 1, nullptr, other < mine ? 20000000ull : kWaitLimitNs))
         fail();
       if (PAIR && other > mine) {
-        mbar_expect_tx(&full[s], S::kStageBytes);
+        mbar_expect_tx(&full[s], ld_cluster_u32(cluster_addr(&units[s], 1)) * S::kBlockBytes);
         if (!mbar_wait(&full[s], mine & 1, nullptr)) fail();
       }
     }
