@@ -444,19 +444,20 @@ xvec_gpu_status check_shape(const Args* a) {
 
 }  // namespace
 
-// Tile shape and depth splits by a cost estimate in SM clocks.  A tile's blocks
-// overlap the epilogue of the tile before, so a wave takes the longer of the two,
-// and the last epilogue comes on top; splits pay for their partial sums' traffic
-// and a second launch.  Measured: 512 clocks a block for a pair's 256 columns
-// (the matrix rate), 400 for 192, 620 for a single CTA's 128 x 128 (twice the
-// bytes per product); about 20 clocks an epilogue column for each matrix that it
-// reads or writes and for an activation, 45 where rows do not allow 16-byte
-// accesses.  192 columns exist for one product along depth (kLinear), where they
-// can fill the last wave better: 10000 x 960 -> 960 fp32 is 200 tiles of three
-// waves instead of 160 larger ones of three.
+// Tile shape and depth splits by a cost estimate in SM clocks: a wave's blocks
+// and epilogue (which overlap in time but share shared memory and power: their
+// times were seen to add up), a start, and for splits the traffic of their partial
+// sums and a second launch.  A block takes 512 clocks for a pair's 256 columns (the
+// matrix rate), 448 for 192, 384 for 128 (shared memory's rate), 590 for a single
+// CTA's 128 x 128.  An epilogue column takes about 10 clocks for each matrix that
+// it reads or writes and for an activation, 25 where rows do not allow 16-byte
+// accesses.  192 columns exist for one product along depth (kLinear), where they can
+// fill the last wave better: 10000 x 960 -> 960 fp32 is 200 tiles of three waves
+// instead of 160 larger ones of three.
 xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
   const double products = storage == XVEC_STORAGE_FP32 ? 6 : 1;
-  const double block[kShapes] = {512 * products, 400 * products, 620 * products};
+  const double block[kShapes] = {512 * products, 448 * products, 384 * products, 590 * products};
+  const double start[kShapes] = {7500, 7500, 7500, 3000};
   int device = 0, sms = 0;
   XVEC_CUDA(cudaGetDevice(&device));
   XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
@@ -479,9 +480,8 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
       if (splits > 1 && (per < 4 || (int64_t)per * (splits - 1) >= all)) continue;
       const double waves = (double)((tm * tn * p.batches * splits + workers - 1) / workers);
       const double epilogue =
-          cols * (splits > 1 ? 50.0 * half : matrices * (p.vec ? 20.0 : 45.0));
-      double cost = waves * std::max(per * block[k], epilogue) +
-                    std::min(per * block[k], epilogue) + 2500;
+          cols * (splits > 1 ? 25.0 * half : matrices * (p.vec ? 10.0 : 25.0));
+      double cost = waves * (per * block[k] + epilogue) + start[k];
       if (splits > 1)
         cost += 6000 + (double)splits * p.rows * p.ldp * p.batches * half * 8 / 2000;
       if (p.splits == 0 || cost < best) {

@@ -248,12 +248,13 @@ struct GemmCall {
   int shape = 0;              // of the tiles (plan_gemm)
   size_t partial_bytes = 0;   // scratch for split sums, at p.partial
 };
-constexpr int kShapes = 3;
+constexpr int kShapes = 4;
 struct TileShape {
   int rows, cols;  // cols: of the accumulator (half as many outputs when gated)
   bool pair;
 };
-constexpr TileShape kTileShapes[kShapes] = {{256, 256, true}, {256, 192, true}, {128, 128, false}};
+constexpr TileShape kTileShapes[kShapes] = {
+    {256, 256, true}, {256, 192, true}, {256, 128, true}, {128, 128, false}};
 // Picks the tiles and splits: fills in c's tiling and partial_bytes.
 xvec_gpu_status plan_gemm(int storage, GemmCall* c);
 // By the storage type of the outputs; float32: operands are three bfloat16 planes.

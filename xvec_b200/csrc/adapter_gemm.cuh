@@ -16,8 +16,13 @@
 //                two of them, so that a tile's epilogue overlaps the next tile)
 //     warps 2-3  column sums of an earlier launch, where the call has some
 //     warps 4-11 epilogue: tcgen05.ld, bias, activation, product, residual
-//   PAIR: two CTAs (cta_group::2) share a tile of 256 rows x BN columns, each
-//   loading half of A's rows and half of B's columns.
+//   PAIR: two CTAs on neighbouring SMs (cta_group::2) share a tile of 256 rows x
+//   BN columns: each loads half of A's rows and half of B's columns and holds half
+//   of the rows' sums.  Operands come out of shared memory at 64 bytes a clock: an
+//   instruction of depth 16 reads 4 KB of A and BN x 16 bytes of B in each SM of a
+//   pair, so 128 clocks for 256 columns (the matrix rate) and 96 for 128; a single
+//   CTA's 128 x 128 reads 8 KB, 128 clocks for a quarter of the first's work, but it
+//   starts and ends 1.5 us sooner, which decides for the smallest products.
 //
 // 16-bit storage multiplies its elements as they are.  float32 storage comes
 // as three bfloat16 planes h + m + l (24 bits, x exactly); a stage holds one
@@ -28,8 +33,7 @@
 // kRound blocks to be added in registers (8 truncations instead of 48), and the
 // five products that are 2^8 times smaller have another that leaves at the end.
 // hh is drained while the small products of the same block are issued, so one
-// accumulator of each suffices and the tile keeps 256 columns: at 128 an
-// instruction waits for its operands in shared memory (105 clocks, not 64).
+// accumulator of each suffices and the tile can keep 256 columns.
 // The drained sums take the registers that the other warps give up (setmaxnreg).
 //
 // Every mbarrier wait is bounded; on expiry the kernel sets *status, stops
@@ -860,7 +864,8 @@ xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
 
 template <int MODE, typename T>
 xvec_gpu_status launch_gemm(const GemmCall& c, cudaStream_t s) {
-  if (c.shape == 2) return launch_shape<MODE, T, false, 128>(c, s);
+  if (c.shape == 3) return launch_shape<MODE, T, false, 128>(c, s);
+  if (c.shape == 2) return launch_shape<MODE, T, true, 128>(c, s);
   if constexpr (MODE == kLinear)
     if (c.shape == 1) return launch_shape<MODE, T, true, 192>(c, s);
   return launch_shape<MODE, T, true, 256>(c, s);
