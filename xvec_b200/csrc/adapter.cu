@@ -561,7 +561,7 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
   cudaStream_t s = static_cast<cudaStream_t>(a.stream);
-  if (a.n <= kFewRows) {
+  if (use_few_rows(a.storage, a.n, a.in_dim, a.out_dim, 1)) {
     FewRows f{};
     f.n = (int)a.n, f.in_dim = a.in_dim, f.out_dim = a.out_dim, f.act = a.activation;
     f.x = a.x, f.w[0] = a.weight, f.bias[0] = a.bias, f.residual = a.residual;
@@ -614,7 +614,7 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
   cudaStream_t s = static_cast<cudaStream_t>(a.stream);
-  if (a.n <= kFewRows) {
+  if (use_few_rows(a.storage, a.n, a.in_dim, a.out_dim, 2)) {
     FewRows f{};
     f.n = (int)a.n, f.in_dim = a.in_dim, f.out_dim = a.out_dim, f.act = a.activation;
     f.x = a.x, f.w[0] = a.gate_weight, f.w[1] = a.up_weight;

@@ -291,7 +291,19 @@ inline bool aligned16(const void* p, int64_t ld, size_t size) {
 }
 
 // The forward calls for a few rows (adapter_few.cu): kLinear, or with two weights kGated.
-constexpr int kFewRows = 8;
+// Whether they go through few_rows.  Estimates in us, M = millions of weights,
+// for each eight rows: few rows 0.65 M (16-bit, up to four rows), 3 M (more), 0.95 M
+// and 1.2 M (float32); the matrix kernel 9.6 + 0.2 M, and for float32, whose
+// weights it has to split first, 15 + 3.3 M.  Measured, 1024 x 1024 fp16: 4 rows 2.9
+// against 9.5, 16 rows 4.4 against 9.5; 4096 x 4096: 4 rows 12.5 against 12.8, 8 rows
+// 22.8 against 12.8; fp32 8 rows 20.5 against 70.
+inline bool use_few_rows(int storage, int64_t n, int64_t in_dim, int64_t out_dim, int weights) {
+  if (n > 64) return false;
+  const double m = 1e-6 * (double)in_dim * (double)out_dim * weights;
+  const double groups = (double)((n + 7) / 8);
+  return storage == XVEC_STORAGE_FP32 ? groups * (n <= 4 ? 0.95 : 1.2) * m < 15 + 3.3 * m
+                                      : groups * (n <= 4 ? 0.65 : 3.0) * m < 9.6 + 0.2 * m;
+}
 struct FewRows {
   int n, in_dim, out_dim, act;
   const void *x, *w[2], *bias[2], *residual;

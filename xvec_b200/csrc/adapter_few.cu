@@ -1,13 +1,15 @@
-// adapter_few.cu — the adapter's forward calls for one to eight rows (single queries).
+// adapter_few.cu — the adapter's forward calls for a few rows (queries).
 //
 // With so few rows every weight is used a few times only: bound by reading the
-// weights once, and at the smallest sizes by latency.  A warp owns kCols output
-// columns and reads their weight rows 8 elements a lane (256 deep at a time), with the
-// x rows beside them (from L1 or L2), in float32 multiply-adds; the partial sums
-// of all rows and columns are added across the lanes in a halving exchange that
-// leaves each sum on one lane, which finishes it.  More columns a warp use an x
-// row more often; fewer spread a small weight over more SMs: one or two columns
-// up to two rows, four for eight.
+// weights once, and at the smallest sizes by latency.  A block owns kCols output
+// columns for up to eight rows; its four warps split the depth (blocks of 256, 8
+// elements a lane), so that even a small layer has its weights under way on every
+// SM at once, and the x rows come from L1 or L2.  float32 multiply-adds; the partial
+// sums of all rows and columns are added across the lanes in a halving exchange
+// that leaves each sum on one lane, then over the warps in shared memory, in a
+// fixed order.  More columns a block use an x row more often; fewer spread a small
+// weight over more SMs: one or two columns up to four rows, four for eight.  More than
+// eight rows read the weights again for each eight.
 #include "adapter.cuh"
 
 namespace xvec {
@@ -47,13 +49,12 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_cons
                                                                bool x_vec, bool w_vec) {
   constexpr int W = GATED ? 2 : 1;
   pdl_begin();
-  const int lane = threadIdx.x & 31;
-  const int c0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * COLS;
-  if (c0 >= p.out_dim) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c0 = blockIdx.x * COLS, r0 = blockIdx.y * ROWS;
   const T* x = static_cast<const T*>(p.x);
   float sum[W][ROWS * COLS] = {};
 #pragma unroll 2
-  for (int k = lane * 8; k < p.in_dim; k += 256) {
+  for (int k = threadIdx.x * 8; k < p.in_dim; k += kWarps * 256) {
     const int count = p.in_dim - k;
     float w[W][COLS][8];
 #pragma unroll
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_cons
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       float v[8];
-      load8(x + (int64_t)min(r, p.n - 1) * p.ldx + k, count, x_vec, v);
+      load8(x + (int64_t)min(r0 + r, p.n - 1) * p.ldx + k, count, x_vec, v);
 #pragma unroll
       for (int m = 0; m < W; ++m)
 #pragma unroll
@@ -75,16 +76,23 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_cons
             sum[m][r * COLS + c] = fmaf(v[j], w[m][c][j], sum[m][r * COLS + c]);
     }
   }
-  float total[W];
+  // Lane `lane` >> kShift holds one sum of its warp; the first warp adds them up.
+  constexpr int kSums = ROWS * COLS, kShift = 5 - log2_of(kSums);
+  __shared__ float part[W][kWarps][kSums];
 #pragma unroll
-  for (int m = 0; m < W; ++m) total[m] = scatter_sum(sum[m], lane);
-  constexpr int kShift = 5 - log2_of(ROWS * COLS);
-  const int r = (lane >> kShift) / COLS, c = c0 + (lane >> kShift) % COLS;
-  if ((lane & ((1 << kShift) - 1)) || r >= p.n || c >= p.out_dim) return;
+  for (int m = 0; m < W; ++m) {
+    const float total = scatter_sum(sum[m], lane);
+    if ((lane & ((1 << kShift) - 1)) == 0) part[m][warp][lane >> kShift] = total;
+  }
+  __syncthreads();
+  const int r = r0 + (int)threadIdx.x / COLS, c = c0 + (int)threadIdx.x % COLS;
+  if (threadIdx.x >= kSums || r >= p.n || c >= p.out_dim) return;
   float pre[W];
 #pragma unroll
   for (int m = 0; m < W; ++m) {
-    pre[m] = total[m];
+    pre[m] = part[m][0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) pre[m] += part[m][w][threadIdx.x];
     if (p.bias[m]) pre[m] += to_f(static_cast<const T*>(p.bias[m])[c]);
     if (p.save[m]) static_cast<T*>(p.save[m])[r * p.lds + c] = from_f<T>(pre[m]);
   }
@@ -96,9 +104,9 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_cons
 
 template <typename T, bool GATED, int ROWS, int COLS>
 xvec_gpu_status launch(const FewRows& f, cudaStream_t s) {
-  constexpr int kPer = kWarps * COLS;
-  XVEC_CUDA(launch_pdl(few_rows_kernel<T, GATED, ROWS, COLS>, dim3((f.out_dim + kPer - 1) / kPer),
-                       kWarps * 32, 0, s, 1, f, aligned16(f.x, f.ldx, sizeof(T)),
+  XVEC_CUDA(launch_pdl(few_rows_kernel<T, GATED, ROWS, COLS>,
+                       dim3((f.out_dim + COLS - 1) / COLS, (f.n + ROWS - 1) / ROWS), kWarps * 32,
+                       0, s, 1, f, aligned16(f.x, f.ldx, sizeof(T)),
                        aligned16(f.w[0], f.ldw, sizeof(T)) &&
                            aligned16(f.w[1], f.ldw, sizeof(T))));
   return XVEC_GPU_OK;
@@ -108,7 +116,7 @@ template <typename T, bool GATED>
 xvec_gpu_status by_rows(const FewRows& f, cudaStream_t s) {
   if (f.n == 1) return launch<T, GATED, 1, 1>(f, s);
   if (f.n == 2) return launch<T, GATED, 2, 1>(f, s);
-  if (f.n <= 4) return launch<T, GATED, 4, 2>(f, s);
+  if (f.n <= 4) return launch<T, GATED, 4, GATED ? 1 : 2>(f, s);
   return launch<T, GATED, 8, GATED ? 2 : 4>(f, s);
 }
 template <typename T>
