@@ -36,6 +36,13 @@ SHAPES = [  # n, in_dim, out_dim
     (128, 64, 128), (129, 257, 130), (300, 960, 960), (513, 31, 17), (1000, 127, 770), (2049, 768, 384),
 ]
 LAYOUTS = [(0, 0), (8, 0), (5, 1)]  # pad, skew
+# Sizes that reach every tile shape of the matrix kernel, whole and split depth, tiles whose last
+# rows and columns are few, more tiles than SMs, and the borders of the few-row path.
+LARGE = [
+    (65, 4096, 72), (64, 1030, 4000), (66, 96, 9000), (200, 5000, 300), (257, 640, 513), (1537, 72, 1027),
+    (3000, 640, 1210), (5000, 1111, 192), (10_000, 192, 576), (40_001, 129, 258), (20_000, 100, 2050),
+    (300, 20_000, 40), (2300, 4096, 1024),
+]
 
 
 def run_linear(xb, kind, n, k, m, activation, bias, residual, save, pad=0, skew=0, seed=0):
@@ -77,6 +84,41 @@ def test_linear(xb, kind, shape):
     out = run_linear(xb, kind, *shape, activation, bias=i % 2 == 0, residual=i % 3 != 1,
                      save=i % 4 != 0, pad=pad, skew=skew, seed=i)
     check_linear(*out, activation)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+def test_large(xb, kind, shape):
+    """Each operator at the sizes that choose other tiles."""
+    i = LARGE.index(shape)
+    pad, skew = LAYOUTS[i % 3]
+    activation = list(ACTS)[i % 4]
+    out = run_linear(xb, kind, *shape, activation, i % 2 == 0, i % 3 != 0, i % 2 == 1, pad, skew, seed=i)
+    check_linear(*out, activation)
+    out = run_gated(xb, kind, *shape, activation, i % 2 == 1, i % 2 == 0, pad, skew, seed=i)
+    check_gated(*out, activation)
+    out = run_linear_backward(xb, kind, *shape, activation, "xwb", pad, skew, seed=i)
+    check_backward(kind, activation, *out)
+    out = run_gated_backward(xb, kind, *shape, activation, "xgubc", pad, skew, seed=i)
+    check_backward(kind, activation, *out)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 24, 33, 63, 64, 65])
+def test_few_rows(xb, kind, n):
+    for k, m in ((40, 3), (8, 130), (700, 257), (1500, 1000)):
+        out = run_linear(xb, kind, n, k, m, "silu", True, n % 2 == 0, True, n % 3, n % 2, seed=n)
+        check_linear(*out, "silu")
+        out = run_gated(xb, kind, n, k, m, "gelu", n % 2 == 1, n % 2 == 0, n % 3, n % 2, seed=n)
+        check_gated(*out, "gelu")
+
+
+def test_leading_dimension_of_a_single_row_is_ignored(xb):
+    x, w = torch.randn(1, 64, device="cuda"), torch.randn(32, 64, device="cuda")
+    y, want = torch.empty(1, 32, device="cuda"), torch.empty(1, 32, device="cuda")
+    xb.linear_device(0, 1, 1, 64, 32, ptr(x), ptr(w), ptr(want), stream=stream())
+    xb.linear_device(0, 1, 1, 64, 32, ptr(x), ptr(w), ptr(y), ldx=1, ldy=5, stream=stream())
+    assert torch.equal(y, want)
 
 
 @pytest.mark.parametrize("pad,skew", LAYOUTS)
@@ -268,6 +310,25 @@ def test_float32_range(xb, kind):
     # fp16 weights near 2^-10 lie within the normal range but for a few subnormals, exact either way.
     want = x.double() @ w.double().t()
     close(y, want, sum_error(x.double(), w.double(), want), "y")
+
+
+@pytest.mark.parametrize("n", [4, 300])
+def test_float32_near_the_ends_of_its_range(xb, n):
+    """Three bfloat16 parts hold a float32 exactly down to bfloat16's smallest step: each element is off
+    by at most 2^-134.  Next to the largest float32 the first part must not round to an infinity."""
+    k, m = 64, 48
+    mk = Maker("fp32", 12)
+    small, w = mk.matrix(n, k, 2.0 ** -126).contiguous(), mk.matrix(m, k, 2.0 ** 100).contiguous()
+    y = torch.empty(n, m, device="cuda")
+    xb.linear_device(0, 1, n, k, m, ptr(small), ptr(w), ptr(y), stream=stream())
+    x64, w64 = small.double(), w.double()
+    want = x64 @ w64.t()
+    close(y, want, sum_error(x64, w64, want) + 2.0 ** -134 * w64.abs().sum(1), "y")
+    big = torch.full((n, 1), torch.finfo(torch.float32).max, device="cuda")
+    one = torch.ones(1, 1, device="cuda")
+    y = torch.empty(n, 1, device="cuda")
+    xb.linear_device(0, 1, n, 1, 1, ptr(big), ptr(one), ptr(y), stream=stream())
+    assert bool((y == big).all())
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
@@ -469,6 +530,94 @@ def test_captured_and_replayed(xb):
             for name in outs:
                 assert torch.equal(s[name], new[name]), name
     graphs.clear()
+
+
+FRESH = """
+import sys, torch
+sys.path[:0] = [{root!r}]
+import xvec_b200 as xb
+n, k, m = {n}, 96, 128
+x, w = torch.randn(n, k, device="cuda"), torch.randn(m, k, device="cuda")
+y, dw, db = torch.empty(n, m, device="cuda"), torch.empty(m, k, device="cuda"), torch.empty(m, device="cuda")
+norm = torch.empty((), device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    s = torch.cuda.current_stream().cuda_stream
+    xb.linear_device(0, 1, n, k, m, x.data_ptr(), w.data_ptr(), y.data_ptr(), stream=s)
+    xb.linear_backward_device(0, 1, n, k, m, y.data_ptr(), x.data_ptr(), w.data_ptr(), dw_ptr=dw.data_ptr(),
+                              db_ptr=db.data_ptr(), stream=s)
+    xb.clip_gradients_device(0, [(1, dw.data_ptr(), dw.data_ptr(), dw.numel())], 1.0, norm.data_ptr(),
+                             stream=s)
+graph.replay()
+torch.cuda.synchronize()
+want = x.double() @ w.double().t()
+assert ((y.double() - want).norm() / want.norm()).item() < 1e-6
+g = want.t() @ x.double()
+assert abs(norm.item() / g.norm().item() - 1) < 1e-5
+assert abs(dw.double().norm().item() - 1) < 1e-5
+del graph
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("n", [3, 1000])
+def test_first_call_of_a_process_inside_a_capture(n):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", FRESH.format(root=root, n=n)], capture_output=True,
+                       text=True, timeout=300)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stderr[-2000:]
+
+
+def test_two_threads_at_once(xb):
+    """Calls of two host threads, each on its own stream and buffers."""
+    import threading
+    want = {c: CALLS[c](xb, "fp32") for c in CALLS}
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(call):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got = CALLS[call](xb, "fp32")
+                torch.cuda.current_stream().synchronize()
+            bad.extend(call for p, q in zip(got, want[call]) if not torch.equal(p, q))
+        except Exception as e:  # reported by the main thread
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in CALLS]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
+def test_queries_through_two_layers_without_waiting(xb):
+    """Calls that follow one another on a stream read what the one before wrote (their launches
+    overlap at the edges), also through the same buffers again and again."""
+    k = 256
+    mk = Maker("fp16", 11)
+    ws = [mk.matrix(k, k, k ** -0.5).contiguous() for _ in range(4)]
+    for n in (1, 6, 200, 3000):
+        x0 = mk.matrix(n, k).contiguous()
+        a, b = x0.clone(), torch.empty_like(x0)
+        for i in range(40):
+            xb.linear_device(0, 2, n, k, k, ptr(a), ptr(ws[i % 4]), ptr(b), activation=xb.ACT_SILU,
+                             residual_ptr=ptr(x0), stream=stream())
+            a, b = b, a
+        got = a.clone()
+        a, b = x0.clone(), torch.empty_like(x0)
+        for i in range(40):
+            xb.linear_device(0, 2, n, k, k, ptr(a), ptr(ws[i % 4]), ptr(b), activation=xb.ACT_SILU,
+                             residual_ptr=ptr(x0), stream=stream())
+            torch.cuda.synchronize()
+            a, b = b, a
+        assert torch.equal(a, got)
 
 
 def test_gradients_against_differences(xb):

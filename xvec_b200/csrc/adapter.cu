@@ -379,9 +379,10 @@ struct Check {
   xvec_gpu_status st = XVEC_GPU_OK;
   explicit Check(size_t size) : size(size) {}
 
-  void ld(const char* name, const void* p, int64_t cols, int64_t* ld) {
+  // (The leading dimension of a single row means nothing.)
+  void ld(const char* name, const void* p, int64_t rows, int64_t cols, int64_t* ld) {
     if (st || !p) return;
-    if (*ld == 0) *ld = cols;
+    if (*ld == 0 || rows <= 1) *ld = cols;
     if (*ld < cols) {
       set_error("adapter: leading dimension %lld of %s is less than its %lld columns",
                 (long long)*ld, name, (long long)cols);
@@ -439,6 +440,7 @@ xvec_gpu_status check_shape(const Args* a) {
     return invalid("dimensions must be in [1, 1048576]");
   if (a->n < 0 || a->n > INT_MAX - 1024) return invalid("row count must be in [0, 2^31 - 1025]");
   if (a->reserved != 0) return invalid("reserved must be 0");
+  if ((uintptr_t)a->status % 4) return invalid("status is not aligned");
   return XVEC_GPU_OK;
 }
 
@@ -496,9 +498,17 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
   return XVEC_GPU_OK;
 }
 
+DeviceGuard::~DeviceGuard() {
+  if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+  if (before >= 0) cudaSetDevice(before);
+}
+
 xvec_gpu_status DeviceGuard::set(int device) {
+  static std::atomic<bool> ready[kMaxDevices];
+  const bool known =
+      device >= 0 && device < kMaxDevices && ready[device].load(std::memory_order_acquire);
   int count = 0;
-  if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
+  if (!known && (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count)) {
     cudaGetLastError();
     set_error("CUDA device %d is not available", device);
     return XVEC_GPU_UNSUPPORTED;
@@ -509,8 +519,9 @@ xvec_gpu_status DeviceGuard::set(int device) {
     XVEC_CUDA(cudaSetDevice(device));
     before = now;
   }
-  static std::atomic<bool> ready[kMaxDevices];
-  if (device < kMaxDevices && ready[device].load(std::memory_order_acquire)) return XVEC_GPU_OK;
+  XVEC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  relaxed = true;
+  if (known) return XVEC_GPU_OK;
   int major = 0, minor = 0;
   XVEC_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
   XVEC_CUDA(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
@@ -518,16 +529,11 @@ xvec_gpu_status DeviceGuard::set(int device) {
     set_error("device %d is not an sm_100 (B200) device", device);
     return XVEC_GPU_UNSUPPORTED;
   }
-  // Keep freed stream-ordered scratch in the pool between calls (a setting
-  // that a stream capture in progress would otherwise refuse).
+  // Keep freed stream-ordered scratch in the pool between calls.
   cudaMemPool_t pool;
   XVEC_CUDA(cudaDeviceGetDefaultMemPool(&pool, device));
   uint64_t threshold = UINT64_MAX;
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  XVEC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-  const cudaError_t set = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold);
-  XVEC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-  XVEC_CUDA(set);
+  XVEC_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold));
   if (device < kMaxDevices) ready[device].store(true, std::memory_order_release);
   return XVEC_GPU_OK;
 }
@@ -544,11 +550,11 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   xvec_gpu_linear_args a = *args;
   if (!a.weight || (a.n && (!a.x || !a.y))) return invalid("x, weight and y are required");
   Check c(elem_bytes(a.storage));
-  c.ld("x", a.x, a.in_dim, &a.ldx);
-  c.ld("weight", a.weight, a.in_dim, &a.ldw);
-  c.ld("residual", a.residual, a.out_dim, &a.ldr);
-  c.ld("y", a.y, a.out_dim, &a.ldy);
-  c.ld("preact", a.preact, a.out_dim, &a.ldz);
+  c.ld("x", a.x, a.n, a.in_dim, &a.ldx);
+  c.ld("weight", a.weight, a.out_dim, a.in_dim, &a.ldw);
+  c.ld("residual", a.residual, a.n, a.out_dim, &a.ldr);
+  c.ld("y", a.y, a.n, a.out_dim, &a.ldy);
+  c.ld("preact", a.preact, a.n, a.out_dim, &a.ldz);
   c.in("x", a.x, a.n, a.in_dim, a.ldx);
   c.in("weight", a.weight, a.out_dim, a.in_dim, a.ldw);
   c.in("bias", a.bias, 1, a.out_dim, a.out_dim);
@@ -597,10 +603,10 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
     return invalid("x, gate_weight, up_weight and h are required");
   if (!a.gate != !a.up) return invalid("gate and up are given together or not at all");
   Check c(elem_bytes(a.storage));
-  c.ld("x", a.x, a.in_dim, &a.ldx);
-  c.ld("the weights", a.gate_weight, a.in_dim, &a.ldw);
-  c.ld("h", a.h, a.out_dim, &a.ldh);
-  c.ld("gate and up", a.gate, a.out_dim, &a.ldg);
+  c.ld("x", a.x, a.n, a.in_dim, &a.ldx);
+  c.ld("the weights", a.gate_weight, a.out_dim, a.in_dim, &a.ldw);
+  c.ld("h", a.h, a.n, a.out_dim, &a.ldh);
+  c.ld("gate and up", a.gate, a.n, a.out_dim, &a.ldg);
   c.in("x", a.x, a.n, a.in_dim, a.ldx);
   c.in("gate_weight", a.gate_weight, a.out_dim, a.in_dim, a.ldw);
   c.in("up_weight", a.up_weight, a.out_dim, a.in_dim, a.ldw);
@@ -772,12 +778,12 @@ extern "C" xvec_gpu_status xvec_gpu_linear_backward_device(
   if (a.n && a.dweight && !a.x) return invalid("dweight needs x");
   if (a.n && a.activation != XVEC_ACT_NONE && !a.preact) return invalid("the activation needs preact");
   Check c(elem_bytes(a.storage));
-  c.ld("dy", a.dy, a.out_dim, &a.lddy);
-  c.ld("x", a.x, a.in_dim, &a.ldx);
-  c.ld("weight", a.weight, a.in_dim, &a.ldw);
-  c.ld("preact", a.preact, a.out_dim, &a.ldz);
-  c.ld("dx", a.dx, a.in_dim, &a.lddx);
-  c.ld("dweight", a.dweight, a.in_dim, &a.lddw);
+  c.ld("dy", a.dy, a.n, a.out_dim, &a.lddy);
+  c.ld("x", a.x, a.n, a.in_dim, &a.ldx);
+  c.ld("weight", a.weight, a.out_dim, a.in_dim, &a.ldw);
+  c.ld("preact", a.preact, a.n, a.out_dim, &a.ldz);
+  c.ld("dx", a.dx, a.n, a.in_dim, &a.lddx);
+  c.ld("dweight", a.dweight, a.out_dim, a.in_dim, &a.lddw);
   c.in("dy", a.dy, a.n, a.out_dim, a.lddy);
   c.in("x", a.x, a.n, a.in_dim, a.ldx);
   c.in("weight", a.weight, a.out_dim, a.in_dim, a.ldw);
@@ -807,12 +813,13 @@ extern "C" xvec_gpu_status xvec_gpu_gated_backward_device(
   if (a.dx && (!a.gate_weight || !a.up_weight)) return invalid("dx needs both weights");
   if (a.n && (a.dgate_weight || a.dup_weight) && !a.x) return invalid("weight gradients need x");
   Check c(elem_bytes(a.storage));
-  c.ld("dh", a.dh, a.out_dim, &a.lddh);
-  c.ld("x", a.x, a.in_dim, &a.ldx);
-  c.ld("the weights", a.gate_weight ? a.gate_weight : a.up_weight, a.in_dim, &a.ldw);
-  c.ld("gate and up", a.gate, a.out_dim, &a.ldg);
-  c.ld("dx", a.dx, a.in_dim, &a.lddx);
-  c.ld("the weight gradients", a.dgate_weight ? a.dgate_weight : a.dup_weight, a.in_dim, &a.lddw);
+  c.ld("dh", a.dh, a.n, a.out_dim, &a.lddh);
+  c.ld("x", a.x, a.n, a.in_dim, &a.ldx);
+  c.ld("the weights", a.gate_weight ? a.gate_weight : a.up_weight, a.out_dim, a.in_dim, &a.ldw);
+  c.ld("gate and up", a.gate, a.n, a.out_dim, &a.ldg);
+  c.ld("dx", a.dx, a.n, a.in_dim, &a.lddx);
+  c.ld("the weight gradients", a.dgate_weight ? a.dgate_weight : a.dup_weight, a.out_dim,
+       a.in_dim, &a.lddw);
   c.in("dh", a.dh, a.n, a.out_dim, a.lddh);
   c.in("x", a.x, a.n, a.in_dim, a.ldx);
   c.in("gate_weight", a.gate_weight, a.out_dim, a.in_dim, a.ldw);

@@ -188,12 +188,14 @@ cudaError_t launch_pdl(void (*kern)(Params...), dim3 grid, int block, size_t sme
   return e;
 }
 
-// Makes `device` current for one call and restores the caller's.
+// Makes `device` current for one call and restores the caller's.  Meanwhile a
+// stream capture of another thread does not forbid the one-time settings and the
+// loading of kernels (none of them belongs into a graph).
 struct DeviceGuard {
   int before = -1;
-  ~DeviceGuard() {
-    if (before >= 0) cudaSetDevice(before);
-  }
+  bool relaxed = false;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  ~DeviceGuard();
   xvec_gpu_status set(int device);
 };
 
