@@ -465,7 +465,7 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
   XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
   GemmParams& p = c->p;
   p.blocks = (int)((c->depth + 63) / 64);
-  p.ldp = (p.cols + 31) / 32 * 32;
+  p.ldp = (p.cols + 63) / 64 * 64;  // whole steps of the epilogue
   const int all = p.blocks * p.segs;
   const int half = c->mode == kGated ? 2 : 1;  // accumulator columns per output column
   const int matrices = 1 + (p.save[0] != nullptr) + (p.save[1] != nullptr) +
@@ -592,6 +592,7 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   const size_t size = elem_bytes(a.storage);
   p.vec = aligned16(a.y, a.ldy, size) && aligned16(a.residual, a.ldr, size) &&
           aligned16(a.preact, a.ldz, size);
+  p.bias_vec = aligned16(a.bias, 0, size);
   return forward(a.storage, g, &x, &w, nullptr, arena, s);
 }
 
@@ -646,6 +647,7 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   const size_t size = elem_bytes(a.storage);
   p.vec = aligned16(a.h, a.ldh, size) && aligned16(a.gate, a.ldg, size) &&
           aligned16(a.up, a.ldg, size);
+  p.bias_vec = aligned16(a.gate_bias, 0, size) && aligned16(a.up_bias, 0, size);
   return forward(a.storage, g, &x, &wg, &wu, arena, s);
 }
 

@@ -218,6 +218,7 @@ struct GemmParams {
   int64_t ldp;
   uint32_t idesc;
   int vec;               // outputs, saves and residual allow 16-byte accesses
+  int bias_vec;          // and the biases
   const void* bias[2];
   const void* residual;
   void* out[2];

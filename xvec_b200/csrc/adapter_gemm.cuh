@@ -58,7 +58,7 @@ constexpr int kBand = 8;      // row tiles per band of the tile order
 constexpr int kFewRegs = 56, kManyRegs = 224;
 constexpr int kRound = 2;     // float32: depth blocks per accumulation in tensor memory
 
-template <typename T, bool PAIR, int BN>
+template <int MODE, typename T, bool PAIR, int BN>
 struct GemmShape {
   // Two epilogue warps per TMEM lane quarter, one per half of the columns.  (Four
   // on 256 columns cost a stage of the ring and were slower: 131072 x 1024 -> 1024
@@ -73,8 +73,12 @@ struct GemmShape {
   static constexpr int kUnits = std::is_same<T, float>::value ? 1 : 2;
   static constexpr uint32_t kBlockBytes = kABytes + kBBytes;
   static constexpr uint32_t kStageBytes = kUnits * kBlockBytes;
-  // Per epilogue warp: a bias per column and a 32 x 64 byte staging block.
-  static constexpr uint32_t kEpiBytes = kEpiWarps * (BN / 2 * 4 + 2048);
+  // Columns that an epilogue warp finishes at a time, and their staging block of 32
+  // rows: 128 bytes a row where its columns come in 64s (or 32 float32), else 64.
+  static constexpr int kOutCols = BN / 2 / (MODE == kGated ? 2 : 1);  // outputs of a warp
+  static constexpr int kStep = sizeof(T) == 2 && kOutCols % 64 == 0 ? 64 : 32;
+  static constexpr int kRowBytes = kStep * sizeof(T);
+  static constexpr uint32_t kEpiBytes = kEpiWarps * 32 * kRowBytes;
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + 512;
@@ -185,13 +189,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
 }
 
 // --- epilogue input and output ------------------------------------------------------
-// A warp holds 32 x 32 values, one row per lane.  They reach memory (and a
-// residual comes from it) through a staging block of 32 rows of 64 bytes, so
-// that each instruction covers whole 64-byte row segments: 4 lanes of 16 bytes
-// per row.  The 16-byte parts of row r are permuted by (r / 2) mod 4, which
+// A warp holds 32 rows of values, one row per lane.  They reach memory (and a
+// residual comes from it) through a staging block of 32 rows of RB bytes, so that
+// each instruction covers whole row segments of RB bytes: RB / 16 lanes of 16
+// bytes per row.  The 16-byte parts of a row are permuted by its number, which
 // keeps both directions free of bank conflicts.
+template <int RB>
 __device__ __forceinline__ uint32_t stage_at(uint32_t buf, int row, int part) {
-  return buf + row * 64 + ((part ^ ((row >> 1) & 3)) << 4);
+  return buf + row * RB + ((part ^ (RB == 128 ? row & 7 : (row >> 1) & 3)) << 4);
 }
 __device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z),
@@ -213,115 +218,138 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
     u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
                    __float_as_uint(v[3]));
   } else {
-    uint32_t* t = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+    u = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
+                   pack2<T>(v[6], v[7]));
   }
   return u;
 }
 
 // Writes v (this lane's row) to base[row * ld + column], rows and cols of it.
-template <typename T>
+template <typename T, int RB, int N>
 __device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows, int cols, bool vec,
-                                     const float (&v)[32], int lane) {
-  constexpr int kCols = 64 / sizeof(T), kPart = 16 / sizeof(T);  // columns per block and part
+                                     const float (&v)[N], int lane) {
+  constexpr int kParts = RB / 16, kPart = 16 / sizeof(T), kCols = RB / sizeof(T);
+  static_assert(N % kCols == 0, "whole staging rows");
 #pragma unroll
-  for (int h = 0; h < 32 / kCols; ++h) {
+  for (int h = 0; h < N / kCols; ++h) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) sts16(stage_at(buf, lane, c), pack16<T>(v + h * kCols + c * kPart));
+    for (int c = 0; c < kParts; ++c)
+      sts16(stage_at<RB>(buf, lane, c), pack16<T>(v + h * kCols + c * kPart));
     __syncwarp();
     T* out = base + h * kCols;
     const int left = cols - h * kCols;
     if (vec && left >= kCols) {
-      const int part = lane & 3;
+      const int part = lane % kParts, row = lane / kParts;
+      uint4 u[kParts];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        if (r < rows)
-          *reinterpret_cast<uint4*>(out + r * ld + part * kPart) = lds16(stage_at(buf, r, part));
+      for (int i = 0; i < kParts; ++i) u[i] = lds16(stage_at<RB>(buf, i * (32 / kParts) + row, part));
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const int r = i * (32 / kParts) + row;
+        if (r < rows) *reinterpret_cast<uint4*>(out + r * ld + part * kPart) = u[i];
       }
     } else {
-      const int col = lane % kCols;
-      for (int r = lane / kCols; r < rows; r += 32 / kCols)
+      // A column a lane, a row after the other.
+#pragma unroll
+      for (int c0 = 0; c0 < kCols; c0 += 32) {
+        const int col = c0 + lane;
         if (col < left) {
-          const uint32_t a = stage_at(buf, r, col / kPart) + (col % kPart) * sizeof(T);
-          if constexpr (sizeof(T) == 4) {
-            float f;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
-            out[r * ld + col] = f;
-          } else {
-            uint16_t b;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(a) : "memory");
-            reinterpret_cast<uint16_t*>(out)[r * ld + col] = b;
+#pragma unroll 8
+          for (int r = 0; r < rows; ++r) {
+            const uint32_t a = stage_at<RB>(buf, r, col / kPart) + (col % kPart) * sizeof(T);
+            if constexpr (sizeof(T) == 4) {
+              float f;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+              out[r * ld + col] = f;
+            } else {
+              uint16_t b;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(a) : "memory");
+              reinterpret_cast<uint16_t*>(out)[r * ld + col] = b;
+            }
           }
         }
+      }
     }
     __syncwarp();
   }
 }
 
-// A 32 x 32 block on its way in: requested early (start), added to this lane's
-// row later (add).  Rows or columns that do not exist are not read.
-template <typename T>
+// A block of 32 rows on its way in: requested early (start), added to this
+// lane's row later (add).  Rows or columns that do not exist are not read.
+template <typename T, int RB>
 struct Incoming {
-  static constexpr int kParts = 32 * sizeof(T) / 16;  // 16-byte parts of a row
+  static constexpr int kParts = RB / 16, N = RB / sizeof(T);
   uint4 v[kParts];
 
   __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, bool whole, int lane) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const int r = (i & 3) * 8 + (lane >> 2);
+      const int r = i * (32 / kParts) + lane / kParts;
       v[i] = make_uint4(0, 0, 0, 0);
       if (whole && r < rows)
-        v[i] = *reinterpret_cast<const uint4*>(base + r * ld + (i >> 2) * (64 / sizeof(T)) +
-                                               (lane & 3) * (16 / sizeof(T)));
+        v[i] = *reinterpret_cast<const uint4*>(base + r * ld + (lane % kParts) * (16 / sizeof(T)));
     }
   }
   __device__ __forceinline__ void add(uint32_t buf, const T* base, int64_t ld, int rows, int cols,
-                                      bool whole, float (&f)[32], int lane) {
+                                      bool whole, float (&f)[N], int lane) {
     if (whole) {
 #pragma unroll
-      for (int h = 0; h < kParts / 4; ++h) {
+      for (int i = 0; i < kParts; ++i)
+        sts16(stage_at<RB>(buf, i * (32 / kParts) + lane / kParts, lane % kParts), v[i]);
+      __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sts16(stage_at(buf, i * 8 + (lane >> 2), lane & 3), v[h * 4 + i]);
-        __syncwarp();
+      for (int c = 0; c < kParts; ++c) {
+        const uint4 u = lds16(stage_at<RB>(buf, lane, c));
+        const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint4 u = lds16(stage_at(buf, lane, c));
-          const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-          for (int j = 0; j < 16 / (int)sizeof(T); ++j)
-            f[h * (64 / sizeof(T)) + c * (16 / sizeof(T)) + j] += to_f(t[j]);
-        }
-        __syncwarp();
+        for (int j = 0; j < 16 / (int)sizeof(T); ++j) f[c * (16 / sizeof(T)) + j] += to_f(t[j]);
       }
+      __syncwarp();
     } else if (lane < rows) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < N; ++j)
         if (j < cols) f[j] += to_f(base[lane * ld + j]);
     }
   }
 };
 
+// x += the biases of its columns, `cols` of which exist (the same for all lanes).
+template <typename T, int N>
+__device__ __forceinline__ void add_bias(const T* bias, int cols, bool vec, float (&x)[N]) {
+  if (!bias) return;
+  if (vec && cols >= N) {
+#pragma unroll
+    for (int c = 0; c < N * (int)sizeof(T) / 16; ++c) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(bias) + c);
+      const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[c * (16 / sizeof(T)) + j] += to_f(t[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < cols) x[j] += to_f(bias[j]);
+  }
+}
+
 // --- the kernel ---------------------------------------------------------------
 template <int MODE, typename T, bool PAIR, int BN>
-__global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
+__global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap0,
                 const __grid_constant__ CUtensorMap bmap1, const __grid_constant__ GemmParams p) {
   using namespace tc;
-  using S = GemmShape<T, PAIR, BN>;
+  using S = GemmShape<MODE, T, PAIR, BN>;
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   constexpr int P = std::is_same<T, float>::value ? 3 : 1;  // planes
   constexpr int kStages = S::kStages, kEpiWarps = S::kEpiWarps;
   constexpr int kTileRows = PAIR ? 256 : 128;
   constexpr int kTileCols = MODE == kGated ? BN / 2 : BN;
   constexpr int kWarpCols = BN / 2;  // accumulator columns per epilogue warp
+  constexpr int kOutCols = S::kOutCols, kStep = S::kStep, RB = S::kRowBytes;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* staging = tiles + kStages * S::kStageBytes;
-  float* bias_all = reinterpret_cast<float*>(staging + kEpiWarps * 2048);
-  uint64_t* full = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * kWarpCols);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + S::kEpiBytes);
   uint64_t* empty = full + kStages;   // the MMAs have read the stage
   uint64_t* tfull = empty + kStages;  // [2] accumulator ready (float32: hh, small)
   uint64_t* tempty = tfull + 2;       // [2] accumulator drained (issuing CTA's count)
@@ -544,8 +572,7 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
     // ---------------- epilogue ----------------
     if constexpr (P == 3) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
     const int quarter = warp & 3, ew = warp - 4, group = ew >> 2;
-    float* bias_s = bias_all + ew * kWarpCols;
-    const uint32_t buf = smem_u32(staging + ew * 2048);
+    const uint32_t buf = smem_u32(staging + ew * 32 * RB);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tfull_at = smem_u32(tfull);
     const bool vec = p.vec != 0;
@@ -568,15 +595,12 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
         else mbar_arrive(&tempty[acc]);
       }
     };
-    // Accumulator column of chunk c: plain modes take the warp's half from left
-    // to right; the gated mode alternates gate and up of the same outputs.
-    constexpr int kChunks = kWarpCols / 32;
-    constexpr int kOutCols = MODE == kGated ? kWarpCols / 2 : kWarpCols;  // output columns
-    auto acc_col = [&](int c) {
-      return MODE == kGated ? (c & 1) * (BN / 2) + group * kOutCols + (c >> 1) * 32
-                            : group * kWarpCols + c * 32;
+    // Accumulator column of output column c of the warp (which: the gate's or the
+    // up's sums).
+    auto acc_col = [&](int which, int c) {
+      return which * (BN / 2) + group * kOutCols + c;
     };
-    constexpr int kStep = MODE == kGated ? 2 : 1;
+    using Step = float[S::kStep];
     uint32_t round = 0, tile = 0;
     for (int i = worker; i < items; i += workers, ++tile) {
       const Item it = item_of(i);
@@ -587,96 +611,87 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
       const T* res = MODE == kLinear && p.splits == 1 && p.residual
                          ? static_cast<const T*>(p.residual) + row0 * p.ldr + warp_col
                          : nullptr;
-      Incoming<T> in;
+      Incoming<T, RB> in;
       // (float32 has no registers for it while it drains.)
-      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, vec && cols >= 32, lane);
-      if constexpr (MODE == kLinear || MODE == kGated) {
-        // The warp's biases: its columns' in order (gated: gate, then up).
-        __syncwarp();
-        for (int c = lane; c < kOutCols; c += 32) {
-          const bool has = c < cols;
-          bias_s[c] = has && p.bias[0] ? to_f(static_cast<const T*>(p.bias[0])[warp_col + c]) : 0.f;
-          if constexpr (MODE == kGated)
-            bias_s[kOutCols + c] =
-                has && p.bias[1] ? to_f(static_cast<const T*>(p.bias[1])[warp_col + c]) : 0.f;
-        }
-        __syncwarp();
-      }
-      // Finishes 32 columns: v the sums (gated: the gate's; up() then gives the
-      // up's, late, so that both are not held at once).
-      auto finish = [&](int c, float (&v)[32], auto&& up) {
-        const int at = (MODE == kGated ? c >> 1 : c) * 32;
-        const int n = (int)min((int64_t)32, cols - at);
+      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, vec && cols >= kStep, lane);
+      // Finishes kStep columns from `at` on: v the sums (gated: the gate's; up() then
+      // gives the up's, late, so that both are not held longer than needed).
+      auto finish = [&](int at, Step& v, auto&& up) {
+        const int n = (int)min((int64_t)kStep, cols - at);
         const int64_t col = warp_col + at;
         if (p.splits > 1) {
           constexpr int kPlanes = MODE == kGated ? 2 : 1;
           float* dst = p.partial +
                        ((int64_t)(it.split * p.batches + it.batch) * kPlanes * p.rows + row0) *
                            p.ldp + col;
-          if (n > 0) emit(buf, dst, p.ldp, rows, 32, true, v, lane);
+          // (ldp covers whole steps.)
+          if (n > 0) emit<float, RB>(buf, dst, p.ldp, rows, kStep, true, v, lane);
           if constexpr (MODE == kGated) {
             up(v);
-            if (n > 0) emit(buf, dst + p.rows * p.ldp, p.ldp, rows, 32, true, v, lane);
+            if (n > 0)
+              emit<float, RB>(buf, dst + p.rows * p.ldp, p.ldp, rows, kStep, true, v, lane);
           }
           return;
         }
         // Bias and the saved pre-activation of the first or second sums.
-        auto affine = [&](int which, float (&x)[32]) {
-          const float4* b = reinterpret_cast<const float4*>(bias_s + which * kOutCols + at);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 t = b[j];
-            x[4 * j] += t.x, x[4 * j + 1] += t.y, x[4 * j + 2] += t.z, x[4 * j + 3] += t.w;
-          }
+        auto affine = [&](int which, Step& x) {
+          const T* b = static_cast<const T*>(p.bias[which]);
+          add_bias(b ? b + col : b, n, p.bias_vec != 0, x);
           if (p.save[which] && n > 0)
-            emit(buf, static_cast<T*>(p.save[which]) + row0 * p.lds + col, p.lds, rows, n, vec, x,
-                 lane);
+            emit<T, RB>(buf, static_cast<T*>(p.save[which]) + row0 * p.lds + col, p.lds, rows, n,
+                        vec, x, lane);
         };
-        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, vec && n == 32, lane);
+        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, vec && n == kStep, lane);
         if constexpr (MODE == kLinear || MODE == kGated) {
           affine(0, v);
           activate_all<T>(p.act, v);
         }
         if constexpr (MODE == kGated) {
-          float u[32];
+          Step u;
           up(u);
           affine(1, u);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= u[j];
+          for (int j = 0; j < kStep; ++j) v[j] *= u[j];
         }
         if (MODE == kLinear && res && n > 0) {
-          in.add(buf, res + at, p.ldr, rows, n, vec && n == 32, v, lane);
-          if (P == 1 && c + 1 < kChunks) in.start(res + at + 32, p.ldr, rows, vec && cols >= at + 64, lane);
+          in.add(buf, res + at, p.ldr, rows, n, vec && n == kStep, v, lane);
+          if (P == 1 && at + kStep < kOutCols)
+            in.start(res + at + kStep, p.ldr, rows, vec && cols >= at + 2 * kStep, lane);
         }
         if (n > 0)
-          emit(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col, p.ldo,
-               rows, n, vec, v, lane);
+          emit<T, RB>(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col,
+                      p.ldo, rows, n, vec, v, lane);
       };
       if constexpr (P == 1) {
         const uint32_t acc = tile & 1, t = tmem_base + acc * BN + lanes;
         if (!wait_acc(acc, (tile >> 1) & 1)) break;
-#pragma unroll 1
-        for (int c = 0; c < kChunks; c += kStep) {
-          // One accumulator chunk; the last one frees the accumulator.
-          auto chunk = [&](int c, float (&v)[32]) {
-            uint32_t raw[32];
-            tmem_ld32(t + acc_col(c), raw);
-            tmem_wait_ld();
-            if (c == kChunks - 1) release_acc(acc);
+        // kStep sums; the accumulator is freed with its last ones.
+        auto take = [&](int which, int at, Step& v) {
+          uint32_t raw[kStep / 32][32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
-          };
-          float v[32];
-          chunk(c, v);
-          finish(c, v, [&](float (&u)[32]) { chunk(c + 1, u); });
+          for (int c = 0; c < kStep / 32; ++c) tmem_ld32(t + acc_col(which, at + c * 32), raw[c]);
+          tmem_wait_ld();
+          if (which == (MODE == kGated ? 1 : 0) && at + kStep == kOutCols) release_acc(acc);
+#pragma unroll
+          for (int c = 0; c < kStep / 32; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[c * 32 + j] = __uint_as_float(raw[c][j]);
+        };
+#pragma unroll 1
+        for (int at = 0; at < kOutCols; at += kStep) {
+          Step v;
+          take(0, at, v);
+          finish(at, v, [&](Step& u) { take(1, at, u); });
         }
       } else {
-        float sum[kChunks][32];
+        // 32 sums at a time: the output columns' (gated: a gate's 32, then the up's).
+        constexpr int kSums = kWarpCols / 32, kPer = MODE == kGated ? 2 : 1;
+        float sum[kSums][32];
         auto drain = [&](uint32_t t, bool first) {
 #pragma unroll
-          for (int c = 0; c < 2 * kChunks; ++c) {
+          for (int c = 0; c < 2 * kSums; ++c) {
             uint32_t raw[16];
-            tmem_ld16(t + lanes + acc_col(c >> 1) + (c & 1) * 16, raw);
+            tmem_ld16(t + lanes + acc_col((c >> 1) % kPer, (c >> 1) / kPer * 32) + (c & 1) * 16, raw);
             tmem_wait_ld();
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -696,18 +711,18 @@ __global__ void __launch_bounds__(GemmShape<T, PAIR, BN>::kThreads, 1)
           release_acc(1);
         }
         if (!ok) break;
-        // A rolled loop over chunks that always takes the first sums and moves the
+        // A rolled loop over steps that always takes the first sums and moves the
         // others up: unrolled, its addresses alone made the sums spill.
 #pragma unroll 1
-        for (int c = 0; c < kChunks; c += kStep) {
-          finish(c, sum[0], [&](float (&u)[32]) {
+        for (int at = 0; at < kOutCols; at += kStep) {
+          finish(at, sum[0], [&](Step& u) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] = sum[kStep - 1][j];
+            for (int j = 0; j < 32; ++j) u[j] = sum[kPer - 1][j];
           });
 #pragma unroll
-          for (int i = 0; i + kStep < kChunks; ++i)
+          for (int i = 0; i + kPer < kSums; ++i)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[i][j] = sum[i + kStep][j];
+            for (int j = 0; j < 32; ++j) sum[i][j] = sum[i + kPer][j];
         }
       }
     }
@@ -820,7 +835,7 @@ inline bool operand_map(CUtensorMap* map, const GemmOperand& o, int box_outer) {
 template <int MODE, typename T, bool PAIR, int BN>
 xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
   GemmParams p = c.p;
-  using S = GemmShape<T, PAIR, BN>;
+  using S = GemmShape<MODE, T, PAIR, BN>;
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   CUtensorMap a, b0, b1;
   const int b_box = B_MN ? kBK : (MODE == kGated && !PAIR) ? S::kBRows / 2 : S::kBRows;
