@@ -460,9 +460,8 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
   const double products = storage == XVEC_STORAGE_FP32 ? 6 : 1;
   const double block[kShapes] = {512 * products, 448 * products, 384 * products, 590 * products};
   const double start[kShapes] = {7500, 7500, 7500, 3000};
-  int device = 0, sms = 0;
-  XVEC_CUDA(cudaGetDevice(&device));
-  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  XVEC_CUDA(cudaGetDevice(&c->device));
+  if (xvec_gpu_status st = count_sms(c->device, &c->sms)) return st;
   GemmParams& p = c->p;
   p.blocks = (int)((c->depth + 63) / 64);
   p.ldp = (p.cols + 63) / 64 * 64;  // whole steps of the epilogue
@@ -475,11 +474,11 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
   for (int k = 0; k < kShapes; ++k) {
     if (k == 1 && c->mode != kLinear) continue;
     const int rows = kTileShapes[k].rows, cols = kTileShapes[k].cols / half;
-    const int workers = kTileShapes[k].pair ? sms / 2 : sms;
+    const int workers = kTileShapes[k].pair ? c->sms / 2 : c->sms;
     const int64_t tm = (p.rows + rows - 1) / rows, tn = (p.cols + cols - 1) / cols;
     for (int splits = 1; splits <= 32; ++splits) {
       const int per = (all + splits - 1) / splits;
-      if (splits > 1 && (per < 4 || (int64_t)per * (splits - 1) >= all)) continue;
+      if (splits > 1 && (per * products < 4 || (int64_t)per * (splits - 1) >= all)) continue;
       const double waves = (double)((tm * tn * p.batches * splits + workers - 1) / workers);
       const double epilogue =
           cols * (splits > 1 ? 25.0 * half : matrices * (p.vec ? 10.0 : 25.0));
@@ -495,6 +494,15 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
   }
   c->partial_bytes =
       p.splits > 1 ? (size_t)p.splits * p.batches * half * p.rows * p.ldp * 4 : 0;
+  return XVEC_GPU_OK;
+}
+
+xvec_gpu_status count_sms(int device, int* sms) {
+  static std::atomic<int> known[kMaxDevices];
+  if (device < kMaxDevices && (*sms = known[device].load(std::memory_order_relaxed)))
+    return XVEC_GPU_OK;
+  XVEC_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+  if (device < kMaxDevices) known[device].store(*sms, std::memory_order_relaxed);
   return XVEC_GPU_OK;
 }
 

@@ -248,6 +248,7 @@ struct GemmCall {
   int64_t depth = 0;
   GemmOperand a, b[2];
   GemmParams p{};
+  int device = 0, sms = 0;    // (plan_gemm)
   int shape = 0;              // of the tiles (plan_gemm)
   size_t partial_bytes = 0;   // scratch for split sums, at p.partial
 };
@@ -260,6 +261,8 @@ constexpr TileShape kTileShapes[kShapes] = {
     {256, 256, true}, {256, 192, true}, {256, 128, true}, {128, 128, false}};
 // Picks the tiles and splits: fills in c's tiling and partial_bytes.
 xvec_gpu_status plan_gemm(int storage, GemmCall* c);
+// The number of SMs of a device.
+xvec_gpu_status count_sms(int device, int* sms);
 // By the storage type of the outputs; float32: operands are three bfloat16 planes.
 xvec_gpu_status gemm_fp32(const GemmCall& c, cudaStream_t s);
 xvec_gpu_status gemm_fp16(const GemmCall& c, cudaStream_t s);

@@ -43,6 +43,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "adapter.cuh"
@@ -849,21 +850,24 @@ xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
   p.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
             ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
   auto kern = gemm_kernel<MODE, T, PAIR, BN>;
-  XVEC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)S::kSmemBytes));
-  if (std::is_same<T, float>::value) {
-    // The register split needs the whole block's share at launch, or it would wait.
-    cudaFuncAttributes fa;
-    XVEC_CUDA(cudaFuncGetAttributes(&fa, kern));
-    if (fa.numRegs * S::kThreads < 128 * kFewRegs + (S::kThreads - 128) * kManyRegs) {
-      set_error("adapter: the matrix kernel was built with %d registers", fa.numRegs);
-      return XVEC_GPU_UNSUPPORTED;
+  static std::atomic<uint64_t> ready{0};  // by device
+  const uint64_t bit = 1ull << (c.device & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    XVEC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)S::kSmemBytes));
+    if (std::is_same<T, float>::value) {
+      // The register split needs the whole block's share at launch, or it would wait.
+      cudaFuncAttributes fa;
+      XVEC_CUDA(cudaFuncGetAttributes(&fa, kern));
+      if (fa.numRegs * S::kThreads < 128 * kFewRegs + (S::kThreads - 128) * kManyRegs) {
+        set_error("adapter: the matrix kernel was built with %d registers", fa.numRegs);
+        return XVEC_GPU_UNSUPPORTED;
+      }
     }
+    if (c.device < 64) ready.fetch_or(bit, std::memory_order_release);
   }
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.batches * p.splits;
-  int device = 0, sms = 0;
-  XVEC_CUDA(cudaGetDevice(&device));
-  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  const int sms = c.sms;
   const int64_t ctas = PAIR ? std::min<int64_t>(items, sms / 2) * 2 : std::min<int64_t>(items, sms);
   XVEC_CUDA(launch_pdl(kern, dim3((unsigned)ctas), S::kThreads, S::kSmemBytes, s,
                        PAIR ? 2 : 1, a, b0, b1, p));

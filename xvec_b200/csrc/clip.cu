@@ -320,7 +320,7 @@ extern "C" xvec_gpu_status xvec_gpu_clip_gradients_device(int32_t device,
   DeviceGuard guard;
   if (xvec_gpu_status st = guard.set(device)) return st;
   int sms = 0;
-  XVEC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  if (xvec_gpu_status st = count_sms(device, &sms)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return num_tensors <= kFew ? clip<kFew>(tensors, num_tensors, max_norm, d_norm, sms, s)
                              : clip<kMany>(tensors, num_tensors, max_norm, d_norm, sms, s);
