@@ -564,7 +564,7 @@ xvec_gpu_status xvec_gpu_rotate_device(int32_t device, const uint8_t* signs, int
  * are contiguous.  Pointers are aligned to their element; 16-byte aligned
  * matrices whose rows are a multiple of 16 bytes apart are read in place,
  * others are first copied into scratch.  Nothing outside the described
- * elements is read or written.
+ * elements is written; reads may touch the rest of the 16 bytes around one.
  *
  * Arithmetic: sums, activations and gradients in float32 or more, one rounding
  * to the storage type for each result.  16-bit storage multiplies its

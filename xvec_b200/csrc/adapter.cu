@@ -176,25 +176,6 @@ xvec_gpu_status forward(int storage, GemmCall& g, Operand* a, Operand* b0, Opera
 // [2][chunks][m]: the column sums of each row chunk in float32, before any
 // rounding.  A block owns 256 columns of a row chunk: 32 threads of 8 columns,
 // 8 rows at a time.  Bound by memory.
-template <typename T>
-struct Eight {
-  static constexpr int N = sizeof(T) / 2;  // 16-byte parts
-  uint4 v[N];
-  __device__ __forceinline__ void load(const T* p, int count, bool vec) {
-    if (vec && count >= 8) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    } else {
-      T* t = reinterpret_cast<T*>(v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = j < count ? p[j] : from_f<T>(0.f);
-    }
-  }
-  __device__ __forceinline__ float operator[](int j) const {
-    return to_f(reinterpret_cast<const T*>(v)[j]);
-  }
-};
-
 // The pre-activation gradients of one backward call and its packings.
 struct Slopes {
   const void *dy, *z, *u;  // u: gated only
@@ -452,8 +433,8 @@ xvec_gpu_status check_shape(const Args* a) {
 // sums and a second launch.  A block takes 512 clocks for a pair's 256 columns (the
 // matrix rate), 448 for 192, 384 for 128 (shared memory's rate), 590 for a single
 // CTA's 128 x 128.  An epilogue column takes about 10 clocks for each matrix that
-// it reads or writes and for an activation, 25 where rows do not allow 16-byte
-// accesses.  192 columns exist for one product along depth (kLinear), where they can
+// it reads or writes and for an activation, up to 25 where rows do not allow
+// 16-byte accesses.  192 columns exist for one product along depth (kLinear), where they can
 // fill the last wave better: 10000 x 960 -> 960 fp32 is 200 tiles of three waves
 // instead of 160 larger ones of three.
 xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
@@ -481,7 +462,7 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
       if (splits > 1 && (per * products < 4 || (int64_t)per * (splits - 1) >= all)) continue;
       const double waves = (double)((tm * tn * p.batches * splits + workers - 1) / workers);
       const double epilogue =
-          cols * (splits > 1 ? 25.0 * half : matrices * (p.vec ? 10.0 : 25.0));
+          cols * (splits > 1 ? 25.0 * half : matrices * (p.vec == 16 ? 10.0 : p.vec >= 4 ? 14.0 : 25.0));
       double cost = waves * (per * block[k] + epilogue) + start[k];
       if (splits > 1)
         cost += 6000 + (double)splits * p.rows * p.ldp * p.batches * half * 8 / 2000;
@@ -598,8 +579,8 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   p.act = a.activation;
   p.status = a.status;
   const size_t size = elem_bytes(a.storage);
-  p.vec = aligned16(a.y, a.ldy, size) && aligned16(a.residual, a.ldr, size) &&
-          aligned16(a.preact, a.ldz, size);
+  p.vec = std::min({access_width(a.y, a.ldy, size), access_width(a.residual, a.ldr, size),
+                    access_width(a.preact, a.ldz, size)});
   p.bias_vec = aligned16(a.bias, 0, size);
   return forward(a.storage, g, &x, &w, nullptr, arena, s);
 }
@@ -653,8 +634,8 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   p.act = a.activation;
   p.status = a.status;
   const size_t size = elem_bytes(a.storage);
-  p.vec = aligned16(a.h, a.ldh, size) && aligned16(a.gate, a.ldg, size) &&
-          aligned16(a.up, a.ldg, size);
+  p.vec = std::min({access_width(a.h, a.ldh, size), access_width(a.gate, a.ldg, size),
+                    access_width(a.up, a.ldg, size)});
   p.bias_vec = aligned16(a.gate_bias, 0, size) && aligned16(a.up_bias, 0, size);
   return forward(a.storage, g, &x, &wg, &wu, arena, s);
 }
@@ -722,18 +703,18 @@ xvec_gpu_status run_backward(const Backward& b) {
   dx.depth = b.out_dim;
   dx.p.rows = b.n, dx.p.cols = b.in_dim, dx.p.segs = b.parts, dx.p.batches = 1;
   dx.p.out[0] = b.dx, dx.p.ldo = b.lddx;
-  dx.p.vec = aligned16(b.dx, b.lddx, size);
+  dx.p.vec = access_width(b.dx, b.lddx, size);
   dx.p.status = b.status;
   dw.mode = kDw;
   dw.depth = b.n;
   dw.p.rows = b.out_dim, dw.p.cols = b.in_dim, dw.p.segs = 1;
-  dw.p.vec = 1;
+  dw.p.vec = 16;
   dw.p.ldo = b.lddw;
   dw.p.status = b.status;
   const int first = b.dw[0] ? 0 : 1;  // 1: only the second weight's gradient
   for (int i = first; i < b.parts && b.dw[i]; ++i) {
     dw.p.out[dw.p.batches++] = b.dw[i];
-    dw.p.vec &= aligned16(b.dw[i], b.lddw, size);
+    dw.p.vec = std::min(dw.p.vec, access_width(b.dw[i], b.lddw, size));
   }
   if (b.dx && (st = plan_gemm(b.storage, &dx))) return st;
   if (dw.p.batches && (st = plan_gemm(b.storage, &dw))) return st;
@@ -741,14 +722,18 @@ xvec_gpu_status run_backward(const Backward& b) {
   const size_t partial_at = arena.add(std::max(dx.partial_bytes, dw.partial_bytes));
 
   if ((st = arena.alloc(s))) return st;
-  for (Operand* o : {&w[0], &w[1], &x}) place(o, arena, &a.packs);
+  Packs packs;
+  for (Operand* o : {&w[0], &w[1], &x}) place(o, arena, &packs);
   if (!direct && products) grad.p = a.out = static_cast<uint16_t*>(arena.at(grad_at));
   if (sums) a.partial = static_cast<float*>(arena.at(sums_at));
-  if (!direct || sums) {
-    if ((st = slopes(b.storage, a, s))) return st;
-  } else if ((st = run_packs(b.storage, a.packs, s))) {
-    return st;
-  }
+  // Small packings share the gradient pass's launch; large ones want the warps that
+  // its registers leave no room for (75103 x 402 fp32: 122 us together).
+  int64_t packed = 0;
+  for (int i = 0; i < packs.n; ++i) packed += packs.p[i].rows * packs.p[i].ld;
+  const bool pass = !direct || sums, together = pass && packed < 4'000'000;
+  if (together) a.packs = packs;
+  if (pass && (st = slopes(b.storage, a, s))) return st;
+  if (!together && (st = run_packs(b.storage, packs, s))) return st;
   GemmParams& carrier = b.dx ? dx.p : dw.p;  // takes the column sums along
   if (sums) {
     carrier.sums = a.partial, carrier.sum_chunks = a.chunks, carrier.sum_cols = a.m;

@@ -137,26 +137,52 @@ __device__ __forceinline__ float activate_slope(int act, float z, float* slope) 
   }
 }
 
-// Eight elements of a row as floats, from an address that may be unaligned
-// (vec = false) and of which only `count` exist (the rest 0).
+// The 16 bytes from p on, of which `count` elements exist (what the others hold
+// is of no account).  `vec`: p is a multiple of 16.  If not, the two 16-byte granules
+// that hold them are read and shifted together: selects by the offset's words, then
+// a funnel shift by its half word.  A granule is read only if it holds one of the
+// elements.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
-  if (vec && count >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0];
-      const float4 b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const T* t = reinterpret_cast<const T*>(&u);
+__device__ __forceinline__ uint4 load16(const T* p, int count, bool vec) {
+  constexpr int kPart = 16 / sizeof(T);
+  const uintptr_t end = (uintptr_t)(p + (count < kPart ? count : kPart));
+  const uint32_t off = vec ? 0 : (uint32_t)(uintptr_t)p & 15;
+  const uint4* base = reinterpret_cast<const uint4*>((uintptr_t)p - off);
+  if (count <= 0) return make_uint4(0, 0, 0, 0);
+  const uint4 a = *base;
+  if (off == 0) return a;
+  const uint4 b = (uintptr_t)(base + 1) < end ? base[1] : make_uint4(0, 0, 0, 0);
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f(t[j]);
-    }
-  } else {
+  for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_f(p[j]) : 0.f;
+  for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+  if (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Eight elements of a row, of which `count` exist.
+template <typename T>
+struct Eight {
+  static constexpr int N = sizeof(T) / 2;  // 16-byte parts
+  uint4 v[N];
+  __device__ __forceinline__ void load(const T* p, int count, bool vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = load16(p + 8 / N * i, count - 8 / N * i, vec);
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    return to_f(reinterpret_cast<const T*>(v)[j]);
+  }
+};
+// The same as floats, zeros where no element is.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&f)[8]) {
+  Eight<T> e;
+  e.load(p, count, vec);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = j < count ? e[j] : 0.f;
 }
 
 // Launches of one call overlap at their edges: a kernel lets the next one start
@@ -217,8 +243,8 @@ struct GemmParams {
   float* partial;        // splits > 1: [splits][batches or halves][rows][ldp] float sums
   int64_t ldp;
   uint32_t idesc;
-  int vec;               // outputs, saves and residual allow 16-byte accesses
-  int bias_vec;          // and the biases
+  int vec;               // bytes of an access that outputs, saves and residual allow
+  int bias_vec;          // the biases allow 16
   const void* bias[2];
   const void* residual;
   void* out[2];
@@ -291,6 +317,11 @@ __device__ __forceinline__ void column_sums(const float* sums, int chunks, int m
   }
 }
 
+// The widest access in bytes, up to 16, that fits every row.
+inline int access_width(const void* p, int64_t ld, size_t size) {
+  const uint64_t bits = 16 | (uintptr_t)p | (uint64_t)ld * size;
+  return (int)(bits & (~bits + 1));
+}
 // Rows read in place with 16-byte accesses.
 inline bool aligned16(const void* p, int64_t ld, size_t size) {
   return (uintptr_t)p % 16 == 0 && ld * (int64_t)size % 16 == 0;

@@ -76,8 +76,9 @@ struct GemmShape {
   static constexpr uint32_t kStageBytes = kUnits * kBlockBytes;
   // Columns that an epilogue warp finishes at a time, and their staging block of 32
   // rows: 128 bytes a row where its columns come in 64s (or 32 float32), else 64.
+  // (Gated sums come in pairs: 64 of each spill.)
   static constexpr int kOutCols = BN / 2 / (MODE == kGated ? 2 : 1);  // outputs of a warp
-  static constexpr int kStep = sizeof(T) == 2 && kOutCols % 64 == 0 ? 64 : 32;
+  static constexpr int kStep = sizeof(T) == 2 && MODE != kGated && kOutCols % 64 == 0 ? 64 : 32;
   static constexpr int kRowBytes = kStep * sizeof(T);
   static constexpr uint32_t kEpiBytes = kEpiWarps * 32 * kRowBytes;
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
@@ -225,9 +226,46 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
   return u;
 }
 
+// The staging rows to memory in accesses of W bytes: 32 W / RB rows at a time.
+template <typename T, int RB, int W>
+__device__ __forceinline__ void copy_out(uint32_t buf, T* out, int64_t ld, int rows, int lane) {
+  constexpr int kLanes = RB / W, kRows = 32 / kLanes;  // lanes of a row, rows at a time
+  const int at = lane % kLanes * W, row = lane / kLanes;
+  char* dst = reinterpret_cast<char*>(out) + at;
+#pragma unroll
+  for (int i0 = 0; i0 < 32 / kRows; i0 += 8) {
+    uint32_t u[8][W / 4];
+#pragma unroll
+    for (int i = 0; i < 8 && i0 + i < 32 / kRows; ++i) {
+      const uint32_t a = stage_at<RB>(buf, (i0 + i) * kRows + row, at / 16) + at % 16;
+      if constexpr (W == 16) {
+        const uint4 t = lds16(a);
+        u[i][0] = t.x, u[i][1] = t.y, u[i][2] = t.z, u[i][3] = t.w;
+      } else if constexpr (W == 8) {
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(u[i][0]), "=r"(u[i][1]) : "r"(a) : "memory");
+      } else {
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u[i][0]) : "r"(a) : "memory");
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8 && i0 + i < 32 / kRows; ++i) {
+      const int r = (i0 + i) * kRows + row;
+      if (r >= rows) continue;
+      char* p = dst + r * ld * (int)sizeof(T);
+      if constexpr (W == 16)
+        *reinterpret_cast<uint4*>(p) = make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
+      else if constexpr (W == 8)
+        *reinterpret_cast<uint2*>(p) = make_uint2(u[i][0], u[i][1]);
+      else
+        *reinterpret_cast<uint32_t*>(p) = u[i][0];
+    }
+  }
+}
+
 // Writes v (this lane's row) to base[row * ld + column], rows and cols of it.
+// width: the bytes of an access that its rows allow (16, 8, 4; 2 for 16-bit types).
 template <typename T, int RB, int N>
-__device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows, int cols, bool vec,
+__device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows, int cols, int width,
                                      const float (&v)[N], int lane) {
   constexpr int kParts = RB / 16, kPart = 16 / sizeof(T), kCols = RB / sizeof(T);
   static_assert(N % kCols == 0, "whole staging rows");
@@ -239,16 +277,10 @@ __device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows
     __syncwarp();
     T* out = base + h * kCols;
     const int left = cols - h * kCols;
-    if (vec && left >= kCols) {
-      const int part = lane % kParts, row = lane / kParts;
-      uint4 u[kParts];
-#pragma unroll
-      for (int i = 0; i < kParts; ++i) u[i] = lds16(stage_at<RB>(buf, i * (32 / kParts) + row, part));
-#pragma unroll
-      for (int i = 0; i < kParts; ++i) {
-        const int r = i * (32 / kParts) + row;
-        if (r < rows) *reinterpret_cast<uint4*>(out + r * ld + part * kPart) = u[i];
-      }
+    if (left >= kCols && width >= 4) {
+      if (width == 16) copy_out<T, RB, 16>(buf, out, ld, rows, lane);
+      else if (width == 8) copy_out<T, RB, 8>(buf, out, ld, rows, lane);
+      else copy_out<T, RB, 4>(buf, out, ld, rows, lane);
     } else {
       // A column a lane, a row after the other.
 #pragma unroll
@@ -279,38 +311,32 @@ __device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows
 // lane's row later (add).  Rows or columns that do not exist are not read.
 template <typename T, int RB>
 struct Incoming {
-  static constexpr int kParts = RB / 16, N = RB / sizeof(T);
+  static constexpr int kParts = RB / 16, kPart = 16 / sizeof(T), N = RB / sizeof(T);
   uint4 v[kParts];
 
-  __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, bool whole, int lane) {
+  __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, int cols, bool vec,
+                                        int lane) {
+    const int part = lane % kParts, row = lane / kParts;
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const int r = i * (32 / kParts) + lane / kParts;
+      const int r = i * (32 / kParts) + row;
       v[i] = make_uint4(0, 0, 0, 0);
-      if (whole && r < rows)
-        v[i] = *reinterpret_cast<const uint4*>(base + r * ld + (lane % kParts) * (16 / sizeof(T)));
+      if (r < rows) v[i] = load16(base + r * ld + part * kPart, cols - part * kPart, vec);
     }
   }
-  __device__ __forceinline__ void add(uint32_t buf, const T* base, int64_t ld, int rows, int cols,
-                                      bool whole, float (&f)[N], int lane) {
-    if (whole) {
+  __device__ __forceinline__ void add(uint32_t buf, float (&f)[N], int lane) {
 #pragma unroll
-      for (int i = 0; i < kParts; ++i)
-        sts16(stage_at<RB>(buf, i * (32 / kParts) + lane / kParts, lane % kParts), v[i]);
-      __syncwarp();
+    for (int i = 0; i < kParts; ++i)
+      sts16(stage_at<RB>(buf, i * (32 / kParts) + lane / kParts, lane % kParts), v[i]);
+    __syncwarp();
 #pragma unroll
-      for (int c = 0; c < kParts; ++c) {
-        const uint4 u = lds16(stage_at<RB>(buf, lane, c));
-        const T* t = reinterpret_cast<const T*>(&u);
+    for (int c = 0; c < kParts; ++c) {
+      const uint4 u = lds16(stage_at<RB>(buf, lane, c));
+      const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
-        for (int j = 0; j < 16 / (int)sizeof(T); ++j) f[c * (16 / sizeof(T)) + j] += to_f(t[j]);
-      }
-      __syncwarp();
-    } else if (lane < rows) {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j < cols) f[j] += to_f(base[lane * ld + j]);
+      for (int j = 0; j < kPart; ++j) f[c * kPart + j] += to_f(t[j]);
     }
+    __syncwarp();
   }
 };
 
@@ -576,7 +602,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
     const uint32_t buf = smem_u32(staging + ew * 32 * RB);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tfull_at = smem_u32(tfull);
-    const bool vec = p.vec != 0;
+    const bool vec = p.vec == 16;  // of the residual
     // Waits for accumulator `acc`.  One lane polls; the others wait at the shuffle.
     auto wait_acc = [&](uint32_t acc, uint32_t parity) {
       int ok = 1;
@@ -602,6 +628,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
       return which * (BN / 2) + group * kOutCols + c;
     };
     using Step = float[S::kStep];
+    auto limit32 = [](int64_t c) { return (int)max((int64_t)0, min((int64_t)kStep, c)); };
     uint32_t round = 0, tile = 0;
     for (int i = worker; i < items; i += workers, ++tile) {
       const Item it = item_of(i);
@@ -614,7 +641,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
                          : nullptr;
       Incoming<T, RB> in;
       // (float32 has no registers for it while it drains.)
-      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, vec && cols >= kStep, lane);
+      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, limit32(cols), vec, lane);
       // Finishes kStep columns from `at` on: v the sums (gated: the gate's; up() then
       // gives the up's, late, so that both are not held longer than needed).
       auto finish = [&](int at, Step& v, auto&& up) {
@@ -626,11 +653,11 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
                        ((int64_t)(it.split * p.batches + it.batch) * kPlanes * p.rows + row0) *
                            p.ldp + col;
           // (ldp covers whole steps.)
-          if (n > 0) emit<float, RB>(buf, dst, p.ldp, rows, kStep, true, v, lane);
+          if (n > 0) emit<float, RB>(buf, dst, p.ldp, rows, kStep, 16, v, lane);
           if constexpr (MODE == kGated) {
             up(v);
             if (n > 0)
-              emit<float, RB>(buf, dst + p.rows * p.ldp, p.ldp, rows, kStep, true, v, lane);
+              emit<float, RB>(buf, dst + p.rows * p.ldp, p.ldp, rows, kStep, 16, v, lane);
           }
           return;
         }
@@ -640,9 +667,9 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           add_bias(b ? b + col : b, n, p.bias_vec != 0, x);
           if (p.save[which] && n > 0)
             emit<T, RB>(buf, static_cast<T*>(p.save[which]) + row0 * p.lds + col, p.lds, rows, n,
-                        vec, x, lane);
+                        p.vec, x, lane);
         };
-        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, vec && n == kStep, lane);
+        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, n, vec, lane);
         if constexpr (MODE == kLinear || MODE == kGated) {
           affine(0, v);
           activate_all<T>(p.act, v);
@@ -655,13 +682,13 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           for (int j = 0; j < kStep; ++j) v[j] *= u[j];
         }
         if (MODE == kLinear && res && n > 0) {
-          in.add(buf, res + at, p.ldr, rows, n, vec && n == kStep, v, lane);
+          in.add(buf, v, lane);
           if (P == 1 && at + kStep < kOutCols)
-            in.start(res + at + kStep, p.ldr, rows, vec && cols >= at + 2 * kStep, lane);
+            in.start(res + at + kStep, p.ldr, rows, limit32(cols - at - kStep), vec, lane);
         }
         if (n > 0)
           emit<T, RB>(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col,
-                      p.ldo, rows, n, vec, v, lane);
+                      p.ldo, rows, n, p.vec, v, lane);
       };
       if constexpr (P == 1) {
         const uint32_t acc = tile & 1, t = tmem_base + acc * BN + lanes;
