@@ -63,18 +63,28 @@ struct Packs {
   Pack p[3];
   int n = 0;
 };
-template <typename T>
-__device__ __forceinline__ void pack(const Pack& p, int64_t thread, int64_t threads) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void pack_rows(const Pack& p, int64_t thread, int64_t threads) {
   const T* src = static_cast<const T*>(p.src);
   const int64_t groups = p.ld / 8, total = groups * p.rows;
+#pragma unroll 2
   for (int64_t i = thread; i < total; i += threads) {
     // (64-bit divisions would cost more than the copy.)
     const int64_t r = total >> 32 ? i / groups : (uint32_t)i / (uint32_t)groups;
     const int c = (int)(i - r * groups) * 8;
+    Eight<T, VEC> e;
+    e.load(src + r * p.lds + c, p.cols - c);
+    e.settle();
     float v[8];
-    load8(src + r * p.lds + c, p.cols - c, p.vec, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < p.cols ? e[j] : 0.f;
     store_operand<T>(static_cast<uint16_t*>(p.dst) + r * p.ld + c, p.rows * p.ld, v);
   }
+}
+template <typename T>
+__device__ __forceinline__ void pack(const Pack& p, int64_t thread, int64_t threads) {
+  if (p.vec) pack_rows<T, true>(p, thread, threads);
+  else pack_rows<T, false>(p, thread, threads);
 }
 // Packs up to three matrices (blockIdx.y) at once.  Bound by memory.
 template <typename T>
@@ -180,7 +190,7 @@ xvec_gpu_status forward(int storage, GemmCall& g, Operand* a, Operand* b0, Opera
 struct Slopes {
   const void *dy, *z, *u;  // u: gated only
   int64_t lddy, ldz, n;
-  int m, act, vec;  // vec: 1, 2, 4 = dy, z, u allow 16-byte accesses
+  int m, act;
   int cols, chunks;  // blocks: of 256 columns, of rows_per_chunk rows
   int64_t rows_per_chunk;
   uint16_t* out;
@@ -193,8 +203,9 @@ struct Slopes {
 // Blocks [0, cols chunks) are the gradients', the others the packings'.
 // kRows rows of a thread are requested before the first is used and held as
 // they came.  (Held as floats they took 122 registers, a quarter of the warps.)
-template <typename T, bool GATED>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
+// VEC: all of dy, z and u allow 16-byte accesses.
+template <typename T, bool GATED, bool VEC>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : VEC ? 4 : 3)
     slope_kernel(const __grid_constant__ Slopes p) {
   pdl_begin();
   const unsigned slope_blocks = (unsigned)p.cols * p.chunks;
@@ -209,7 +220,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
   const T* z = static_cast<const T*>(p.z);
   const T* u = static_cast<const T*>(p.u);
   const int64_t lddy = p.lddy, ldz = p.ldz, n = p.n, ld = p.ld;
-  const int m = p.m, act = p.act, vec = p.vec;
+  const int m = p.m, act = p.act;
   uint16_t* out = p.out;
   constexpr int kOuts = GATED ? 2 : 1;
   constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
@@ -222,17 +233,20 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
   float sum[kOuts][8] = {};
   if (c < m) {
     for (int64_t r = r0 + ty; r < r1; r += 8 * kRows) {
-      Eight<T> dr[kRows], zr[kRows], ur[kRows];
+      Eight<T, VEC> dr[kRows], zr[kRows], ur[kRows];
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const int64_t q = r + 8 * i < r1 ? r + 8 * i : r;
-        dr[i].load(dy + q * lddy + c, m - c, vec & 1);
-        if (act_needed) zr[i].load(z + q * ldz + c, m - c, vec & 2);
-        if (GATED) ur[i].load(u + q * ldz + c, m - c, vec & 4);
+        dr[i].load(dy + q * lddy + c, m - c);
+        if (act_needed) zr[i].load(z + q * ldz + c, m - c);
+        if (GATED) ur[i].load(u + q * ldz + c, m - c);
       }
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         if (r + 8 * i >= r1) break;
+        dr[i].settle();
+        if (act_needed) zr[i].settle();
+        if (GATED) ur[i].settle();
         float d[kOuts][8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -294,13 +308,15 @@ void plan_slopes(Slopes* a) {
 
 template <typename T>
 xvec_gpu_status slopes_t(Slopes& a, cudaStream_t s) {
-  a.vec = (aligned16(a.dy, a.lddy, sizeof(T)) ? 1 : 0) |
-          (aligned16(a.z, a.ldz, sizeof(T)) ? 2 : 0) | (aligned16(a.u, a.ldz, sizeof(T)) ? 4 : 0);
+  const bool vec = aligned16(a.dy, a.lddy, sizeof(T)) &&
+                   (aligned16(a.z, a.ldz, sizeof(T)) || (!a.u && a.act == XVEC_ACT_NONE)) &&
+                   (!a.u || aligned16(a.u, a.ldz, sizeof(T)));
   int64_t most = 0;
   for (int i = 0; i < a.packs.n; ++i)
     most = std::max(most, a.packs.p[i].rows * a.packs.p[i].ld / 8);
   a.pack_blocks = grid_of(most);
-  auto* kern = a.u ? slope_kernel<T, true> : slope_kernel<T, false>;
+  auto* kern = a.u ? (vec ? slope_kernel<T, true, true> : slope_kernel<T, true, false>)
+                   : (vec ? slope_kernel<T, false, true> : slope_kernel<T, false, false>);
   XVEC_CUDA(launch_pdl(kern, dim3((unsigned)a.cols * a.chunks + a.pack_blocks * a.packs.n), 256, 0,
                        s, 1, a));
   return XVEC_GPU_OK;
@@ -579,8 +595,7 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   p.act = a.activation;
   p.status = a.status;
   const size_t size = elem_bytes(a.storage);
-  p.vec = std::min({access_width(a.y, a.ldy, size), access_width(a.residual, a.ldr, size),
-                    access_width(a.preact, a.ldz, size)});
+  p.vec = std::min(access_width(a.y, a.ldy, size), access_width(a.preact, a.ldz, size));
   p.bias_vec = aligned16(a.bias, 0, size);
   return forward(a.storage, g, &x, &w, nullptr, arena, s);
 }

@@ -137,21 +137,10 @@ __device__ __forceinline__ float activate_slope(int act, float z, float* slope) 
   }
 }
 
-// The 16 bytes from p on, of which `count` elements exist (what the others hold
-// is of no account).  `vec`: p is a multiple of 16.  If not, the two 16-byte granules
-// that hold them are read and shifted together: selects by the offset's words, then
-// a funnel shift by its half word.  A granule is read only if it holds one of the
-// elements.
+// Sixteen bytes that start `off` bytes into granule a and end in the next, b:
+// selects by the offset's words, then a funnel shift by its half word.
 template <typename T>
-__device__ __forceinline__ uint4 load16(const T* p, int count, bool vec) {
-  constexpr int kPart = 16 / sizeof(T);
-  const uintptr_t end = (uintptr_t)(p + (count < kPart ? count : kPart));
-  const uint32_t off = vec ? 0 : (uint32_t)(uintptr_t)p & 15;
-  const uint4* base = reinterpret_cast<const uint4*>((uintptr_t)p - off);
-  if (count <= 0) return make_uint4(0, 0, 0, 0);
-  const uint4 a = *base;
-  if (off == 0) return a;
-  const uint4 b = (uintptr_t)(base + 1) < end ? base[1] : make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, uint32_t off) {
   uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
@@ -163,27 +152,37 @@ __device__ __forceinline__ uint4 load16(const T* p, int count, bool vec) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Eight elements of a row, of which `count` exist.
-template <typename T>
+// The 16-byte granule at p, if it starts before `end`.
+__device__ __forceinline__ uint4 granule(uintptr_t p, uintptr_t end) {
+  return p < end ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+}
+
+// Eight elements of a row, of which `count` exist (what the others hold is of no
+// account), in two steps: load requests the 16-byte granules that hold them, each
+// only if it holds one of the elements; settle, once they are needed, shifts
+// them together where they do not start on 16 bytes (VEC: they do).
+template <typename T, bool VEC>
 struct Eight {
   static constexpr int N = sizeof(T) / 2;  // 16-byte parts
-  uint4 v[N];
-  __device__ __forceinline__ void load(const T* p, int count, bool vec) {
+  uint4 v[VEC ? N : N + 1];
+  uint32_t off;
+  __device__ __forceinline__ void load(const T* p, int count) {
+    off = VEC ? 0 : (uint32_t)(uintptr_t)p & 15;
+    const uintptr_t base = (uintptr_t)p - off;
+    const uintptr_t end = (uintptr_t)(p + (count < 8 ? count : 8));
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = load16(p + 8 / N * i, count - 8 / N * i, vec);
+    for (int i = 0; i < (VEC ? N : N + 1); ++i) v[i] = granule(base + 16 * i, end);
+  }
+  __device__ __forceinline__ void settle() {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = shifted<T>(v[i], v[i + 1], off);
+    }
   }
   __device__ __forceinline__ float operator[](int j) const {
     return to_f(reinterpret_cast<const T*>(v)[j]);
   }
 };
-// The same as floats, zeros where no element is.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&f)[8]) {
-  Eight<T> e;
-  e.load(p, count, vec);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = j < count ? e[j] : 0.f;
-}
 
 // Launches of one call overlap at their edges: a kernel lets the next one start
 // as soon as all its own blocks have started (pdl_begin), and touches memory only
@@ -243,7 +242,7 @@ struct GemmParams {
   float* partial;        // splits > 1: [splits][batches or halves][rows][ldp] float sums
   int64_t ldp;
   uint32_t idesc;
-  int vec;               // bytes of an access that outputs, saves and residual allow
+  int vec;               // bytes of an access that outputs and saves allow
   int bias_vec;          // the biases allow 16
   const void* bias[2];
   const void* residual;

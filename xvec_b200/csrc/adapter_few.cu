@@ -44,9 +44,9 @@ __device__ __forceinline__ float scatter_sum(float (&v)[N], int lane) {
 }
 constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 
-template <typename T, bool GATED, int ROWS, int COLS>
-__global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_constant__ FewRows p,
-                                                               bool x_vec, bool w_vec) {
+// VEC: x and the weights allow 16-byte accesses, in_dim is a multiple of 8.
+template <typename T, bool GATED, int ROWS, int COLS, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_constant__ FewRows p) {
   constexpr int W = GATED ? 2 : 1;
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -56,24 +56,32 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_cons
 #pragma unroll 2
   for (int k = threadIdx.x * 8; k < p.in_dim; k += kWarps * 256) {
     const int count = p.in_dim - k;
-    float w[W][COLS][8];
+    Eight<T, VEC> w[W][COLS];
 #pragma unroll
     for (int m = 0; m < W; ++m)
 #pragma unroll
       for (int c = 0; c < COLS; ++c)  // (a column that does not exist repeats the last)
-        load8(static_cast<const T*>(p.w[m]) + (int64_t)min(c0 + c, p.out_dim - 1) * p.ldw + k,
-              count, w_vec, w[m][c]);
+        w[m][c].load(
+            static_cast<const T*>(p.w[m]) + (int64_t)min(c0 + c, p.out_dim - 1) * p.ldw + k, count);
+#pragma unroll
+    for (int m = 0; m < W; ++m)
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) w[m][c].settle();
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      float v[8];
-      load8(x + (int64_t)min(r0 + r, p.n - 1) * p.ldx + k, count, x_vec, v);
+      Eight<T, VEC> v;
+      v.load(x + (int64_t)min(r0 + r, p.n - 1) * p.ldx + k, count);
+      v.settle();
 #pragma unroll
-      for (int m = 0; m < W; ++m)
+      for (int j = 0; j < 8; ++j) {
+        const bool in = VEC || j < count;  // (past the row's end lie other elements)
 #pragma unroll
-        for (int c = 0; c < COLS; ++c)
+        for (int m = 0; m < W; ++m)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            sum[m][r * COLS + c] = fmaf(v[j], w[m][c][j], sum[m][r * COLS + c]);
+          for (int c = 0; c < COLS; ++c)
+            sum[m][r * COLS + c] =
+                fmaf(in ? v[j] : 0.f, in ? w[m][c][j] : 0.f, sum[m][r * COLS + c]);
+      }
     }
   }
   // Lane `lane` >> kShift holds one sum of its warp; the first warp adds them up.
@@ -104,11 +112,12 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const __grid_cons
 
 template <typename T, bool GATED, int ROWS, int COLS>
 xvec_gpu_status launch(const FewRows& f, cudaStream_t s) {
-  XVEC_CUDA(launch_pdl(few_rows_kernel<T, GATED, ROWS, COLS>,
-                       dim3((f.out_dim + COLS - 1) / COLS, (f.n + ROWS - 1) / ROWS), kWarps * 32,
-                       0, s, 1, f, aligned16(f.x, f.ldx, sizeof(T)),
-                       aligned16(f.w[0], f.ldw, sizeof(T)) &&
-                           aligned16(f.w[1], f.ldw, sizeof(T))));
+  const bool vec = aligned16(f.x, f.ldx, sizeof(T)) && aligned16(f.w[0], f.ldw, sizeof(T)) &&
+                   aligned16(f.w[1], f.ldw, sizeof(T)) && f.in_dim % 8 == 0;
+  auto* kern = vec ? few_rows_kernel<T, GATED, ROWS, COLS, true>
+                   : few_rows_kernel<T, GATED, ROWS, COLS, false>;
+  XVEC_CUDA(launch_pdl(kern, dim3((f.out_dim + COLS - 1) / COLS, (f.n + ROWS - 1) / ROWS),
+                       kWarps * 32, 0, s, 1, f));
   return XVEC_GPU_OK;
 }
 

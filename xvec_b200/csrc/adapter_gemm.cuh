@@ -308,33 +308,42 @@ __device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows
 }
 
 // A block of 32 rows on its way in: requested early (start), added to this
-// lane's row later (add).  Rows or columns that do not exist are not read.
+// lane's row later (add).  Rows that do not start on 16 bytes come as the granules
+// that hold them, one more than they have parts (each lane keeps its row's last),
+// and are shifted together from the staging block.  Rows or columns that do not
+// exist are not read.
 template <typename T, int RB>
 struct Incoming {
   static constexpr int kParts = RB / 16, kPart = 16 / sizeof(T), N = RB / sizeof(T);
-  uint4 v[kParts];
+  uint4 v[kParts], last;
+  uint32_t off;  // of this lane's row
 
-  __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, int cols, bool vec,
-                                        int lane) {
-    const int part = lane % kParts, row = lane / kParts;
+  __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, int cols, int lane) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const int r = i * (32 / kParts) + row;
-      v[i] = make_uint4(0, 0, 0, 0);
-      if (r < rows) v[i] = load16(base + r * ld + part * kPart, cols - part * kPart, vec);
+      const int r = i * (32 / kParts) + lane / kParts;
+      const uintptr_t p = (uintptr_t)(base + r * ld), end = (uintptr_t)(base + r * ld + cols);
+      v[i] = granule(p / 16 * 16 + lane % kParts * 16, r < rows ? end : 0);
     }
+    const uintptr_t p = (uintptr_t)(base + lane * ld), end = (uintptr_t)(base + lane * ld + cols);
+    off = (uint32_t)p & 15;
+    last = granule(p / 16 * 16 + RB, lane < rows && off ? end : 0);
   }
   __device__ __forceinline__ void add(uint32_t buf, float (&f)[N], int lane) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i)
       sts16(stage_at<RB>(buf, i * (32 / kParts) + lane / kParts, lane % kParts), v[i]);
     __syncwarp();
+    uint4 u = lds16(stage_at<RB>(buf, lane, 0));
+    const bool straight = __all_sync(0xffffffffu, off == 0);
 #pragma unroll
     for (int c = 0; c < kParts; ++c) {
-      const uint4 u = lds16(stage_at<RB>(buf, lane, c));
+      const uint4 next = c + 1 < kParts ? lds16(stage_at<RB>(buf, lane, c + 1)) : last;
+      if (!straight) u = shifted<T>(u, next, off);
       const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
       for (int j = 0; j < kPart; ++j) f[c * kPart + j] += to_f(t[j]);
+      u = next;
     }
     __syncwarp();
   }
@@ -602,7 +611,6 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
     const uint32_t buf = smem_u32(staging + ew * 32 * RB);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tfull_at = smem_u32(tfull);
-    const bool vec = p.vec == 16;  // of the residual
     // Waits for accumulator `acc`.  One lane polls; the others wait at the shuffle.
     auto wait_acc = [&](uint32_t acc, uint32_t parity) {
       int ok = 1;
@@ -641,7 +649,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
                          : nullptr;
       Incoming<T, RB> in;
       // (float32 has no registers for it while it drains.)
-      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, limit32(cols), vec, lane);
+      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, limit32(cols), lane);
       // Finishes kStep columns from `at` on: v the sums (gated: the gate's; up() then
       // gives the up's, late, so that both are not held longer than needed).
       auto finish = [&](int at, Step& v, auto&& up) {
@@ -669,7 +677,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
             emit<T, RB>(buf, static_cast<T*>(p.save[which]) + row0 * p.lds + col, p.lds, rows, n,
                         p.vec, x, lane);
         };
-        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, n, vec, lane);
+        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, n, lane);
         if constexpr (MODE == kLinear || MODE == kGated) {
           affine(0, v);
           activate_all<T>(p.act, v);
@@ -684,7 +692,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
         if (MODE == kLinear && res && n > 0) {
           in.add(buf, v, lane);
           if (P == 1 && at + kStep < kOutCols)
-            in.start(res + at + kStep, p.ldr, rows, limit32(cols - at - kStep), vec, lane);
+            in.start(res + at + kStep, p.ldr, rows, limit32(cols - at - kStep), lane);
         }
         if (n > 0)
           emit<T, RB>(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col,
