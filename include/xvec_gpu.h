@@ -568,14 +568,19 @@ xvec_gpu_status xvec_gpu_rotate_device(int32_t device, const uint8_t* signs, int
  *
  * Arithmetic: sums, activations and gradients in float32 or more, one rounding
  * to the storage type for each result.  16-bit storage multiplies its
- * elements exactly; float32 storage multiplies three bfloat16 parts of each
- * element (all products above 2^-24 of the whole), so float32 results have
- * float32 accuracy, but an infinity in a float32 operand may come out as a NaN.
- * Gradients of pre-activations are rounded to 16 bits in between for 16-bit
- * storage.  Results do not vary from run to run.
+ * elements exactly; the matrix units add them up in float32, truncating.
+ * float32 storage multiplies three bfloat16 parts of each element (all
+ * products above 2^-24 of the whole) and adds most sums in registers, so that
+ * float32 results have float32 accuracy (2-norm errors of 1e-7 to 3e-7), but an
+ * infinity in a float32 operand may come out as a NaN, and elements below
+ * 2^-109 are held to 2^-134.  Gradients of pre-activations are rounded to
+ * 16 bits in between for 16-bit storage.  Results do not vary from run to run
+ * on a device, but a different number of rows may change their last bits.
  *
  * Every call enqueues on `stream` and does not wait; it can be captured into
- * a CUDA graph.  Scratch is allocated and freed in stream order.  n = 0 does
+ * a CUDA graph.  Scratch is allocated and freed in stream order (float32: 6
+ * bytes for each element of every operand; 16-bit: only what cannot be read in
+ * place, the pre-activation gradients and split sums).  n = 0 does
  * nothing in the forward calls and gives zero weight and bias gradients.  An
  * output may not overlap an input or another output (XVEC_GPU_INVALID_ARGUMENT),
  * except that y may be the residual itself.  `status` (device int32, may be

@@ -16,6 +16,8 @@ the search path so that tests read like the reference's own:
   assignKMeans                                   kmeans_assign (kmeans.go:382-479)
   core.MergeSearchResults                        merge_results_device (query.go:154-191)
   segment fan-out + merge (collection.go:4040-4066)  Comm, sharded_search(_device)
+  (learned adapters: no counterpart)             linear_device, gated_device, their
+                                                 *_backward_device, clip_gradients_device
 
 There is no CPU fallback: importing this module fails if the shared library is
 missing, and every search runs on a CUDA device.

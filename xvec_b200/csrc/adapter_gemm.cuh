@@ -318,6 +318,10 @@ struct Incoming {
   uint4 v[kParts], last;
   uint32_t off;  // of this lane's row
 
+  // (A plain load: the residual may be the output itself.)
+  static __device__ __forceinline__ uint4 granule(uintptr_t p, uintptr_t end) {
+    return p < end ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+  }
   __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, int cols, int lane) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
