@@ -76,9 +76,8 @@ struct GemmShape {
   static constexpr uint32_t kStageBytes = kUnits * kBlockBytes;
   // Columns that an epilogue warp finishes at a time, and their staging block of 32
   // rows: 128 bytes a row where its columns come in 64s (or 32 float32), else 64.
-  // (Gated sums come in pairs: 64 of each spill.)
   static constexpr int kOutCols = BN / 2 / (MODE == kGated ? 2 : 1);  // outputs of a warp
-  static constexpr int kStep = sizeof(T) == 2 && MODE != kGated && kOutCols % 64 == 0 ? 64 : 32;
+  static constexpr int kStep = sizeof(T) == 2 && kOutCols % 64 == 0 ? 64 : 32;
   static constexpr int kRowBytes = kStep * sizeof(T);
   static constexpr uint32_t kEpiBytes = kEpiWarps * 32 * kRowBytes;
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
@@ -262,48 +261,59 @@ __device__ __forceinline__ void copy_out(uint32_t buf, T* out, int64_t ld, int r
   }
 }
 
-// Writes v (this lane's row) to base[row * ld + column], rows and cols of it.
-// width: the bytes of an access that its rows allow (16, 8, 4; 2 for 16-bit types).
+// N values of this lane's row into the staging block, from part `part` on.
 template <typename T, int RB, int N>
-__device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows, int cols, int width,
-                                     const float (&v)[N], int lane) {
-  constexpr int kParts = RB / 16, kPart = 16 / sizeof(T), kCols = RB / sizeof(T);
-  static_assert(N % kCols == 0, "whole staging rows");
+__device__ __forceinline__ void stage_put(uint32_t buf, int part, const float* v, int lane) {
+  constexpr int kPart = 16 / sizeof(T);
 #pragma unroll
-  for (int h = 0; h < N / kCols; ++h) {
+  for (int c = 0; c < N / kPart; ++c)
+    sts16(stage_at<RB>(buf, lane, part + c), pack16<T>(v + c * kPart));
+}
+// The staging block to out[row * ld + column], rows and cols of it.  width: the
+// bytes of an access that its rows allow (16, 8, 4; 2 for 16-bit types).
+template <typename T, int RB>
+__device__ __forceinline__ void stage_out(uint32_t buf, T* out, int64_t ld, int rows, int cols,
+                                          int width, int lane) {
+  constexpr int kPart = 16 / sizeof(T), kCols = RB / sizeof(T);
+  __syncwarp();
+  if (cols >= kCols && width >= 4) {
+    if (width == 16) copy_out<T, RB, 16>(buf, out, ld, rows, lane);
+    else if (width == 8) copy_out<T, RB, 8>(buf, out, ld, rows, lane);
+    else copy_out<T, RB, 4>(buf, out, ld, rows, lane);
+  } else {
+    // A column a lane, a row after the other.
 #pragma unroll
-    for (int c = 0; c < kParts; ++c)
-      sts16(stage_at<RB>(buf, lane, c), pack16<T>(v + h * kCols + c * kPart));
-    __syncwarp();
-    T* out = base + h * kCols;
-    const int left = cols - h * kCols;
-    if (left >= kCols && width >= 4) {
-      if (width == 16) copy_out<T, RB, 16>(buf, out, ld, rows, lane);
-      else if (width == 8) copy_out<T, RB, 8>(buf, out, ld, rows, lane);
-      else copy_out<T, RB, 4>(buf, out, ld, rows, lane);
-    } else {
-      // A column a lane, a row after the other.
-#pragma unroll
-      for (int c0 = 0; c0 < kCols; c0 += 32) {
-        const int col = c0 + lane;
-        if (col < left) {
+    for (int c0 = 0; c0 < kCols; c0 += 32) {
+      const int col = c0 + lane;
+      if (col < cols) {
 #pragma unroll 8
-          for (int r = 0; r < rows; ++r) {
-            const uint32_t a = stage_at<RB>(buf, r, col / kPart) + (col % kPart) * sizeof(T);
-            if constexpr (sizeof(T) == 4) {
-              float f;
-              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
-              out[r * ld + col] = f;
-            } else {
-              uint16_t b;
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(a) : "memory");
-              reinterpret_cast<uint16_t*>(out)[r * ld + col] = b;
-            }
+        for (int r = 0; r < rows; ++r) {
+          const uint32_t a = stage_at<RB>(buf, r, col / kPart) + (col % kPart) * sizeof(T);
+          if constexpr (sizeof(T) == 4) {
+            float f;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+            out[r * ld + col] = f;
+          } else {
+            uint16_t b;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(a) : "memory");
+            reinterpret_cast<uint16_t*>(out)[r * ld + col] = b;
           }
         }
       }
     }
-    __syncwarp();
+  }
+  __syncwarp();
+}
+// Writes v (this lane's row) to base[row * ld + column], a staging block at a time.
+template <typename T, int RB, int N>
+__device__ __forceinline__ void emit(uint32_t buf, T* base, int64_t ld, int rows, int cols, int width,
+                                     const float (&v)[N], int lane) {
+  constexpr int kCols = RB / sizeof(T);
+  static_assert(N % kCols == 0, "whole staging rows");
+#pragma unroll
+  for (int h = 0; h < N / kCols; ++h) {
+    stage_put<T, RB, kCols>(buf, 0, v + h * kCols, lane);
+    stage_out<T, RB>(buf, base + h * kCols, ld, rows, cols - h * kCols, width, lane);
   }
 }
 
@@ -654,10 +664,10 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
       Incoming<T, RB> in;
       // (float32 has no registers for it while it drains.)
       if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, limit32(cols), lane);
-      // Finishes kStep columns from `at` on: v the sums (gated: the gate's; up() then
-      // gives the up's, late, so that both are not held longer than needed).
+      // Finishes kStep columns from `at` on: v the sums (gated: the gate's; up(h, u)
+      // then gives the up's, 32 at a time, since not all are held at once).
       auto finish = [&](int at, Step& v, auto&& up) {
-        const int n = (int)min((int64_t)kStep, cols - at);
+        const int n = limit32(cols - at);
         const int64_t col = warp_col + at;
         if (p.splits > 1) {
           constexpr int kPlanes = MODE == kGated ? 2 : 1;
@@ -667,31 +677,42 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           // (ldp covers whole steps.)
           if (n > 0) emit<float, RB>(buf, dst, p.ldp, rows, kStep, 16, v, lane);
           if constexpr (MODE == kGated) {
-            up(v);
-            if (n > 0)
-              emit<float, RB>(buf, dst + p.rows * p.ldp, p.ldp, rows, kStep, 16, v, lane);
+#pragma unroll
+            for (int h = 0; h < kStep / 32; ++h) {
+              float u[32];
+              up(h, u);
+              if (n > 0)
+                emit<float, RB>(buf, dst + p.rows * p.ldp + h * 32, p.ldp, rows, 32, 16, u, lane);
+            }
           }
           return;
         }
-        // Bias and the saved pre-activation of the first or second sums.
-        auto affine = [&](int which, Step& x) {
-          const T* b = static_cast<const T*>(p.bias[which]);
-          add_bias(b ? b + col : b, n, p.bias_vec != 0, x);
-          if (p.save[which] && n > 0)
-            emit<T, RB>(buf, static_cast<T*>(p.save[which]) + row0 * p.lds + col, p.lds, rows, n,
-                        p.vec, x, lane);
-        };
         if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, n, lane);
+        const bool vec = p.bias_vec != 0;
+        auto biases = [&](int which) {
+          const T* b = static_cast<const T*>(p.bias[which]);
+          return b ? b + col : b;
+        };
+        auto saved = [&](int which) {
+          return static_cast<T*>(p.save[which]) + row0 * p.lds + col;
+        };
         if constexpr (MODE == kLinear || MODE == kGated) {
-          affine(0, v);
+          add_bias(biases(0), n, vec, v);
+          if (p.save[0] && n > 0) emit<T, RB>(buf, saved(0), p.lds, rows, n, p.vec, v, lane);
           activate_all<T>(p.act, v);
         }
         if constexpr (MODE == kGated) {
-          Step u;
-          up(u);
-          affine(1, u);
 #pragma unroll
-          for (int j = 0; j < kStep; ++j) v[j] *= u[j];
+          for (int h = 0; h < kStep / 32; ++h) {
+            float u[32];
+            up(h, u);
+            const T* b = biases(1);
+            add_bias(b ? b + h * 32 : b, n - h * 32, vec, u);
+            if (p.save[1]) stage_put<T, RB, 32>(buf, h * 32 * (int)sizeof(T) / 16, u, lane);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[h * 32 + j] *= u[j];
+          }
+          if (p.save[1]) stage_out<T, RB>(buf, saved(1), p.lds, rows, n, p.vec, lane);
         }
         if (MODE == kLinear && res && n > 0) {
           in.add(buf, v, lane);
@@ -705,15 +726,16 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
       if constexpr (P == 1) {
         const uint32_t acc = tile & 1, t = tmem_base + acc * BN + lanes;
         if (!wait_acc(acc, (tile >> 1) & 1)) break;
-        // kStep sums; the accumulator is freed with its last ones.
-        auto take = [&](int which, int at, Step& v) {
-          uint32_t raw[kStep / 32][32];
+        // N sums; the accumulator is freed with its last ones.
+        auto take = [&](int which, int at, auto& v) {
+          constexpr int N = sizeof(v) / 4;
+          uint32_t raw[N / 32][32];
 #pragma unroll
-          for (int c = 0; c < kStep / 32; ++c) tmem_ld32(t + acc_col(which, at + c * 32), raw[c]);
+          for (int c = 0; c < N / 32; ++c) tmem_ld32(t + acc_col(which, at + c * 32), raw[c]);
           tmem_wait_ld();
-          if (which == (MODE == kGated ? 1 : 0) && at + kStep == kOutCols) release_acc(acc);
+          if (which == (MODE == kGated ? 1 : 0) && at + N == kOutCols) release_acc(acc);
 #pragma unroll
-          for (int c = 0; c < kStep / 32; ++c)
+          for (int c = 0; c < N / 32; ++c)
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[c * 32 + j] = __uint_as_float(raw[c][j]);
         };
@@ -721,7 +743,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
         for (int at = 0; at < kOutCols; at += kStep) {
           Step v;
           take(0, at, v);
-          finish(at, v, [&](Step& u) { take(1, at, u); });
+          finish(at, v, [&](int h, float (&u)[32]) { take(1, at + h * 32, u); });
         }
       } else {
         // 32 sums at a time: the output columns' (gated: a gate's 32, then the up's).
@@ -755,7 +777,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
         // others up: unrolled, its addresses alone made the sums spill.
 #pragma unroll 1
         for (int at = 0; at < kOutCols; at += kStep) {
-          finish(at, sum[0], [&](Step& u) {
+          finish(at, sum[0], [&](int, float (&u)[32]) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) u[j] = sum[kPer - 1][j];
           });
