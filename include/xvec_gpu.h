@@ -571,7 +571,7 @@ xvec_gpu_status xvec_gpu_rotate_device(int32_t device, const uint8_t* signs, int
  * elements exactly; the matrix units add them up in float32, truncating.
  * float32 storage multiplies three bfloat16 parts of each element (all
  * products above 2^-24 of the whole) and adds most sums in registers, so that
- * float32 results have float32 accuracy (2-norm errors of 1e-7 to 3e-7), but an
+ * float32 results have float32 accuracy (2-norm errors of 1e-7 to 4e-7), but an
  * infinity in a float32 operand may come out as a NaN, and elements below
  * 2^-109 are held to 2^-134.  Gradients of pre-activations are rounded to
  * 16 bits in between for 16-bit storage.  Results do not vary from run to run

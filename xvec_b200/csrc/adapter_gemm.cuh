@@ -30,10 +30,12 @@
 // (what is left out is below 2^-24 of the product).  The accumulator's own
 // additions truncate (measured: 48 of them leave 1.1e-6 of the 2-norm at depth
 // 960), so hh has an accumulator of its own that leaves tensor memory every
-// kRound blocks to be added in registers (8 truncations instead of 48), and the
-// five products that are 2^8 times smaller have another that leaves at the end.
-// hh is drained while the small products of the same block are issued, so one
-// accumulator of each suffices and the tile can keep 256 columns.
+// kRound blocks to be added in registers (8 truncations; 32 in a tile's first
+// round), and the five products that are 2^8 times smaller have another that leaves
+// at the end.  hh is drained while the small products of the same block are issued,
+// so one accumulator of each suffices and the tile can keep 256 columns.  The planes come
+// in the order m, h, l: m's stage is free after two thirds of the products, and the
+// next block's first copy starts that much sooner (the ring holds two blocks).
 // The drained sums take the registers that the other warps give up (setmaxnreg).
 //
 // Every mbarrier wait is bounded; on expiry the kernel sets *status, stops
@@ -57,7 +59,13 @@ constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr int kBand = 8;      // row tiles per band of the tile order
 constexpr int kFewRegs = 56, kManyRegs = 224;
-constexpr int kRound = 2;     // float32: depth blocks per accumulation in tensor memory
+// float32: depth blocks per accumulation in tensor memory.  A tile's first one is
+// longer: so far the product runs ahead while the tile before is finished.
+constexpr int kFirstRound = 8, kRound = 2;
+// Whether block `k` of a tile begins an accumulation.
+__host__ __device__ constexpr bool opens_round(int k) {
+  return k == 0 || (k >= kFirstRound && (k - kFirstRound) % kRound == 0);
+}
 
 template <int MODE, typename T, bool PAIR, int BN>
 struct GemmShape {
@@ -523,7 +531,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
             const uint32_t at = tiles_at + stage * S::kStageBytes, bar = bars + stage * 8;
             const uint32_t blocks = min(n, S::kUnits);
             if (issuer) expect_bytes(full_at + stage * 8, (PAIR ? 2 : 1) * blocks * S::kBlockBytes);
-            load(bar, at, pl);
+            load(bar, at, P == 1 ? 0 : pl == 0 ? 1 : pl == 1 ? 0 : 2);
             if constexpr (P == 1) {
               if ((k += kBK) == k_end) k = 0, ++seg;
               if (blocks > 1) {
@@ -585,26 +593,27 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
         } else {
           const uint32_t d = tmem_base, small = tmem_base + BN;
           for (int k = it.k0; k < it.k1; ++k) {
-            const bool opens = (k - it.k0) % kRound == 0;
-            const bool closes = (k - it.k0) % kRound == kRound - 1 || k + 1 == it.k1;
+            const bool opens = opens_round(k - it.k0);
+            const bool closes = k + 1 == it.k1 || opens_round(k + 1 - it.k0);
             uint32_t h, m, l;
+            if (k == it.k0 && !(ok = wait_bar(tempty_at + 8, (tile & 1) ^ 1, s_abort, limit))) break;
+            if (!(ok = next(&m))) break;
+            multiply(m, m, small, k > it.k0);
             if (opens) {
               if (!(ok = wait_bar(tempty_at, (round & 1) ^ 1, s_abort, limit))) break;
+              tmem_fence_after();
               ++round;
             }
             if (!(ok = next(&h))) break;
             multiply(h, h, d, !opens);
             if (closes) commit<PAIR>(tfull_at);
-            if (k == it.k0 && !(ok = wait_bar(tempty_at + 8, (tile & 1) ^ 1, s_abort, limit))) break;
-            if (!(ok = next(&m))) break;
-            multiply(m, m, small, k > it.k0);
             multiply(h, m, small, 1);
             multiply(m, h, small, 1);
+            commit<PAIR>(empty_at + m * 8);
             if (!(ok = next(&l))) break;
             multiply(h, l, small, 1);
             multiply(l, h, small, 1);
             commit<PAIR>(empty_at + h * 8);
-            commit<PAIR>(empty_at + m * 8);
             commit<PAIR>(empty_at + l * 8);
           }
           commit<PAIR>(tfull_at + 8);
@@ -763,7 +772,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           }
         };
         bool ok = true;
-        for (int k = it.k0; k < it.k1 && ok; k += kRound, ++round) {
+        for (int k = it.k0; k < it.k1 && ok; k += k == it.k0 ? kFirstRound : kRound, ++round) {
           if (!(ok = wait_acc(0, round & 1))) break;
           drain(tmem_base, k == it.k0);
           release_acc(0);
