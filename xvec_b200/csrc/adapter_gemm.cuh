@@ -341,6 +341,9 @@ struct Incoming {
     return p < end ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
   }
   __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, int cols, int lane) {
+    // Without columns the row's address may lie past the matrix, and the granule
+    // that it falls into with it.
+    if (cols <= 0) rows = 0;
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
       const int r = i * (32 / kParts) + lane / kParts;
