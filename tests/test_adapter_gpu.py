@@ -620,6 +620,45 @@ def test_queries_through_two_layers_without_waiting(xb):
         assert torch.equal(a, got)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_gradients_through_many_layers_without_waiting(xb, kind):
+    """Backward calls that follow one another without a wait: each reads the dx that the one before
+    wrote, while that one's weight gradients may still be under way; all results as with a wait after
+    every call."""
+    k, layers = 160, 24
+    mk = Maker(kind, 13)
+    ws = [mk.matrix(k, k, k ** -0.5).contiguous() for _ in range(3)]
+    for n in (5, 130, 1500):
+        x, z, dy = mk.matrix(n, k).contiguous(), mk.matrix(n, k).contiguous(), mk.matrix(n, k).contiguous()
+
+        def run(wait):
+            d, outs = dy.clone(), []
+            for i in range(layers):
+                w = ws[i % 3]
+                dx, dw, dw2 = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+                db = torch.empty(k, device="cuda", dtype=x.dtype)
+                if i % 2:
+                    xb.linear_backward_device(0, STORAGE[kind], n, k, k, ptr(d), ptr(x), ptr(w),
+                                              preact_ptr=ptr(z), activation=xb.ACT_GELU,
+                                              dx_ptr=ptr(dx), dw_ptr=ptr(dw), db_ptr=ptr(db),
+                                              stream=stream())
+                    outs += [dx, dw, db]
+                else:
+                    xb.gated_backward_device(0, STORAGE[kind], n, k, k, ptr(d), ptr(x), ptr(w), ptr(ws[2]),
+                                             ptr(z), ptr(x), dx_ptr=ptr(dx), dgate_weight_ptr=ptr(dw),
+                                             dup_weight_ptr=ptr(dw2), stream=stream())
+                    outs += [dx, dw, dw2]
+                if wait:
+                    torch.cuda.synchronize()
+                d = dx
+            torch.cuda.synchronize()
+            return outs
+
+        want = run(True)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(run(False), want))
+
+
 def test_gradients_against_differences(xb):
     """The gradients are the slopes of the forward pass itself: central differences of a float32
     adapter along random directions.  f(t) = <c, y(t)> in float64 of float32 outputs: rounding leaves

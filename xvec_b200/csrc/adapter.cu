@@ -735,8 +735,7 @@ xvec_gpu_status run_backward(const Backward& b) {
   }
   if (b.dx && (st = plan_gemm(b.storage, &dx))) return st;
   if (dw.p.batches && (st = plan_gemm(b.storage, &dw))) return st;
-  // (One after the other: they can share the place for split sums.)
-  const size_t partial_at = arena.add(std::max(dx.partial_bytes, dw.partial_bytes));
+  const size_t dx_partial = arena.add(dx.partial_bytes), dw_partial = arena.add(dw.partial_bytes);
 
   if ((st = arena.alloc(s))) return st;
   Packs packs;
@@ -760,7 +759,7 @@ xvec_gpu_status run_backward(const Backward& b) {
   if (b.dx) {
     dx.a = grad;
     dx.b[0] = w[0].g, dx.b[1] = w[1].g;
-    if (dx.partial_bytes) dx.p.partial = static_cast<float*>(arena.at(partial_at));
+    if (dx.partial_bytes) dx.p.partial = static_cast<float*>(arena.at(dx_partial));
     if ((st = gemm(b.storage, dx, s))) return st;
   }
   if (dw.p.batches) {
@@ -770,7 +769,9 @@ xvec_gpu_status run_backward(const Backward& b) {
       dw.a.planes = planes_of(b.storage);
     }
     dw.b[0] = x.g;
-    if (dw.partial_bytes) dw.p.partial = static_cast<float*>(arena.at(partial_at));
+    if (dw.partial_bytes) dw.p.partial = static_cast<float*>(arena.at(dw_partial));
+    // Directly after dx's product, whose inputs were complete when it began.
+    dw.p.beside = b.dx && !dx.partial_bytes;
     if ((st = gemm(b.storage, dw, s))) return st;
   }
   return XVEC_GPU_OK;

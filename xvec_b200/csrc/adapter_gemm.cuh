@@ -463,7 +463,8 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
     }
     tmem_fence_before();
   }
-  pdl_begin();
+  if (p.beside) pdl_launch();  // (all it reads comes through TMA, from L2)
+  else pdl_begin();
   __syncthreads();
   if constexpr (PAIR) cluster_sync_all();
   tmem_fence_after();
@@ -823,6 +824,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
       }
     }
   }
+  if (p.beside) pdl_wait();
   if constexpr (PAIR) cluster_sync_all();
   if (warp == 1) {
     tmem_fence_after();
