@@ -94,6 +94,24 @@ def test_squares_that_leave_float32(xb, kind, big):
         close(o, t.double() / 4, 2.0 ** -19 * t.double().abs(), "clipped")
 
 
+@pytest.mark.parametrize("limit", [1.0, 1e-3, 1e-12, 1e-30])
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_factors_below_float32(xb, kind, limit):
+    """Gradients near the type's largest value and a small limit: the factor itself may lie below
+    float32's normal numbers, the results do not.  The bound is test_clip's: the norm within 2^-20,
+    two roundings more, and half a step of the type."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    sign = torch.randint(0, 2, (2051,), generator=g, device="cuda") * 2 - 1
+    x = ((1 + torch.rand(2051, generator=g, device="cuda")) * 1e38 * sign).to(TYPES[kind])
+    # The norm alone leaves float32 here and is written as infinity; the factor is finite.
+    scale = limit / math.sqrt(x.double().square().sum().item())
+    for out in (torch.full_like(x, SENTINEL), x.clone()):
+        source = out if out[0] == x[0] else x
+        want = x.double() * scale
+        clip(xb, [source], limit, [out])
+        close(out, want, 2.0 ** -19 * want.abs(), "clipped")
+
+
 def test_one_large_value_among_small_ones(xb):
     t = torch.full((300_000,), 1e-21, device="cuda")
     t[123_456] = 2e-20

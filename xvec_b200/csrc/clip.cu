@@ -14,6 +14,7 @@
 // 1e19, and what is not finite) is squared in float64, so that neither overflow
 // nor underflow of a square matters.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <new>
 
@@ -166,6 +167,14 @@ __device__ __forceinline__ void scale_range(const T* in, T* out, int64_t i0, int
   if (e < i1) out[e] = from_f<T>(to_f(in[e]) * f);
 }
 
+// The same by a factor that float32 cannot hold to its full precision.
+template <typename T>
+__device__ __noinline__ void scale_range_tiny(const T* in, T* out, int64_t i0, int64_t i1,
+                                              double f) {
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads)
+    out[i] = from_f<T>((float)(to_f(in[i]) * f));
+}
+
 // sums[block] = the sum of squares of the block's chunks.
 template <int N>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
@@ -196,7 +205,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   for (int i = threadIdx.x; i < num_sums; i += kThreads) s += sums[i];
   const double n = sqrt(block_sum(s));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-  const float f = isfinite(n) && n > max_norm ? (float)(max_norm / n) : 1.f;
+  const double factor = isfinite(n) && n > max_norm ? max_norm / n : 1.0;
+  const float f = (float)factor;
+  // Below float32's normal numbers the factor loses bits, down to zero, while its
+  // product with gradients near 1e38 is an ordinary number: float64 there, and
+  // nothing to gain from speed.  (float16 values times such a factor are zeros.)
+  const bool tiny = factor > 0 && factor < FLT_MIN;
   if (blockIdx.x >= t.chunks) return;
   for (uint32_t c = blockIdx.x + (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x;;
        c -= gridDim.x) {
@@ -204,7 +218,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     if (f != 1.f || e.in != e.out) {
       const int64_t i0 = (int64_t)(c - e.first_chunk) * chunk_elems(e.storage);
       const int64_t i1 = min(e.count, i0 + chunk_elems(e.storage));
-      if (e.storage == XVEC_STORAGE_FP32)
+      if (tiny && e.storage == XVEC_STORAGE_FP32)
+        scale_range_tiny(static_cast<const float*>(e.in), static_cast<float*>(e.out), i0, i1,
+                         factor);
+      else if (tiny && e.storage == XVEC_STORAGE_BF16)
+        scale_range_tiny(static_cast<const bf16*>(e.in), static_cast<bf16*>(e.out), i0, i1, factor);
+      else if (e.storage == XVEC_STORAGE_FP32)
         scale_range(static_cast<const float*>(e.in), static_cast<float*>(e.out), i0, i1, f);
       else if (e.storage == XVEC_STORAGE_FP16)
         scale_range(static_cast<const __half*>(e.in), static_cast<__half*>(e.out), i0, i1, f);
