@@ -67,18 +67,28 @@ template <typename T, bool VEC>
 __device__ __forceinline__ void pack_rows(const Pack& p, int64_t thread, int64_t threads) {
   const T* src = static_cast<const T*>(p.src);
   const int64_t groups = p.ld / 8, total = groups * p.rows;
-#pragma unroll 2
-  for (int64_t i = thread; i < total; i += threads) {
-    // (64-bit divisions would cost more than the copy.)
-    const int64_t r = total >> 32 ? i / groups : (uint32_t)i / (uint32_t)groups;
-    const int c = (int)(i - r * groups) * 8;
-    Eight<T, VEC> e;
-    e.load(src + r * p.lds + c, p.cols - c);
-    e.settle();
-    float v[8];
+  constexpr int kAhead = 2;  // groups requested before the first is stored
+  for (int64_t i0 = thread; i0 < total; i0 += kAhead * threads) {
+    Eight<T, VEC> e[kAhead];
+    int64_t r[kAhead];
+    int c[kAhead];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < p.cols ? e[j] : 0.f;
-    store_operand<T>(static_cast<uint16_t*>(p.dst) + r * p.ld + c, p.rows * p.ld, v);
+    for (int a = 0; a < kAhead; ++a) {
+      const int64_t i = i0 + a * threads < total ? i0 + a * threads : i0;
+      // (64-bit divisions would cost more than the copy.)
+      r[a] = total >> 32 ? i / groups : (uint32_t)i / (uint32_t)groups;
+      c[a] = (int)(i - r[a] * groups) * 8;
+      e[a].load(src + r[a] * p.lds + c[a], p.cols - c[a]);
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      if (i0 + a * threads >= total) break;
+      e[a].settle();
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c[a] + j < p.cols ? e[a][j] : 0.f;
+      store_operand<T>(static_cast<uint16_t*>(p.dst) + r[a] * p.ld + c[a], p.rows * p.ld, v);
+    }
   }
 }
 template <typename T>

@@ -152,9 +152,12 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, uint32_
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// The 16-byte granule at p, if it starts before `end`.
+// The 16-byte granule at p, if it starts before `end`.  A plain load, as everywhere in
+// these kernels: they are resident before the launch that writes their inputs has
+// completed (pdl_wait), and a non-coherent load needs memory that does not change
+// while its kernel runs.
 __device__ __forceinline__ uint4 granule(uintptr_t p, uintptr_t end) {
-  return p < end ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+  return p < end ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
 }
 
 // Eight elements of a row, of which `count` exist (what the others hold is of no

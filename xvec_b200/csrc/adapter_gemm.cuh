@@ -336,10 +336,6 @@ struct Incoming {
   uint4 v[kParts], last;
   uint32_t off;  // of this lane's row
 
-  // (A plain load: the residual may be the output itself.)
-  static __device__ __forceinline__ uint4 granule(uintptr_t p, uintptr_t end) {
-    return p < end ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-  }
   __device__ __forceinline__ void start(const T* base, int64_t ld, int rows, int cols, int lane) {
     // Without columns the row's address may lie past the matrix, and the granule
     // that it falls into with it.
@@ -381,7 +377,7 @@ __device__ __forceinline__ void add_bias(const T* bias, int cols, bool vec, floa
   if (vec && cols >= N) {
 #pragma unroll
     for (int c = 0; c < N * (int)sizeof(T) / 16; ++c) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(bias) + c);
+      const uint4 u = reinterpret_cast<const uint4*>(bias)[c];
       const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
       for (int j = 0; j < 16 / (int)sizeof(T); ++j) x[c * (16 / sizeof(T)) + j] += to_f(t[j]);

@@ -113,14 +113,13 @@ __device__ __forceinline__ double square_range(const T* in, int64_t i0, int64_t 
   double s0 = 0, s1 = 0;
   int i = threadIdx.x;
   for (; i + 3 * kThreads < vectors; i += 4 * kThreads) {
-    const uint4 a = __ldg(p + i), b = __ldg(p + i + kThreads);
-    const uint4 c = __ldg(p + i + 2 * kThreads), d = __ldg(p + i + 3 * kThreads);
+    const uint4 a = p[i], b = p[i + kThreads], c = p[i + 2 * kThreads], d = p[i + 3 * kThreads];
     s0 += vector_squares<T>(a);
     s1 += vector_squares<T>(b);
     s0 += vector_squares<T>(c);
     s1 += vector_squares<T>(d);
   }
-  for (; i < vectors; i += kThreads) s0 += vector_squares<T>(__ldg(p + i));
+  for (; i < vectors; i += kThreads) s0 += vector_squares<T>(p[i]);
   const int64_t tail = head + (int64_t)vectors * N;
   const int64_t e = threadIdx.x < head - i0 ? i0 + threadIdx.x : tail + threadIdx.x - (head - i0);
   if (e < i1) {
