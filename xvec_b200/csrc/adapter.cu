@@ -177,7 +177,7 @@ xvec_gpu_status forward(int storage, GemmCall& g, Operand* a, Operand* b0, Opera
                         cudaStream_t s) {
   xvec_gpu_status st = plan_gemm(storage, &g);
   if (st) return st;
-  const size_t partial = arena.add(g.partial_bytes);
+  const size_t partial = arena.add(g.partial_bytes), runs = arena.add(g.run_bytes);
   if ((st = arena.alloc(s))) return st;
   Packs packs;
   place(a, arena, &packs);
@@ -187,6 +187,7 @@ xvec_gpu_status forward(int storage, GemmCall& g, Operand* a, Operand* b0, Opera
   g.a = a->g, g.b[0] = b0->g;
   if (b1) g.b[1] = b1->g;
   if (g.partial_bytes) g.p.partial = static_cast<float*>(arena.at(partial));
+  if (g.run_bytes) g.p.runs = static_cast<float*>(arena.at(runs));
   return gemm(storage, g, s);
 }
 
@@ -549,6 +550,10 @@ xvec_gpu_status plan_gemm(int storage, GemmCall* c) {
   }
   c->partial_bytes =
       p.splits > 1 ? (size_t)p.splits * p.batches * half * p.rows * p.ldp * 4 : 0;
+  // 128 rows of accumulator columns for each CTA.
+  c->run_bytes = storage == XVEC_STORAGE_FP32 && p.blocks_per_split > run_blocks(true)
+                     ? (size_t)c->sms * kTileShapes[c->shape].cols * 128 * 4
+                     : 0;
   return XVEC_GPU_OK;
 }
 
@@ -792,6 +797,7 @@ xvec_gpu_status run_backward(const Backward& b) {
   if (b.dx && (st = plan_gemm(b.storage, &dx))) return st;
   if (dw.p.batches && (st = plan_gemm(b.storage, &dw))) return st;
   const size_t dx_partial = arena.add(dx.partial_bytes), dw_partial = arena.add(dw.partial_bytes);
+  const size_t dx_runs = arena.add(dx.run_bytes), dw_runs = arena.add(dw.run_bytes);
 
   if ((st = arena.alloc(s))) return st;
   Packs packs;
@@ -817,6 +823,7 @@ xvec_gpu_status run_backward(const Backward& b) {
     dx.a = grad;
     dx.b[0] = w[0].g, dx.b[1] = w[1].g;
     if (dx.partial_bytes) dx.p.partial = static_cast<float*>(arena.at(dx_partial));
+    if (dx.run_bytes) dx.p.runs = static_cast<float*>(arena.at(dx_runs));
     if ((st = gemm(b.storage, dx, s))) return st;
   }
   if (dw.p.batches) {
@@ -827,6 +834,7 @@ xvec_gpu_status run_backward(const Backward& b) {
     }
     dw.b[0] = x.g;
     if (dw.partial_bytes) dw.p.partial = static_cast<float*>(arena.at(dw_partial));
+    if (dw.run_bytes) dw.p.runs = static_cast<float*>(arena.at(dw_runs));
     // Directly after dx's product, whose inputs were complete when it began.
     dw.p.beside = b.dx && !dx.partial_bytes;
     if ((st = gemm(b.storage, dw, s))) return st;

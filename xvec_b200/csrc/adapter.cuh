@@ -248,6 +248,7 @@ struct GemmParams {
   int splits, blocks_per_split;  // of the segs * blocks depth blocks
   float* partial;        // splits > 1: [splits][batches or halves][rows][ldp] float sums
   int64_t ldp;
+  float* runs;           // float32, long sums: those of finished runs, by thread
   uint32_t idesc;
   int vec;               // bytes of an access that outputs and saves allow
   int bias_vec;          // the biases allow 16
@@ -288,7 +289,11 @@ struct GemmCall {
   int device = 0, sms = 0;    // (plan_gemm)
   int shape = 0;              // of the tiles (plan_gemm)
   size_t partial_bytes = 0;   // scratch for split sums, at p.partial
+  size_t run_bytes = 0;       // scratch for float32's long sums, at p.runs
 };
+// Depth blocks of 64 that one accumulation takes (adapter_gemm.cuh): 16-bit storage 2048
+// terms, float32 4096 (whose large products leave the accumulator far more often).
+constexpr int run_blocks(bool float32) { return float32 ? 64 : 32; }
 constexpr int kShapes = 4;
 struct TileShape {
   int rows, cols;  // cols: of the accumulator (half as many outputs when gated)
@@ -296,7 +301,7 @@ struct TileShape {
 };
 constexpr TileShape kTileShapes[kShapes] = {
     {256, 256, true}, {256, 192, true}, {256, 128, true}, {128, 128, false}};
-// Picks the tiles and splits: fills in c's tiling and partial_bytes.
+// Picks the tiles and splits: fills in c's tiling and its scratch.
 xvec_gpu_status plan_gemm(int storage, GemmCall* c);
 // The number of SMs of a device.
 xvec_gpu_status count_sms(int device, int* sms);

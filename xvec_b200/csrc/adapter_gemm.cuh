@@ -38,6 +38,16 @@
 // next block's first copy starts that much sooner (the ring holds two blocks).
 // The drained sums take the registers that the other warps give up (setmaxnreg).
 //
+// LONG: sums of more than kRun blocks (2048 terms, float32 4096) are taken in runs of
+// that many, each in fresh accumulators.  Truncation always points to zero: over 131072 terms of
+// one sign a single 16-bit accumulator lost 8.4e-4 of the sum (1e-7 for each of its
+// 8192 additions; binary16's half step is 4.9e-4).  16-bit types then hold a
+// tile's sums in registers, as float32 does, where the runs are added in float32
+// (linear backward 16384 x 2048 -> 1024 bf16 118 -> 121 us with runs of 2048 or 4096).
+// float32's small products need runs as well (262144 terms of either sign: 3.7e-6 of
+// the 2-norm without); its registers are added up in a scratch of the epilogue's own,
+// each thread reading back what it wrote itself, so that no sum has many terms.
+//
 // Every mbarrier wait is bounded; on expiry the kernel sets *status, stops
 // issuing work, drains its own copies and frees its tensor memory.
 #pragma once
@@ -58,16 +68,19 @@ constexpr int kBM = 128;      // rows per CTA (TMEM lanes)
 constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr int kBand = 8;      // row tiles per band of the tile order
-constexpr int kFewRegs = 56, kManyRegs = 224;
+// Registers of a thread where sums are held: of the first four warps, and of the epilogue's.
+constexpr int kFewRegs = 56;
+template <typename T>
+constexpr int kManyRegs = std::is_same<T, float>::value ? 224 : 216;
 // float32: depth blocks per accumulation in tensor memory.  A tile's first one is
 // longer: so far the product runs ahead while the tile before is finished.
 constexpr int kFirstRound = 8, kRound = 2;
-// Whether block `k` of a tile begins an accumulation.
+// Whether block `k` of a run begins an accumulation.
 __host__ __device__ constexpr bool opens_round(int k) {
   return k == 0 || (k >= kFirstRound && (k - kFirstRound) % kRound == 0);
 }
 
-template <int MODE, typename T, bool PAIR, int BN>
+template <int MODE, typename T, bool PAIR, int BN, bool LONG>
 struct GemmShape {
   // Two epilogue warps per TMEM lane quarter, one per half of the columns.  (Four
   // on 256 columns cost a stage of the ring and were slower: 131072 x 1024 -> 1024
@@ -80,12 +93,16 @@ struct GemmShape {
   // stage's handshake takes its single threads about 350 clocks, one block's
   // instructions 512 or less.
   static constexpr int kUnits = std::is_same<T, float>::value ? 1 : 2;
+  static constexpr int kRun = run_blocks(std::is_same<T, float>::value);
+  static_assert(kRun % kUnits == 0, "a stage belongs to one run");
   static constexpr uint32_t kBlockBytes = kABytes + kBBytes;
   static constexpr uint32_t kStageBytes = kUnits * kBlockBytes;
   // Columns that an epilogue warp finishes at a time, and their staging block of 32
   // rows: 128 bytes a row where its columns come in 64s (or 32 float32), else 64.
   static constexpr int kOutCols = BN / 2 / (MODE == kGated ? 2 : 1);  // outputs of a warp
-  static constexpr int kStep = sizeof(T) == 2 && kOutCols % 64 == 0 ? 64 : 32;
+  // Sums are held in registers (else read from tensor memory as they are finished).
+  static constexpr bool kHold = std::is_same<T, float>::value || LONG;
+  static constexpr int kStep = sizeof(T) == 2 && !kHold && kOutCols % 64 == 0 ? 64 : 32;
   static constexpr int kRowBytes = kStep * sizeof(T);
   static constexpr uint32_t kEpiBytes = kEpiWarps * 32 * kRowBytes;
   static constexpr int kFit = (int)((232448 - 1024 - 512 - kEpiBytes) / kStageBytes);
@@ -390,12 +407,12 @@ __device__ __forceinline__ void add_bias(const T* bias, int cols, bool vec, floa
 }
 
 // --- the kernel ---------------------------------------------------------------
-template <int MODE, typename T, bool PAIR, int BN>
-__global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
+template <int MODE, typename T, bool PAIR, int BN, bool LONG>
+__global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN, LONG>::kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap0,
                 const __grid_constant__ CUtensorMap bmap1, const __grid_constant__ GemmParams p) {
   using namespace tc;
-  using S = GemmShape<MODE, T, PAIR, BN>;
+  using S = GemmShape<MODE, T, PAIR, BN, LONG>;
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   constexpr int P = std::is_same<T, float>::value ? 3 : 1;  // planes
   constexpr int kStages = S::kStages, kEpiWarps = S::kEpiWarps;
@@ -485,9 +502,9 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
     return it;
   };
 
-  // float32: 384 threads of 168 registers become 128 of kFewRegs and 256 of kManyRegs.
+  // Held sums: 384 threads of 168 registers become 128 of kFewRegs and 256 of kManyRegs.
   if (warp < 4) {
-    if constexpr (P == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    if constexpr (S::kHold) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
     if (warp == 0 && lane == 0) {
       // ---------------- TMA producer ----------------
       const uint32_t tiles_at = smem_u32(tiles), empty_at = smem_u32(empty);
@@ -575,30 +592,30 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           mma_16bit<PAIR>(d, a + k * kDepthStep<A_MN>, b + k * kDepthStep<B_MN>, p.idesc,
                           k == 0 ? keep : 1u);
       };
-      uint32_t round = 0, tile = 0;
-      for (int i = worker; i < items && ok; i += workers, ++tile) {
-        const Item it = item_of(i);
+      uint32_t round = 0, run = 0;
+      // The product of blocks [k0, k1), one run (or a whole tile).
+      auto multiply_run = [&](int k0, int k1) {
         if constexpr (P == 1) {
-          const uint32_t acc = tile & 1, d = tmem_base + acc * BN;
-          if (!(ok = wait_bar(tempty_at + acc * 8, ((tile >> 1) & 1) ^ 1, s_abort, limit))) break;
+          const uint32_t acc = run & 1, d = tmem_base + acc * BN;
+          if (!(ok = wait_bar(tempty_at + acc * 8, ((run >> 1) & 1) ^ 1, s_abort, limit))) return;
           tmem_fence_after();
-          for (int k = it.k0; k < it.k1; k += S::kUnits) {
+          for (int k = k0; k < k1; k += S::kUnits) {
             uint32_t at;
             if (!(ok = next(&at))) break;
-            multiply(at, at, d, k > it.k0);
-            if (k + 1 < it.k1) multiply(at, at, d, 1, S::kBlockBytes >> 4);
+            multiply(at, at, d, k > k0);
+            if (k + 1 < k1) multiply(at, at, d, 1, S::kBlockBytes >> 4);
             commit<PAIR>(empty_at + at * 8);
           }
           commit<PAIR>(tfull_at + acc * 8);
         } else {
           const uint32_t d = tmem_base, small = tmem_base + BN;
-          for (int k = it.k0; k < it.k1; ++k) {
-            const bool opens = opens_round(k - it.k0);
-            const bool closes = k + 1 == it.k1 || opens_round(k + 1 - it.k0);
+          for (int k = k0; k < k1; ++k) {
+            const bool opens = opens_round(k - k0);
+            const bool closes = k + 1 == k1 || opens_round(k + 1 - k0);
             uint32_t h, m, l;
-            if (k == it.k0 && !(ok = wait_bar(tempty_at + 8, (tile & 1) ^ 1, s_abort, limit))) break;
+            if (k == k0 && !(ok = wait_bar(tempty_at + 8, (run & 1) ^ 1, s_abort, limit))) break;
             if (!(ok = next(&m))) break;
-            multiply(m, m, small, k > it.k0);
+            multiply(m, m, small, k > k0);
             if (opens) {
               if (!(ok = wait_bar(tempty_at, (round & 1) ^ 1, s_abort, limit))) break;
               tmem_fence_after();
@@ -618,6 +635,16 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           }
           commit<PAIR>(tfull_at + 8);
         }
+      };
+      for (int i = worker; i < items && ok; i += workers) {
+        const Item it = item_of(i);
+        if constexpr (LONG) {
+          for (int k = it.k0; k < it.k1 && ok; k += S::kRun, ++run)
+            multiply_run(k, min(it.k1, k + S::kRun));
+        } else {
+          multiply_run(it.k0, it.k1);
+          ++run;
+        }
       }
       if (!ok) fail();
       // Retire every issued MMA before tensor memory is released.
@@ -629,7 +656,8 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
     }
   } else {
     // ---------------- epilogue ----------------
-    if constexpr (P == 3) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
+    if constexpr (S::kHold)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs<T>));
     const int quarter = warp & 3, ew = warp - 4, group = ew >> 2;
     const uint32_t buf = smem_u32(staging + ew * 32 * RB);
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -660,8 +688,14 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
     };
     using Step = float[S::kStep];
     auto limit32 = [](int64_t c) { return (int)max((int64_t)0, min((int64_t)kStep, c)); };
-    uint32_t round = 0, tile = 0;
-    for (int i = worker; i < items; i += workers, ++tile) {
+    // float32: this thread's sums of the finished runs, a warp's 32 lanes side by side.
+    // (The address is not kept in registers, of which none are left.)
+    auto runs = [&](int at) {
+      return p.runs + (((int64_t)blockIdx.x * kEpiWarps + ew) * kWarpCols + at) * 32 + lane;
+    };
+    uint32_t round = 0, run = 0;
+    int done = 0;  // blocks of item i whose sums are in scratch (float32, LONG)
+    for (int i = worker; i < items;) {
       const Item it = item_of(i);
       const int64_t row0 = (int64_t)it.tm * kTileRows + rank * kBM + quarter * 32;
       const int rows = (int)max((int64_t)0, min((int64_t)32, p.rows - row0));
@@ -671,8 +705,8 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
                          ? static_cast<const T*>(p.residual) + row0 * p.ldr + warp_col
                          : nullptr;
       Incoming<T, RB> in;
-      // (float32 has no registers for it while it drains.)
-      if (MODE == kLinear && P == 1 && res) in.start(res, p.ldr, rows, limit32(cols), lane);
+      // (Held sums leave no registers for it.)
+      if (MODE == kLinear && !S::kHold && res) in.start(res, p.ldr, rows, limit32(cols), lane);
       // Finishes kStep columns from `at` on: v the sums (gated: the gate's; up(h, u)
       // then gives the up's, 32 at a time, since not all are held at once).
       auto finish = [&](int at, Step& v, auto&& up) {
@@ -696,7 +730,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           }
           return;
         }
-        if (MODE == kLinear && P == 3 && res) in.start(res + at, p.ldr, rows, n, lane);
+        if (MODE == kLinear && S::kHold && res) in.start(res + at, p.ldr, rows, n, lane);
         const bool vec = p.bias_vec != 0;
         auto biases = [&](int which) {
           const T* b = static_cast<const T*>(p.bias[which]);
@@ -725,16 +759,17 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
         }
         if (MODE == kLinear && res && n > 0) {
           in.add(buf, v, lane);
-          if (P == 1 && at + kStep < kOutCols)
+          if (!S::kHold && at + kStep < kOutCols)
             in.start(res + at + kStep, p.ldr, rows, limit32(cols - at - kStep), lane);
         }
         if (n > 0)
           emit<T, RB>(buf, static_cast<T*>(p.out[MODE == kDw ? it.batch : 0]) + row0 * p.ldo + col,
                       p.ldo, rows, n, p.vec, v, lane);
       };
-      if constexpr (P == 1) {
-        const uint32_t acc = tile & 1, t = tmem_base + acc * BN + lanes;
-        if (!wait_acc(acc, (tile >> 1) & 1)) break;
+      if constexpr (!S::kHold) {
+        const uint32_t acc = run & 1, t = tmem_base + acc * BN + lanes;
+        if (!wait_acc(acc, (run >> 1) & 1)) break;
+        ++run;
         // N sums; the accumulator is freed with its last ones.
         auto take = [&](int which, int at, auto& v) {
           constexpr int N = sizeof(v) / 4;
@@ -772,14 +807,43 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
           }
         };
         bool ok = true;
-        for (int k = it.k0; k < it.k1 && ok; k += k == it.k0 ? kFirstRound : kRound, ++round) {
-          if (!(ok = wait_acc(0, round & 1))) break;
-          drain(tmem_base, k == it.k0);
-          release_acc(0);
-        }
-        if (ok && (ok = wait_acc(1, tile & 1))) {
-          drain(tmem_base + BN, false);
-          release_acc(1);
+        if constexpr (P == 1) {
+          for (int k = it.k0; k < it.k1 && ok; k += S::kRun, ++run) {
+            const uint32_t acc = run & 1;
+            if (!(ok = wait_acc(acc, (run >> 1) & 1))) break;
+            drain(tmem_base + acc * BN, k == it.k0);
+            release_acc(acc);
+          }
+        } else {
+          const int k0 = LONG ? it.k0 + done : it.k0;
+          const int k1 = LONG ? min(it.k1, k0 + S::kRun) : it.k1;
+          for (int k = k0; k < k1 && ok; k += k == k0 ? kFirstRound : kRound, ++round) {
+            if (!(ok = wait_acc(0, round & 1))) break;
+            drain(tmem_base, k == k0);
+            release_acc(0);
+          }
+          if (ok && (ok = wait_acc(1, run & 1))) {
+            drain(tmem_base + BN, false);
+            release_acc(1);
+          }
+          ++run;
+          if constexpr (LONG) {
+            if (ok && done) {
+              const float* r = runs(0);
+#pragma unroll
+              for (int j = 0; j < kWarpCols; ++j) {
+                sum[j / 32][j % 32] += r[j * 32];
+                if (j % 8 == 7) asm volatile("" ::: "memory");  // (eight on their way)
+              }
+            }
+            if (ok && k1 < it.k1) {
+              float* r = runs(0);
+#pragma unroll
+              for (int j = 0; j < kWarpCols; ++j) r[j * 32] = sum[j / 32][j % 32];
+              done += S::kRun;
+              continue;
+            }
+          }
         }
         if (!ok) break;
         // A rolled loop over steps that always takes the first sums and moves the
@@ -796,6 +860,8 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN>::kThreads, 1)
             for (int j = 0; j < 32; ++j) sum[i][j] = sum[i + kPer][j];
         }
       }
+      done = 0;
+      i += workers;
     }
   }
 
@@ -904,10 +970,10 @@ inline bool operand_map(CUtensorMap* map, const GemmOperand& o, int box_outer) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int MODE, typename T, bool PAIR, int BN>
-xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
+template <int MODE, typename T, bool PAIR, int BN, bool LONG>
+xvec_gpu_status launch_sums(const GemmCall& c, cudaStream_t s) {
   GemmParams p = c.p;
-  using S = GemmShape<MODE, T, PAIR, BN>;
+  using S = GemmShape<MODE, T, PAIR, BN, LONG>;
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   CUtensorMap a, b0, b1;
   const int b_box = B_MN ? kBK : (MODE == kGated && !PAIR) ? S::kBRows / 2 : S::kBRows;
@@ -920,17 +986,17 @@ xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
   const uint32_t f = c.bf16 ? 1u : 0u;
   p.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
             ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
-  auto kern = gemm_kernel<MODE, T, PAIR, BN>;
+  auto kern = gemm_kernel<MODE, T, PAIR, BN, LONG>;
   static std::atomic<uint64_t> ready{0};  // by device
   const uint64_t bit = 1ull << (c.device & 63);
   if (!(ready.load(std::memory_order_acquire) & bit)) {
     XVEC_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)S::kSmemBytes));
-    if (std::is_same<T, float>::value) {
+    if (S::kHold) {
       // The register split needs the whole block's share at launch, or it would wait.
       cudaFuncAttributes fa;
       XVEC_CUDA(cudaFuncGetAttributes(&fa, kern));
-      if (fa.numRegs * S::kThreads < 128 * kFewRegs + (S::kThreads - 128) * kManyRegs) {
+      if (fa.numRegs * S::kThreads < 128 * kFewRegs + (S::kThreads - 128) * kManyRegs<T>) {
         set_error("adapter: the matrix kernel was built with %d registers", fa.numRegs);
         return XVEC_GPU_UNSUPPORTED;
       }
@@ -950,6 +1016,12 @@ xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
                          256, 0, s, 1, p));
   }
   return XVEC_GPU_OK;
+}
+
+template <int MODE, typename T, bool PAIR, int BN>
+xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
+  return c.p.blocks_per_split > run_blocks(std::is_same<T, float>::value) ? launch_sums<MODE, T, PAIR, BN, true>(c, s)
+                                     : launch_sums<MODE, T, PAIR, BN, false>(c, s);
 }
 
 template <int MODE, typename T>
