@@ -50,30 +50,48 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return u;
 }
 
-constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
-// Phi(z), the standard normal distribution, and exp(-z^2 / 2): the rational
-// approximation 7.1.26 of Abramowitz and Stegun, Phi off by at most 7.5e-8 (a
-// little over float32's half step at 1), with a reciprocal, an exponential and
-// six multiply-adds.  With erff the epilogue was the longest part of a tile: a
-// float32 10000 x 960 -> 960 call took 149 us.
+// exp(-x) for x >= 0: the 16-bit types' form is off by x 2^-23 relative to itself.
+template <typename T>
+__device__ __forceinline__ float exp_minus(float x) {
+  return sizeof(T) == 4 ? expf(-x) : __expf(-x);
+}
+
+// Phi(z), the standard normal distribution, and *gauss = exp(-z^2 / 2).  For a = |z|:
+//   Phi(-a) = exp(-a^2 / 2) R(a),  R(a) = erfc(a / sqrt 2) exp(a^2 / 2) / 2 = t P(t),
+//   t = 1 / (1 + 39/128 a),
+// P of degree 7, fitted to R on a = 0..14.5 for the least largest relative error (1.0e-7).  So
+// the far negative tail, where gelu is small, keeps its relative accuracy: evaluated in
+// float32 Phi(-a) is off by 4.3e-7 of itself at most (a <= 12; the 16-bit exponential
+// adds a^2 2^-24), and Phi(a) by 2.2e-7.  float32 makes up for the rounding of a^2.  With
+// erff the epilogue was the longest part of a tile (float32 10000 x 960 -> 960 149 us).
+template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
-  const float x = fabsf(z) * kSqrtHalf;
-  const float e = __expf(-x * x);
-  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  const float tail = 0.5f * q * t * e;  // Phi(-|z|)
+  // (At 16 both are 0; an infinite square would have no rounding to make up for.)
+  const float a = fminf(fabsf(z), 16.f), s = a * a;
+  float e = exp_minus<T>(0.5f * s);
+  if (sizeof(T) == 4) e = fmaf(-0.5f * fmaf(a, a, -s), e, e);
+  const float t = __fdividef(1.f, fmaf(0.3046875f, a, 1.f));
+  float q = fmaf(0.036564309f, t, -0.15296334f);
+  q = fmaf(q, t, 0.18648443f);
+  q = fmaf(q, t, -0.038461823f);
+  q = fmaf(q, t, 0.12123448f);
+  q = fmaf(q, t, 0.10327935f);
+  q = fmaf(q, t, 0.12234776f);
+  q = fmaf(q, t, 0.12151483f);
+  const float tail = q * t * e;
   *gauss = e;
   return z < 0.f ? tail : 1.f - tail;
 }
-// 1 / (1 + exp(-z)).  The quotient is off by at most 2 units in the last place.
+// 1 / (1 + exp(-z)), and its difference to 1 in *rest, both without cancellation or overflow:
+// off by a few units in the last place wherever they are normal numbers.
 template <typename T>
-__device__ __forceinline__ float sigmoid(float z) {
-  return __fdividef(1.f, 1.f + (sizeof(T) == 4 ? expf(-z) : __expf(-z)));
+__device__ __forceinline__ float sigmoid(float z, float* rest) {
+  const float e = exp_minus<T>(fabsf(z)), r = __fdividef(1.f, 1.f + e);
+  const float er = e * r;
+  *rest = z < 0.f ? r : er;
+  return z < 0.f ? er : r;
 }
 
 template <typename T>
@@ -83,11 +101,20 @@ __device__ __forceinline__ float relu(float z) {
 template <typename T>
 __device__ __forceinline__ float gelu(float z) {
   float e;
-  return z * normal_cdf(z, &e);
+  return z * normal_cdf<T>(z, &e);
 }
+// z / (1 + exp(-z)).  The fast quotient is 0 for divisors above 2^126, which bfloat16's and
+// float32's small results would notice: bfloat16 divides both sides by 2^8 (good down to -92,
+// where silu leaves the normal numbers), at two instructions; float32 has no bits to lose
+// in the exponential's argument.
 template <typename T>
 __device__ __forceinline__ float silu(float z) {
-  return z * sigmoid<T>(z);
+  constexpr float kLog256 = 5.5451774f;
+  if constexpr (std::is_same<T, __half>::value) return __fdividef(z, 1.f + __expf(-z));
+  if constexpr (std::is_same<T, bf16>::value)
+    return __fdividef(z * 0.00390625f, 0.00390625f + __expf(-z - kLog256));
+  float rest;
+  return z * sigmoid<T>(z, &rest);
 }
 
 // act(z) for results of type T.
@@ -122,13 +149,14 @@ __device__ __forceinline__ float activate_slope(int act, float z, float* slope) 
       return relu<T>(z);
     case XVEC_ACT_GELU: {
       float e;
-      const float cdf = normal_cdf(z, &e);
+      const float cdf = normal_cdf<T>(z, &e);
       *slope = fmaf(z * e, kInvSqrt2Pi, cdf);
       return z * cdf;
     }
     case XVEC_ACT_SILU: {
-      const float s = sigmoid<T>(z);
-      *slope = s * (1.f + z * (1.f - s));
+      float rest;
+      const float s = sigmoid<T>(z, &rest);
+      *slope = s * fmaf(z, rest, 1.f);
       return z * s;
     }
     default:
