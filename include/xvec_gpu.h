@@ -574,7 +574,11 @@ xvec_gpu_status xvec_gpu_rotate_device(int32_t device, const uint8_t* signs, int
  * float32 results have float32 accuracy (2-norm errors of 1e-7 to 4e-7), but an
  * infinity in a float32 operand may come out as a NaN, and elements below
  * 2^-109 are held to 2^-134.  Gradients of pre-activations are rounded to
- * 16 bits in between for 16-bit storage.  Results do not vary from run to run
+ * 16 bits in between for 16-bit storage, since they are operands of products:
+ * errors of dx and weight gradients are sqrt(2) of one rounding's.  For binary16
+ * they are scaled by a power of two where the largest of a call lies outside
+ * 2^-6..65504, so that only the results have to fit the type (what is below
+ * 2^-40 of the largest is lost).  Results do not vary from run to run
  * on a device, but a different number of rows may change their last bits.
  *
  * Every call enqueues on `stream` and does not wait; it can be captured into

@@ -71,8 +71,9 @@ def test_gated(xb, shape, scale):
 
 
 @pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
-@pytest.mark.parametrize("scale", [2.0 ** 15, 1.0, 2.0 ** -12, 2.0 ** -20])
+@pytest.mark.parametrize("scale", [18000.0, 1.0, 2.0 ** -12, 2.0 ** -20])
 def test_linear(xb, activation, scale):
+    """Incoming gradients up to 3.5 x 18000 = 63000, which a slope of up to 1.13 brings above 65504."""
     n, k, m = 1500, 136, 200
     mk = Maker("fp16", 2)
     dy, z = make(mk, n, m, scale), make(mk, n, m, 1.0)
@@ -90,7 +91,7 @@ def test_linear(xb, activation, scale):
 
 
 def test_values_that_are_not_finite_stay_in_their_rows(xb):
-    """An infinity or a NaN among the incoming gradients is no reason to scale the others."""
+    """An infinity or a NaN among the incoming gradients does not decide how the others are held."""
     n, k, m = 300, 64, 72
     mk = Maker("fp16", 3)
     for scale in (1.0, 2.0 ** -12):
@@ -107,8 +108,7 @@ def test_values_that_are_not_finite_stay_in_their_rows(xb):
         d = dy.double() * slope("gelu", z.double())
         want = (d @ w.double())[~bad]
         err = (dx[~bad].double() - want).norm() / want.norm()
-        # (Not scaled: gradients near 2^-12 are held to 2^-25 each.)
-        assert err.item() < BOUND + (2.0 ** -13 if scale < 1 else 0)
+        assert err.item() < BOUND
 
 
 def test_zero_gradients(xb):

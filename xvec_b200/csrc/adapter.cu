@@ -11,6 +11,7 @@
 // (elementwise, with their column sums) into scratch and run the products.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 
 #include "adapter.cuh"
@@ -205,9 +206,35 @@ struct Slopes {
   uint16_t* out;
   int64_t ld;
   float* partial;
+  float* peaks;  // [cols chunks] each block's largest finite |gradient| (binary16 operands)
+  float* scale;  // what the operands' products are multiplied by (AGAIN)
   Packs packs;
   unsigned pack_blocks;  // for each packing
 };
+
+// --- the scale of binary16 operands
+// The least largest value that needs no scaling: binary16 holds what is 2^-8 of it in full.
+constexpr float kLeastPeak = 0.015625f;
+// The largest v of the block's 256 threads, on every thread.
+__device__ __forceinline__ float block_max(float v) {
+  __shared__ float part[8];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v = fmaxf(v, part[i]);
+  return v;
+}
+// The power of two that the operands are multiplied by.
+__device__ __forceinline__ float operand_scale(const float* peaks, int num) {
+  float peak = 0.f;
+  for (int i = threadIdx.x; i < num; i += 256) peak = fmaxf(peak, peaks[i]);
+  peak = block_max(peak);
+  if (peak == 0.f || (peak >= kLeastPeak && peak <= 65504.f)) return 1.f;
+  return ldexpf(1.f, min(14 - ilogbf(peak), 126));
+}
 
 // Blocks [0, cols chunks) are the gradients', the others the packings'.  A block
 // owns 256 columns of a row chunk: 32 threads of 8 columns, 8 rows at a time; bound
@@ -215,12 +242,23 @@ struct Slopes {
 // kRows rows of a thread are requested before the first is used and held as
 // they came.  (Held as floats they took 122 registers, a quarter of the warps.)
 // VEC: all of dy, z and u allow 16-byte accesses.
-template <typename T, bool GATED, bool VEC>
+// AGAIN: after a first pass, binary16 operands only.  A gradient of two or three stored
+// values easily leaves binary16's range where its products do not.  If the largest is
+// outside kLeastPeak..65504, the operands are written once more, times the power of two
+// that brings it to 2^14..2^15; values below 2^-40 of it are lost.  Else nothing but
+// *scale = 1 is left to do (4 us; the maxima cost the first pass 4 us of 54).
+template <typename T, bool GATED, bool VEC, bool AGAIN>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : VEC ? 4 : 3)
     slope_kernel(const __grid_constant__ Slopes p) {
   pdl_begin();
+  float up = 1.f;
+  if constexpr (AGAIN) {
+    up = operand_scale(p.peaks, p.cols * p.chunks);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.scale = 1.f / up;  // (a power of two)
+    if (up == 1.f) return;
+  }
   const unsigned slope_blocks = (unsigned)p.cols * p.chunks;
-  if (blockIdx.x >= slope_blocks) {
+  if (!AGAIN && blockIdx.x >= slope_blocks) {
     const unsigned b = blockIdx.x - slope_blocks, which = b / p.pack_blocks;
     pack<T>(p.packs.p[which], (int64_t)(b - which * p.pack_blocks) * 256 + threadIdx.x,
             (int64_t)p.pack_blocks * 256);
@@ -241,7 +279,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : VEC ? 4 : 3)
   const int64_t r0 = chunk * p.rows_per_chunk;
   const int64_t r1 = min(n, r0 + p.rows_per_chunk);
   const bool act_needed = GATED || act != XVEC_ACT_NONE;
-  float sum[kOuts][8] = {};
+  constexpr bool kPeak = std::is_same<T, __half>::value && !AGAIN;
+  float sum[kOuts][8] = {}, peak = 0.f;
   if (c < m) {
     for (int64_t r = r0 + ty; r < r1; r += 8 * kRows) {
       Eight<T, VEC> dr[kRows], zr[kRows], ur[kRows];
@@ -274,15 +313,36 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : VEC ? 4 : 3)
         }
 #pragma unroll
         for (int o = 0; o < kOuts; ++o) {
+          if constexpr (AGAIN) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[o][j] *= up;
+          }
           if (out)
             store_operand<T>(out + (o * kPlanes * n + r + 8 * i) * ld + c, n * ld, d[o]);
+          if constexpr (kPeak) {
+            float most = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(d[o][j]));
+            if (most > FLT_MAX || m - c < 8) {  // only what is finite and exists
+              most = 0.f;
+              for (int j = 0; j < 8; ++j)
+                if (fabsf(d[o][j]) <= FLT_MAX && c + j < m) most = fmaxf(most, fabsf(d[o][j]));
+            }
+            peak = fmaxf(peak, most);
+          }
 #pragma unroll
           for (int j = 0; j < 8; ++j) sum[o][j] += d[o][j];
         }
       }
     }
   }
-  if (p.partial) {
+  if constexpr (kPeak) {
+    if (p.peaks) {
+      peak = block_max(peak);
+      if (threadIdx.x == 0) p.peaks[blockIdx.x] = peak;
+    }
+  }
+  if (!AGAIN && p.partial) {
     __shared__ float part[8][256];
 #pragma unroll
     for (int o = 0; o < kOuts; ++o) {
@@ -367,10 +427,17 @@ xvec_gpu_status slopes_t(Slopes& a, cudaStream_t s) {
   for (int i = 0; i < a.packs.n; ++i)
     most = std::max(most, a.packs.p[i].rows * a.packs.p[i].ld / 8);
   a.pack_blocks = grid_of(most);
-  auto* kern = a.u ? (vec ? slope_kernel<T, true, true> : slope_kernel<T, true, false>)
-                   : (vec ? slope_kernel<T, false, true> : slope_kernel<T, false, false>);
-  XVEC_CUDA(launch_pdl(kern, dim3((unsigned)a.cols * a.chunks + a.pack_blocks * a.packs.n), 256, 0,
-                       s, 1, a));
+  auto* kern = a.u ? (vec ? slope_kernel<T, true, true, false> : slope_kernel<T, true, false, false>)
+                   : (vec ? slope_kernel<T, false, true, false> : slope_kernel<T, false, false, false>);
+  const unsigned blocks = (unsigned)a.cols * a.chunks;
+  XVEC_CUDA(launch_pdl(kern, dim3(blocks + a.pack_blocks * a.packs.n), 256, 0, s, 1, a));
+  if constexpr (std::is_same<T, __half>::value) {
+    if (a.peaks) {
+      auto* again = a.u ? (vec ? slope_kernel<T, true, true, true> : slope_kernel<T, true, false, true>)
+                        : (vec ? slope_kernel<T, false, true, true> : slope_kernel<T, false, false, true>);
+      XVEC_CUDA(launch_pdl(again, dim3(blocks), 256, 0, s, 1, a));
+    }
+  }
   return XVEC_GPU_OK;
 }
 
@@ -775,6 +842,9 @@ xvec_gpu_status run_backward(const Backward& b) {
   a.lddy = b.lddy, a.ldz = b.ldpre, a.n = b.n, a.m = b.out_dim, a.act = b.act;
   a.ld = grad.ld;
   plan_slopes(&a);
+  const bool scaled = b.storage == XVEC_STORAGE_FP16 && !direct && products;
+  const size_t peaks_at = scaled ? arena.add((size_t)a.cols * a.chunks * 4) : 0;
+  const size_t scale_at = scaled ? arena.add(4) : 0;
   const size_t sums_at = sums ? arena.add((size_t)2 * a.chunks * a.m * 4) : 0;
   GemmCall dx, dw;
   dx.mode = kDx;
@@ -804,6 +874,10 @@ xvec_gpu_status run_backward(const Backward& b) {
   for (Operand* o : {&w[0], &w[1], &x}) place(o, arena, &packs);
   if (!direct && products) grad.p = a.out = static_cast<uint16_t*>(arena.at(grad_at));
   if (sums) a.partial = static_cast<float*>(arena.at(sums_at));
+  if (scaled) {
+    a.peaks = static_cast<float*>(arena.at(peaks_at));
+    dx.p.scale = dw.p.scale = a.scale = static_cast<float*>(arena.at(scale_at));
+  }
   // Small packings share the gradient pass's launch; large ones want the warps that
   // its registers leave no room for (75103 x 402 fp32: 122 us together).
   int64_t packed = 0;

@@ -277,6 +277,7 @@ struct GemmParams {
   float* partial;        // splits > 1: [splits][batches or halves][rows][ldp] float sums
   int64_t ldp;
   float* runs;           // float32, long sums: those of finished runs, by thread
+  const float* scale;    // what sums are multiplied by (binary16 kDx, kDw; may be NULL)
   uint32_t idesc;
   int vec;               // bytes of an access that outputs and saves allow
   int bias_vec;          // the biases allow 16

@@ -693,6 +693,9 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN, LONG>::kThreads, 
     auto runs = [&](int at) {
       return p.runs + (((int64_t)blockIdx.x * kEpiWarps + ew) * kWarpCols + at) * 32 + lane;
     };
+    // (From L2: this launch may have begun before it waited for any other, p.beside.)
+    constexpr bool kScaled = std::is_same<T, __half>::value && (MODE == kDx || MODE == kDw);
+    const float scale = kScaled && p.scale ? __ldcg(p.scale) : 1.f;
     uint32_t round = 0, run = 0;
     int done = 0;  // blocks of item i whose sums are in scratch (float32, LONG)
     for (int i = worker; i < items;) {
@@ -756,6 +759,10 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN, LONG>::kThreads, 
             for (int j = 0; j < 32; ++j) v[h * 32 + j] *= u[j];
           }
           if (p.save[1]) stage_out<T, RB>(buf, saved(1), p.lds, rows, n, p.vec, lane);
+        }
+        if constexpr (kScaled) {
+#pragma unroll
+          for (int j = 0; j < kStep; ++j) v[j] *= scale;
         }
         if (MODE == kLinear && res && n > 0) {
           in.add(buf, v, lane);
@@ -909,6 +916,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Gem
   const int batch = blockIdx.y;
   constexpr int kPlanes = MODE == kGated ? 2 : 1;
   const int64_t step = (int64_t)p.batches * kPlanes * p.rows * p.ldp;  // between splits
+  const float scale = p.scale ? *p.scale : 1.f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / groups, col = (i - row * groups) * 4;
@@ -925,7 +933,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Gem
     for (int j = 0; j < 4; ++j) {
       const int64_t c = col + j;
       if (c >= p.cols) break;
-      float y = v[0][j];
+      float y = v[0][j] * scale;
       if (MODE == kLinear || MODE == kGated) {
         if (p.bias[0]) y += to_f(static_cast<const T*>(p.bias[0])[c]);
         if (p.save[0]) static_cast<T*>(p.save[0])[row * p.lds + c] = from_f<T>(y);
