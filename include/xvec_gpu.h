@@ -584,7 +584,10 @@ xvec_gpu_status xvec_gpu_rotate_device(int32_t device, const uint8_t* signs, int
  * Every call enqueues on `stream` and does not wait; it can be captured into
  * a CUDA graph.  Scratch is allocated and freed in stream order (float32: 6
  * bytes for each element of every operand; 16-bit: only what cannot be read in
- * place, the pre-activation gradients and split sums).  n = 0 does
+ * place, the pre-activation gradients and split sums), from a memory pool of
+ * the library's own: the device's default pool stays as the caller set it up.  Up
+ * to 16 GiB of freed scratch stay in it for the next calls, what is above goes back at
+ * the next synchronization, and xvec_gpu_trim_scratch gives back the rest.  n = 0 does
  * nothing in the forward calls and gives zero weight and bias gradients.  An
  * output may not overlap an input or another output (XVEC_GPU_INVALID_ARGUMENT),
  * except that y may be the residual itself.  `status` (device int32, may be
@@ -727,6 +730,10 @@ typedef struct {
 xvec_gpu_status xvec_gpu_clip_gradients_device(int32_t device, const xvec_gpu_tensor* tensors,
                                                int32_t num_tensors, double max_norm,
                                                float* d_norm, void* stream);
+
+/* Gives the scratch that the calls above keep on a device, and that no enqueued
+ * call still uses, back to the system. */
+xvec_gpu_status xvec_gpu_trim_scratch(int32_t device);
 
 /* Counters (the reference's RuntimeStats role, collection.go:5185-5315, for
  * the device path).  Device-time fields are filled only while timing is

@@ -70,7 +70,7 @@ EXPORTED_SYMBOLS = (
     "xvec_gpu_rotation_signs", "xvec_gpu_rotate", "xvec_gpu_rotate_device",
     "xvec_gpu_rabitq_set_graph", "xvec_gpu_diskann_set_model", "xvec_gpu_diskann_set_graph",
     "xvec_gpu_linear_device", "xvec_gpu_linear_backward_device", "xvec_gpu_gated_device",
-    "xvec_gpu_gated_backward_device", "xvec_gpu_clip_gradients_device",
+    "xvec_gpu_gated_backward_device", "xvec_gpu_clip_gradients_device", "xvec_gpu_trim_scratch",
 )
 
 
@@ -206,6 +206,7 @@ def _load() -> ctypes.CDLL:
                        ("gated", GatedArgs), ("gated_backward", GatedBackwardArgs)):
         getattr(lib, f"xvec_gpu_{name}_device").argtypes = [ctypes.POINTER(args)]
     lib.xvec_gpu_clip_gradients_device.argtypes = [i32, vp, i32, ctypes.c_double, vp, vp]
+    lib.xvec_gpu_trim_scratch.argtypes = [i32]
     lib.xvec_gpu_rotate_device.argtypes = [i32, vp, i64, i32, vp, i64, vp, i32, vp, vp]
     lib.xvec_gpu_set_wait_limit_ns.restype = i64
     lib.xvec_gpu_set_wait_limit_ns.argtypes = [i64]
@@ -366,6 +367,12 @@ def clip_gradients_device(device: int, tensors: Sequence[tuple], max_norm: float
     table = (ctypes.c_int64 * max(1, len(flat)))(*flat)
     _check(_lib.xvec_gpu_clip_gradients_device(device, table, len(flat) // 4, max_norm,
                                                norm_ptr or None, stream or None))
+
+
+def trim_scratch(device: int) -> None:
+    """Gives back the scratch that the learned adapters and the clipping keep on a
+    device between calls (xvec_gpu_trim_scratch)."""
+    _check(_lib.xvec_gpu_trim_scratch(device))
 
 
 def device_count() -> int:

@@ -252,6 +252,7 @@ cudaError_t launch_pdl(void (*kern)(Params...), dim3 grid, int block, size_t sme
 // stream capture of another thread does not forbid the one-time settings and the
 // loading of kernels (none of them belongs into a graph).
 struct DeviceGuard {
+  cudaMemPool_t pool = nullptr;  // the device's scratch
   int before = -1;
   bool relaxed = false;
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;

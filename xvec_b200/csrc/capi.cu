@@ -52,10 +52,11 @@ xvec_gpu_status DeviceBuffer::reserve(size_t need, size_t keep, cudaStream_t str
   return XVEC_GPU_OK;
 }
 
-xvec_gpu_status Scratch::alloc(size_t nbytes, cudaStream_t s) {
+xvec_gpu_status Scratch::alloc(size_t nbytes, cudaStream_t s, cudaMemPool_t pool) {
   stream = s;
   if (nbytes == 0) nbytes = 16;
-  cudaError_t e = cudaMallocAsync(&ptr, nbytes, s);
+  cudaError_t e =
+      pool ? cudaMallocFromPoolAsync(&ptr, nbytes, pool, s) : cudaMallocAsync(&ptr, nbytes, s);
   if (e != cudaSuccess) {
     cudaGetLastError();
     ptr = nullptr;

@@ -106,7 +106,8 @@ struct Scratch {
   ~Scratch() {
     if (ptr) cudaFreeAsync(ptr, stream);
   }
-  xvec_gpu_status alloc(size_t bytes, cudaStream_t s);
+  // From `pool`, else the device's default pool.
+  xvec_gpu_status alloc(size_t bytes, cudaStream_t s, cudaMemPool_t pool = nullptr);
   template <typename T>
   T* as() const {
     return static_cast<T*>(ptr);

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 // Launches over all tensors, N at a time: sums (pass 0) and scaling (pass 1).
 template <int N>
 xvec_gpu_status clip(const xvec_gpu_tensor* tensors, int num, double max_norm, float* d_norm,
-                     int sms, cudaStream_t s) {
+                     int sms, const DeviceGuard& guard, cudaStream_t s) {
   const int max_blocks = sms * kBlocksPerSm;
   Table<N> t;
   // Fills t from tensor *i on; false when nothing is left.
@@ -256,7 +256,7 @@ xvec_gpu_status clip(const xvec_gpu_tensor* tensors, int num, double max_norm, f
   int blocks = 0;
   for (int i = 0; fill(&i);) blocks += (int)std::min<uint32_t>(t.chunks, max_blocks);
   Scratch sums;
-  if (xvec_gpu_status st = sums.alloc((size_t)blocks * 8, s)) return st;
+  if (xvec_gpu_status st = sums.alloc((size_t)blocks * 8, s, guard.pool)) return st;
   int done = 0;
   for (int i = 0; fill(&i);) {
     const int b = (int)std::min<uint32_t>(t.chunks, max_blocks);
@@ -341,7 +341,7 @@ extern "C" xvec_gpu_status xvec_gpu_clip_gradients_device(int32_t device,
   int sms = 0;
   if (xvec_gpu_status st = count_sms(device, &sms)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return num_tensors <= kFew    ? clip<kFew>(tensors, num_tensors, max_norm, d_norm, sms, s)
-         : num_tensors <= kSome ? clip<kSome>(tensors, num_tensors, max_norm, d_norm, sms, s)
-                                : clip<kMany>(tensors, num_tensors, max_norm, d_norm, sms, s);
+  return num_tensors <= kFew    ? clip<kFew>(tensors, num_tensors, max_norm, d_norm, sms, guard, s)
+         : num_tensors <= kSome ? clip<kSome>(tensors, num_tensors, max_norm, d_norm, sms, guard, s)
+                                : clip<kMany>(tensors, num_tensors, max_norm, d_norm, sms, guard, s);
 }
