@@ -530,6 +530,7 @@ struct Check {
     aligned(name, p);
     outs[num_outs++] = {name, p, rows, cols, ld};
   }
+  void status(const int32_t* p) { out("status", p, 1, 4 / size, 4 / size); }
   void aligned(const char* name, const void* p) {
     if (st || (uintptr_t)p % size == 0) return;
     set_error("adapter: %s is not aligned to its elements", name);
@@ -719,6 +720,7 @@ extern "C" xvec_gpu_status xvec_gpu_linear_device(const xvec_gpu_linear_args* ar
   c.in(residual, a.residual, a.n, a.out_dim, a.ldr);
   c.out(y, a.y, a.n, a.out_dim, a.ldy);
   c.out("preact", a.preact, a.n, a.out_dim, a.ldz);
+  c.status(a.status);
   if ((st = c.overlaps(y, residual))) return st;
   if (a.n == 0) return XVEC_GPU_OK;
   DeviceGuard guard;
@@ -772,6 +774,7 @@ extern "C" xvec_gpu_status xvec_gpu_gated_device(const xvec_gpu_gated_args* args
   c.out("h", a.h, a.n, a.out_dim, a.ldh);
   c.out("gate", a.gate, a.n, a.out_dim, a.ldg);
   c.out("up", a.up, a.n, a.out_dim, a.ldg);
+  c.status(a.status);
   if ((st = c.overlaps())) return st;
   if (a.n == 0) return XVEC_GPU_OK;
   DeviceGuard guard;
@@ -965,6 +968,7 @@ extern "C" xvec_gpu_status xvec_gpu_linear_backward_device(
   c.out("dx", a.dx, a.n, a.in_dim, a.lddx);
   c.out("dweight", a.dweight, a.out_dim, a.in_dim, a.lddw);
   c.out("dbias", a.dbias, 1, a.out_dim, a.out_dim);
+  c.status(a.status);
   if ((st = c.overlaps())) return st;
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
@@ -1005,6 +1009,7 @@ extern "C" xvec_gpu_status xvec_gpu_gated_backward_device(
   c.out("dup_weight", a.dup_weight, a.out_dim, a.in_dim, a.lddw);
   c.out("dgate_bias", a.dgate_bias, 1, a.out_dim, a.out_dim);
   c.out("dup_bias", a.dup_bias, 1, a.out_dim, a.out_dim);
+  c.status(a.status);
   if ((st = c.overlaps())) return st;
   DeviceGuard guard;
   if ((st = guard.set(a.device))) return st;
