@@ -734,7 +734,7 @@ __global__ void __launch_bounds__(GemmShape<MODE, T, PAIR, BN, LONG>::kThreads, 
           return;
         }
         if (MODE == kLinear && S::kHold && res) in.start(res + at, p.ldr, rows, n, lane);
-        const bool vec = p.bias_vec != 0;
+        [[maybe_unused]] const bool vec = p.bias_vec != 0;  // (forward products)
         auto biases = [&](int which) {
           const T* b = static_cast<const T*>(p.bias[which]);
           return b ? b + col : b;
