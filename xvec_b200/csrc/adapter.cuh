@@ -84,12 +84,21 @@ __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
   *gauss = e;
   return z < 0.f ? tail : 1.f - tail;
 }
-// 1 / (1 + exp(-z)), and its difference to 1 in *rest, both without cancellation or overflow:
-// off by a few units in the last place wherever they are normal numbers.
+// 1 / (1 + exp(-z)), and its difference to 1 in *rest.  The fast quotient is 0 for divisors
+// above 2^126 (z below -87.3), which bfloat16's and float32's small results would
+// notice: bfloat16 divides both sides by 2^8; float32, which has no bits to lose in the
+// exponential's argument, takes exp(-|z|), and so has *rest without cancellation.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float z, float* rest) {
-  const float e = exp_minus<T>(fabsf(z)), r = __fdividef(1.f, 1.f + e);
-  const float er = e * r;
+  constexpr float kLog256 = 5.5451774f, kBy256 = 0.00390625f;
+  if constexpr (sizeof(T) == 2) {
+    const float s = std::is_same<T, bf16>::value
+                        ? __fdividef(kBy256, kBy256 + __expf(-z - kLog256))
+                        : __fdividef(1.f, 1.f + __expf(-z));
+    *rest = 1.f - s;
+    return s;
+  }
+  const float e = exp_minus<T>(fabsf(z)), r = __fdividef(1.f, 1.f + e), er = e * r;
   *rest = z < 0.f ? r : er;
   return z < 0.f ? er : r;
 }
@@ -103,16 +112,8 @@ __device__ __forceinline__ float gelu(float z) {
   float e;
   return z * normal_cdf<T>(z, &e);
 }
-// z / (1 + exp(-z)).  The fast quotient is 0 for divisors above 2^126, which bfloat16's and
-// float32's small results would notice: bfloat16 divides both sides by 2^8 (good down to -92,
-// where silu leaves the normal numbers), at two instructions; float32 has no bits to lose
-// in the exponential's argument.
 template <typename T>
 __device__ __forceinline__ float silu(float z) {
-  constexpr float kLog256 = 5.5451774f;
-  if constexpr (std::is_same<T, __half>::value) return __fdividef(z, 1.f + __expf(-z));
-  if constexpr (std::is_same<T, bf16>::value)
-    return __fdividef(z * 0.00390625f, 0.00390625f + __expf(-z - kLog256));
   float rest;
   return z * sigmoid<T>(z, &rest);
 }
