@@ -371,7 +371,7 @@ def clip_gradients_device(device: int, tensors: Sequence[tuple], max_norm: float
 
 def trim_scratch(device: int) -> None:
     """Gives back the scratch that the learned adapters and the clipping keep on a
-    device between calls (xvec_gpu_trim_scratch)."""
+    device between calls, but for what enqueued calls still use (xvec_gpu_trim_scratch)."""
     _check(_lib.xvec_gpu_trim_scratch(device))
 
 
