@@ -142,3 +142,27 @@ def test_around_the_lengths_of_an_accumulation(xb, kind, deep):
     xb.linear_backward_device(0, STORAGE[kind], deep, n, m, ptr(wt), ptr(xt), 0, dw_ptr=ptr(dw),
                               stream=stream())
     assert bool(((dw.double() - want.t()).abs() <= bound.t()).all())
+
+
+# Enough tiles that no depth is split, depths of several accumulations, ragged tiles.
+LONG = [(9472, 2500, 1000), (5001, 4499, 1301), (9000, 6208, 515), (2600, 8195, 2304)]
+LAYOUTS = [(0, 0), (8, 0), (5, 1)]  # pad, skew
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("layout", LAYOUTS, ids=str)
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_sums_with_everything_around_them(xb, kind, shape, layout):
+    """Bias, activation, residual, saved pre-activations and their gradients in every layout; nothing
+    around the outputs is written."""
+    from test_adapter_gpu import (check_backward, check_gated, check_linear, run_gated,
+                                  run_gated_backward, run_linear, run_linear_backward)
+    i = LONG.index(shape)
+    activation = ("silu", "gelu", "relu", "none")[i]
+    n, k, m = shape
+    check_linear(*run_linear(xb, kind, *shape, activation, True, True, i % 2 == 0, *layout, seed=i), activation)
+    check_gated(*run_gated(xb, kind, n, k, m // 2, activation, i % 2 == 0, True, *layout, seed=i), activation)
+    # The backward products' depths are the rows and the output columns.
+    check_backward(kind, activation, *run_linear_backward(xb, kind, k, m, n, activation, "xwb", *layout, seed=i))
+    check_backward(kind, activation,
+                   *run_gated_backward(xb, kind, k, m, n, activation, "xgubc", *layout, seed=i))
