@@ -69,7 +69,8 @@ constexpr int kBM = 128;      // rows per CTA (TMEM lanes)
 constexpr int kBK = 64;       // depth per stage: 128 bytes, one swizzle row
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr int kBand = 8;      // row tiles per band of the tile order
-// Registers of a thread where sums are held: of the first four warps, and of the epilogue's.
+// Registers of a thread where sums are held: of the first four warps, and of the epilogue's
+// (together no more than the launch's; the host checks).
 constexpr int kFewRegs = 56;
 template <typename T>
 constexpr int kManyRegs = std::is_same<T, float>::value ? 224 : 216;
@@ -1029,8 +1030,9 @@ xvec_gpu_status launch_sums(const GemmCall& c, cudaStream_t s) {
 
 template <int MODE, typename T, bool PAIR, int BN>
 xvec_gpu_status launch_shape(const GemmCall& c, cudaStream_t s) {
-  return c.p.blocks_per_split > run_blocks(std::is_same<T, float>::value) ? launch_sums<MODE, T, PAIR, BN, true>(c, s)
-                                     : launch_sums<MODE, T, PAIR, BN, false>(c, s);
+  const bool many = c.p.blocks_per_split > run_blocks(std::is_same<T, float>::value);
+  return many ? launch_sums<MODE, T, PAIR, BN, true>(c, s)
+              : launch_sums<MODE, T, PAIR, BN, false>(c, s);
 }
 
 template <int MODE, typename T>
